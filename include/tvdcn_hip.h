@@ -197,6 +197,89 @@ tvdcn_status tvdcn_to_channels_last(int32_t dtype, int64_t batch, int64_t channe
 tvdcn_status tvdcn_from_channels_last(int32_t dtype, int64_t batch, int64_t channels, int64_t spatial_numel,
                                       const void *input, void *output, void *stream);
 
+/*
+ * Operators on channels-last maps: rows x channels, contiguous, with rows = batch x pixels (a
+ * (batch, channels, *size) tensor in channels-last memory, or a (rows, channels) matrix). No
+ * counterpart in the reference; they stand next to its layers in a model. float32, float16 and
+ * bfloat16; float64 is TVDCN_STATUS_NOT_SUPPORTED. Parameters have the map's type. Pointers are
+ * 16-byte aligned, workspaces too; at most 2^20 channels. Sums, statistics and products are held
+ * in float32 and every result is rounded once. Results do not change from call to call.
+ */
+typedef enum {
+    TVDCN_ACT_NONE = 0,
+    TVDCN_ACT_RELU = 1,
+    TVDCN_ACT_SILU = 2,   /* z * sigmoid(z) */
+    TVDCN_ACT_GELU = 3    /* z * Phi(z), Phi the normal distribution function */
+} tvdcn_activation;
+
+/*
+ * 8-bit maps. For every block of 32 channels of a row (the last one may be shorter) one exponent
+ * byte, k + 127 with k the least integer >= -126 for which max |x| <= 127 * 2^k, and for every
+ * value the code q = x / 2^k rounded to the nearest integer, ties to even. The code stands for
+ * q * 2^k, clamped to the finite values of the map's type. A block that holds an infinity or a NaN
+ * has the byte 255 and comes back as NaN. codes: rows x channels; exponents: rows x
+ * ceil(channels / 32).
+ */
+tvdcn_status tvdcn_compress_activation(int32_t dtype, int64_t rows, int64_t channels, const void *input, int8_t *codes,
+                                       uint8_t *exponents, void *stream);
+tvdcn_status tvdcn_expand_activation(int32_t dtype, int64_t rows, int64_t channels, const int8_t *codes,
+                                     const uint8_t *exponents, void *output, void *stream);
+
+/*
+ * Group normalisation, affine map and activation: y = act(weight * (x - mean) * rstd + bias), mean
+ * and rstd = 1 / sqrt(variance + eps) over the pixels and the channels / groups channels of each
+ * (image, group); weight and bias may be NULL (1 and 0). mean and rstd (batch x groups, float32)
+ * are written by the forward and read by the backward. In the backward the input may be given as
+ * its 8-bit map instead (input NULL, codes and exponents not). grad_input, grad_weight and
+ * grad_bias may be NULL (not computed).
+ */
+typedef struct {
+    int32_t dtype;       /* tvdcn_dtype */
+    int32_t activation;  /* tvdcn_activation */
+    int64_t batch;
+    int64_t pixels;      /* of an image */
+    int64_t channels;
+    int64_t groups;
+    double eps;
+} tvdcn_norm_desc;
+size_t tvdcn_group_norm_act_forward_workspace_size(const tvdcn_norm_desc *desc);
+size_t tvdcn_group_norm_act_backward_workspace_size(const tvdcn_norm_desc *desc);
+tvdcn_status tvdcn_group_norm_act_forward(const tvdcn_norm_desc *desc, const void *input, const void *weight,
+                                          const void *bias, void *output, float *mean, float *rstd, void *workspace,
+                                          size_t workspace_bytes, void *stream);
+tvdcn_status tvdcn_group_norm_act_backward(const tvdcn_norm_desc *desc, const void *grad_out, const void *input,
+                                           const int8_t *codes, const uint8_t *exponents, const void *weight,
+                                           const void *bias, const float *mean, const float *rstd, void *grad_input,
+                                           void *grad_weight, void *grad_bias, void *workspace, size_t workspace_bytes,
+                                           void *stream);
+
+/*
+ * The pointwise convolution: y = act(z) + residual, z = x weight^T + bias over the channels of
+ * every row; weight (out_channels x in_channels), bias and residual (rows x out_channels) may be
+ * NULL. pre (rows x out_channels, may be NULL) receives z. The backward takes z as pre wherever
+ * the activation is not TVDCN_ACT_NONE (TVDCN_ACT_RELU: a tensor that is positive where z is, as y
+ * is without a residual) and the input as such or as its 8-bit map (input NULL, codes and exponents
+ * not; kept_int8 = 1 in the workspace query). grad_input, grad_weight and grad_bias may be NULL
+ * (not computed); the residual's gradient is grad_out itself. float32 products take three bfloat16
+ * pieces per value: an infinite operand may give a NaN.
+ */
+typedef struct {
+    int32_t dtype;       /* tvdcn_dtype */
+    int32_t activation;  /* tvdcn_activation */
+    int64_t rows;
+    int64_t in_channels;
+    int64_t out_channels;
+} tvdcn_pointwise_desc;
+size_t tvdcn_pointwise_conv_forward_workspace_size(const tvdcn_pointwise_desc *desc);
+size_t tvdcn_pointwise_conv_backward_workspace_size(const tvdcn_pointwise_desc *desc, int32_t kept_int8);
+tvdcn_status tvdcn_pointwise_conv_forward(const tvdcn_pointwise_desc *desc, const void *input, const void *weight,
+                                          const void *bias, const void *residual, void *output, void *pre,
+                                          void *workspace, size_t workspace_bytes, void *stream);
+tvdcn_status tvdcn_pointwise_conv_backward(const tvdcn_pointwise_desc *desc, const void *grad_out, const void *input,
+                                           const int8_t *codes, const uint8_t *exponents, const void *weight,
+                                           const void *pre, void *grad_input, void *grad_weight, void *grad_bias,
+                                           void *workspace, size_t workspace_bytes, void *stream);
+
 /* Thread-local text of the last error (empty string when none). */
 const char *tvdcn_last_error(void);
 
@@ -221,7 +304,10 @@ enum {
     TVDCN_KERNEL_WEIGHT_GRAD = 3,   /* re-gather + MFMA weight gradient */
     TVDCN_KERNEL_BIAS_GRAD = 4,
     TVDCN_KERNEL_MASK_SOFTMAX = 5,
-    TVDCN_KERNEL_FAMILIES = 6
+    TVDCN_KERNEL_GROUP_NORM = 6,
+    TVDCN_KERNEL_POINTWISE = 7,
+    TVDCN_KERNEL_INT8_MAP = 8,      /* 8-bit maps, compress and expand */
+    TVDCN_KERNEL_FAMILIES = 9
 };
 void tvdcn_kernel_timer_enable(int32_t enable);
 tvdcn_status tvdcn_kernel_timer_read(int32_t family, double *total_ms, int64_t *launches);

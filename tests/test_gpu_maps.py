@@ -1,0 +1,408 @@
+"""The operators on channels-last maps on the GPU, against their definitions in float64 (map_reference.py): every type,
+activation and direction, channel counts of any kind, grids of none to three axes down to single pixels, other
+memory orders, streams, graphs, and maps beyond 32-bit offsets."""
+import pytest
+import torch
+
+import tvdcn
+from map_reference import ACTIVATIONS, as_map, as_rows, check, kept, make, norm, pointwise, value
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def leaf(t):
+    return None if t is None else t.detach().requires_grad_(True)
+
+
+def run_norm(x, groups, w, b, act, dy, eps=1e-5, keep=False):
+    x, w, b = leaf(x), leaf(w), leaf(b)
+    y = tvdcn.group_norm_act(x, groups, w, b, eps, act, keep)
+    grads = torch.autograd.grad(y, [t for t in (x, w, b) if t is not None], dy)
+    return [y, *grads]
+
+
+def run_pointwise(x, w, b, r, act, dy, keep=False):
+    x, w, b, r = leaf(x), leaf(w), leaf(b), leaf(r)
+    y = tvdcn.pointwise_conv(x, w, b, r, act, keep)
+    grads = torch.autograd.grad(y, [t for t in (x, w, b, r) if t is not None], dy)
+    if r is not None:
+        assert torch.equal(grads[-1], dy)
+        grads = grads[:-1]
+    return [y, *grads]
+
+
+def norm_case(shape, dtype, seed=0, **kw):
+    c = shape[1]
+    return (make(shape, dtype, seed, **kw), make((c,), dtype, seed + 1, spread=0.3, shift=1.0),
+            make((c,), dtype, seed + 2, spread=0.3), make(shape, dtype, seed + 3))
+
+
+NORM_SHAPES = [
+    ((2, 8, 5, 3), 2), ((1, 3, 7), 1), ((3, 63, 11, 13), 7), ((2, 72, 9, 9), 9), ((1, 256, 33, 31), 32), ((37, 48), 3),
+    ((1, 40, 1), 1), ((2, 5, 3, 2, 7), 5), ((1, 2064, 3, 2), 3), ((2, 2100, 5), 2), ((1, 1, 600), 1), ((5, 260, 70), 130),
+    ((1000, 16, 2), 2),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape,groups", NORM_SHAPES)
+def test_norm(shape, groups, dtype):
+    for i, act in enumerate(ACTIVATIONS):
+        x, w, b, dy = norm_case(shape, dtype, seed=10 * i)
+        check(run_norm(x, groups, w, b, act, dy), norm(x, groups, w, b, 1e-5, act, dy), (shape, act))
+    with torch.no_grad():
+        check([tvdcn.group_norm_act(x, groups)], norm(x, groups, None, None, 1e-5, "none"), shape)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape,groups", [((2, 64, 9, 7), 4), ((3, 63, 40), 7), ((1, 36, 5, 5), 3)])
+def test_norm_kept_in_8_bits(shape, groups, dtype):
+    for act in ACTIVATIONS:
+        x, w, b, dy = norm_case(shape, dtype, seed=5)
+        got = run_norm(x, groups, w, b, act, dy, keep=True)
+        check(got, norm(x, groups, w, b, 1e-5, act, dy, keep_int8=True), (shape, act))
+        assert torch.equal(got[0], tvdcn.group_norm_act(x, groups, w, b, 1e-5, act))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_norm_of_large_means_and_constant_groups(dtype):
+    """A mean of 40 spreads does not cancel; a group of one value everywhere is its bias, whatever eps > 0."""
+    x, w, b, dy = norm_case((2, 32, 17, 19), dtype, shift=40.0)
+    check(run_norm(x, 4, w, b, "silu", dy), norm(x, 4, w, b, 1e-5, "silu", dy))
+    flat = torch.full_like(x, 3.0)
+    y = tvdcn.group_norm_act(flat, 4, w, b)
+    assert torch.equal(y, b.view(1, -1, 1, 1).expand_as(y))
+
+
+def test_norm_values_that_are_not_finite_stay_in_their_group():
+    x, w, b, dy = norm_case((2, 32, 9, 9), torch.float32)
+    ref = tvdcn.group_norm_act(x, 4, w, b, 1e-5, "silu")
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        z = x.clone(memory_format=torch.preserve_format)
+        z[1, 9, 4, 4] = bad
+        y = tvdcn.group_norm_act(z, 4, w, b, 1e-5, "silu")
+        assert not torch.isfinite(y[1, 8:16]).any()
+        y[1, 8:16] = ref[1, 8:16]
+        assert torch.equal(y, ref)
+
+
+POINT_SHAPES = [   # map, out channels
+    ((1, 8), 8), ((1, 256), 1024), ((7, 64), 40), ((2, 3, 5, 3), 5), ((3, 71, 13, 11), 101), ((1, 256, 25, 38), 256),
+    ((2, 96, 40, 33), 130), ((1, 130, 129), 64), ((1, 1, 300), 1), ((2, 7, 3, 4, 5), 200), ((1, 520, 65), 72), ((4, 64, 1000), 136),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape,out", POINT_SHAPES)
+def test_pointwise(shape, out, dtype):
+    for i, act in enumerate(ACTIVATIONS):
+        x = make(shape, dtype, i)
+        w = make((out, shape[1]), dtype, i + 1, spread=shape[1] ** -0.5)
+        b = make((out,), dtype, i + 2, spread=0.3) if i % 2 == 0 else None
+        r = make((shape[0], out, *shape[2:]), dtype, i + 3) if i in (1, 2) else None
+        dy = make((shape[0], out, *shape[2:]), dtype, i + 4)
+        want = pointwise(x, w, b, r, act, dy)
+        check(run_pointwise(x, w, b, r, act, dy), want[:3] + (want[3:] if b is not None else []), (shape, out, act))
+        with torch.no_grad():
+            check([tvdcn.pointwise_conv(x, w, b, r, act)], want[:1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape,out", [((2, 64, 9, 7), 48), ((3, 71, 130), 33), ((1, 36, 5, 5), 8)])
+def test_pointwise_kept_in_8_bits(shape, out, dtype):
+    for act in ACTIVATIONS:
+        x, w = make(shape, dtype, 1), make((out, shape[1]), dtype, 2, spread=shape[1] ** -0.5)
+        b, dy = make((out,), dtype, 3), make((shape[0], out, *shape[2:]), dtype, 4)
+        got = run_pointwise(x, w, b, None, act, dy, keep=True)
+        check(got, pointwise(x, w, b, None, act, dy, keep_int8=True), (shape, act))
+        for g, r in zip(got[:2], run_pointwise(x, w, b, None, act, dy)):
+            assert torch.equal(g, r)
+
+
+def test_pointwise_float32_is_float32_accurate():
+    """The pieces and their six products: independent roundings leave about sqrt(6 K / 32) last bits, 6e-7 at K = 600."""
+    x, w = make((1, 600, 400), torch.float32, 1), make((192, 600), torch.float32, 2)
+    dy = make((1, 192, 400), torch.float32, 3)
+    for g, (r, _) in zip(run_pointwise(x, w, None, None, "none", dy), pointwise(x, w, None, None, "none", dy)):
+        assert (g.double() - r).norm() / r.norm() < 2e-6
+    big = torch.tensor([[3.4e38, 1e-3, 1.0, 0, 0, 0, 0, 0]], device="cuda")
+    assert torch.equal(tvdcn.pointwise_conv(big, torch.eye(8, device="cuda")), big)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_only_the_gradients_asked_for(dtype):
+    x, w, b = make((2, 24, 9), dtype, 1), make((16, 24), dtype, 2), make((16,), dtype, 3)
+    dy = make((2, 16, 9), dtype, 4)
+    full = run_pointwise(x, w, b, None, "gelu", dy)
+    for i in range(3):
+        ts = [x, w, b]
+        ts[i] = leaf(ts[i])
+        y = tvdcn.pointwise_conv(*ts, activation="gelu")
+        assert torch.equal(torch.autograd.grad(y, ts[i], dy)[0], full[1 + i])
+    g, s, dx = make((24,), dtype, 5), make((24,), dtype, 6), make((2, 24, 9), dtype, 7)
+    full = run_norm(x, 3, g, s, "silu", dx)
+    for i in range(3):
+        ts = [x, g, s]
+        ts[i] = leaf(ts[i])
+        y = tvdcn.group_norm_act(ts[0], 3, ts[1], ts[2], activation="silu")
+        assert torch.equal(torch.autograd.grad(y, ts[i], dx)[0], full[1 + i])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(2, 64, 9, 7), (3, 71, 40), (1, 33), (5, 3, 2, 3, 4), (1, 1024, 31)])
+def test_round_trip(shape, dtype):
+    for spread in (1.0, 1e-6, 300.0):
+        x = make(shape, dtype, 1, spread=spread)
+        x[..., 0] = 0
+        codes, exps = tvdcn.compress_activation(x)
+        assert codes.shape == x.shape and exps.shape[1] == (shape[1] + 31) // 32
+        back = tvdcn.expand_activation(codes, exps, dtype)
+        assert back.shape == x.shape and torch.equal(back.double(), as_map(kept(as_rows(x.double()), dtype), x, shape[1]))
+        # the host's form is the same to the bit
+        for a, b in zip((codes, exps), tvdcn.compress_activation(x.cpu())):
+            assert torch.equal(a.cpu(), b)
+        assert torch.equal(tvdcn.expand_activation(codes.cpu(), exps.cpu(), dtype), back.cpu())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_round_trip_at_the_ends_of_the_range(dtype):
+    info = torch.finfo(dtype)
+    x = torch.zeros(6, 64, dtype=dtype, device="cuda")
+    x[0, 0], x[0, 1] = info.max, -info.max
+    x[1, 3], x[1, 40] = info.tiny, info.tiny * info.eps
+    x[2, 5], x[2, 6] = float("inf"), 1.0
+    x[3, 33] = float("nan")
+    x[4, 0], x[4, 1], x[4, 2], x[4, 3] = 127.0, 0.5, 1.5, -2.5     # ties to even
+    x[5, 0], x[5, 1] = 127.5, 1.0                                    # above 127 steps: the next exponent
+    codes, exps = tvdcn.compress_activation(x)
+    back = tvdcn.expand_activation(codes, exps, dtype)
+    want = kept(x.double(), dtype).to(dtype)
+    assert torch.equal(torch.isnan(back), torch.isnan(want)) and torch.equal(back.nan_to_num(0), want.nan_to_num(0))
+    assert back[4, :4].tolist() == [127.0, 0.0, 2.0, -2.0] and exps[2, 0] == 255 and exps[2, 1] == 1
+    for a, b in zip((codes, exps), tvdcn.compress_activation(x.cpu())):
+        assert torch.equal(a.cpu(), b)
+
+
+def test_memory_orders_and_alignment():
+    """Contiguous, sliced, offset and expanded tensors give what their channels-last copies give, to the bit."""
+    base = make((2, 48, 6, 10), torch.float16, 1)
+    w, b = make((32, 48), torch.float16, 2), make((32,), torch.float16, 3)
+    g, s = make((48,), torch.float16, 4), make((48,), torch.float16, 5)
+    pad = make((2, 50, 6, 11), torch.float16, 6)
+    odd = torch.empty(base.numel() + 1, dtype=torch.float16, device="cuda")[1:].view(2, 6, 10, 48).movedim(-1, 1)
+    odd.copy_(base)
+    for x in (base.contiguous(), base.transpose(2, 3), pad[:, 1:49, :, 1:], odd, base[:1].expand(3, -1, -1, -1)):
+        y = x.movedim(1, -1).contiguous().movedim(-1, 1)
+        dy = torch.ones((), dtype=torch.float16, device="cuda").expand(x.shape[0], 32, *x.shape[2:])
+        for p, q in zip(run_pointwise(x, w, b, None, "silu", dy), run_pointwise(y, w, b, None, "silu", dy.contiguous())):
+            assert torch.equal(p, q)
+        dx = pad[:1, :48, :1, :1].expand(x.shape)
+        for p, q in zip(run_norm(x, 4, g, s, "gelu", dx), run_norm(y, 4, g, s, "gelu", dx.contiguous())):
+            assert torch.equal(p, q)
+        for p, q in zip(tvdcn.compress_activation(x), tvdcn.compress_activation(y)):
+            assert torch.equal(p, q)
+    wt = make((48, 32), torch.float16, 7).t()
+    assert torch.equal(tvdcn.pointwise_conv(base, wt[:, :, None, None]), tvdcn.pointwise_conv(base, wt.contiguous()))
+
+
+def test_empty_maps():
+    for shape in ((0, 16, 4, 4), (2, 16, 0, 4), (0, 16)):
+        x = torch.empty(shape, device="cuda", requires_grad=True)
+        w = torch.randn(8, 16, device="cuda", requires_grad=True)
+        b = torch.randn(8, device="cuda", requires_grad=True)
+        y = tvdcn.pointwise_conv(x, w, b, None, "gelu")
+        y.sum().backward()
+        assert y.shape == (shape[0], 8, *shape[2:]) and x.grad.shape == shape
+        assert not w.grad.any() and not b.grad.any()
+        g = torch.randn(16, device="cuda", requires_grad=True)
+        s = torch.randn(16, device="cuda", requires_grad=True)
+        y = tvdcn.group_norm_act(x, 4, g, s)
+        y.sum().backward()
+        assert y.shape == shape and not g.grad.any() and not s.grad.any()
+        codes, exps = tvdcn.compress_activation(x.detach())
+        assert tvdcn.expand_activation(codes, exps, torch.float32).shape == shape
+
+
+def block(x, p, keep):
+    """convolution, normalisation and activation, projection added to the input: as a model runs them"""
+    y = tvdcn.deform_conv2d(x, p["cw"], p["co"], padding=1)
+    y = tvdcn.group_norm_act(y, 4, p["g"], p["s"], activation="silu", keep_int8=keep)
+    return tvdcn.pointwise_conv(y, p["w"], p["b"], x, "gelu", keep)
+
+
+def block_params(seed, dtype=torch.float32, c=32):
+    k = dict(cw=make((c, c, 3, 3), dtype, seed, spread=0.08), co=make((2, 18, 12, 10), dtype, seed + 1),
+             g=make((c,), dtype, seed + 2, shift=1.0), s=make((c,), dtype, seed + 3), w=make((c, c), dtype, seed + 4, spread=0.2),
+             b=make((c,), dtype, seed + 5))
+    return {n: leaf(t.contiguous()) for n, t in k.items()}
+
+
+@pytest.mark.parametrize("keep", [False, True])
+def test_block_of_all_three(keep):
+    """The operators together behind a deformable convolution: each one's result and gradients against float64 on the
+    values that it was given."""
+    p, x = block_params(1), leaf(make((2, 32, 12, 10), torch.float32, 20))
+    conv = tvdcn.deform_conv2d(x, p["cw"], p["co"], padding=1)
+    a = leaf(conv)
+    n = tvdcn.group_norm_act(a, 4, p["g"], p["s"], activation="silu", keep_int8=keep)
+    m, r = leaf(n), leaf(x)
+    y = tvdcn.pointwise_conv(m, p["w"], p["b"], r, "gelu", keep)
+    dy = make(y.shape, torch.float32, 30)
+    dm, dw, db, dr = torch.autograd.grad(y, [m, p["w"], p["b"], r], dy)
+    check([y, dm, dw, db], pointwise(m.detach(), p["w"].detach(), p["b"].detach(), x.detach(), "gelu", dy, keep))
+    da, dg, ds = torch.autograd.grad(n, [a, p["g"], p["s"]], dm)
+    check([n, da, dg, ds], norm(a.detach(), 4, p["g"].detach(), p["s"].detach(), 1e-5, "silu", dm, keep))
+    dx = torch.autograd.grad(conv, [x, p["cw"]], da)
+    # in one graph: the same to the bit but for the convolution's own gradients, whose sums have no fixed order
+    y2 = block(x, p, keep)
+    got = torch.autograd.grad(y2, [x, p["cw"], p["g"], p["s"], p["w"], p["b"]], dy)
+    assert torch.equal(y2, y)
+    for g, want in zip(got[2:], (dg, ds, dw, db)):
+        assert torch.equal(g, want)
+    for g, want in zip(got[:2], (dx[0] + dr, dx[1])):
+        assert (g - want).norm() <= 1e-5 * want.norm()
+
+
+def test_gradients_against_differences():
+    """Directional derivatives of the block's loss in float32 against central differences of its float64 form."""
+    x, w, b = make((2, 24, 5, 4), torch.float32, 1), make((16, 24), torch.float32, 2, spread=0.2), make((16,), torch.float32, 3)
+    g, s = make((24,), torch.float32, 4, shift=1.0), make((24,), torch.float32, 5)
+    t = make((2, 16, 5, 4), torch.float32, 6)
+    ts = [leaf(v) for v in (x, g, s, w, b)]
+    y = tvdcn.pointwise_conv(tvdcn.group_norm_act(ts[0], 3, ts[1], ts[2], activation="gelu"), ts[3], ts[4], None, "silu")
+    grads = torch.autograd.grad(y, ts, t)
+
+    def loss(v):
+        n = norm(v[0], 3, v[1], v[2], 1e-5, "gelu")[0][0]
+        return (value(as_rows(n) @ v[3].t() + v[4], "silu") * as_rows(t.double())).sum()
+
+    d64 = [v.double() for v in (x, g, s, w, b)]
+    for i in range(5):
+        d = make(d64[i].shape, torch.float64, 50 + i)
+        h = 1e-5
+        up, down = list(d64), list(d64)
+        up[i], down[i] = d64[i] + h * d, d64[i] - h * d
+        want = (loss(up) - loss(down)) / (2 * h)
+        # a second-order difference leaves about h^2 of the third derivative; float32 gradients 1e-6 of each term
+        scale = (grads[i].double() * d).abs().sum()
+        assert abs((grads[i].double() * d).sum() - want) <= 1e-5 * scale + 1e-6
+
+
+def test_results_do_not_change_from_call_to_call():
+    x, w, b = make((4, 128, 40, 40), torch.bfloat16, 1), make((256, 128), torch.bfloat16, 2), make((256,), torch.bfloat16, 3)
+    dy, dx = make((4, 256, 40, 40), torch.bfloat16, 4), make((4, 128, 40, 40), torch.bfloat16, 5)
+    g, s = make((128,), torch.bfloat16, 6), make((128,), torch.bfloat16, 7)
+    a, c = run_pointwise(x, w, b, None, "gelu", dy), run_norm(x, 8, g, s, "gelu", dx)
+    for _ in range(3):
+        for p, q in zip(a + c, run_pointwise(x, w, b, None, "gelu", dy) + run_norm(x, 8, g, s, "gelu", dx)):
+            assert torch.equal(p, q)
+
+
+def test_streams():
+    """Calls on two streams at once, each on its own stream's data."""
+    sets = [[make((4, 64, 30, 31), torch.float16, 10 * i), make((96, 64), torch.float16, 10 * i + 1),
+             make((64,), torch.float16, 10 * i + 2)] for i in range(2)]
+
+    def go(x, w, g):
+        y = tvdcn.group_norm_act(x, 4, g, None, activation="relu", keep_int8=True)
+        return tvdcn.pointwise_conv(y, w, None, None, "silu", True)
+
+    want = [go(*s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(go(*sets[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, want[i]) for g in got[i])
+
+
+@pytest.mark.parametrize("keep", [False, True])
+def test_graph(keep):
+    """Forward and backward captured and replayed on new inputs, with eager calls between, against the eager results."""
+    dtype = torch.bfloat16
+    x, dy = make((2, 64, 24, 20), dtype, 1), make((2, 96, 24, 20), dtype, 2)
+    ps = [make((64,), dtype, 3, shift=1.0), make((64,), dtype, 4), make((96, 64), dtype, 5, spread=0.1), make((96,), dtype, 6)]
+
+    def step(x, dy, ps):
+        x, *ps = [leaf(t) for t in (x, *ps)]
+        y = tvdcn.group_norm_act(x, 4, ps[0], ps[1], activation="silu", keep_int8=keep)
+        y = tvdcn.pointwise_conv(y, ps[2], ps[3], None, "gelu", keep)
+        return [y.detach(), *torch.autograd.grad(y, [x, *ps], dy)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(x, dy, ps)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(x, dy, ps)
+    for seed in (100, 200, 300):
+        nx, ndy = make(x.shape, dtype, seed), make(dy.shape, dtype, seed + 1)
+        want = step(nx, ndy, ps)
+        x.copy_(nx)
+        dy.copy_(ndy)
+        graph.replay()
+        torch.cuda.synchronize()
+        for g, r in zip(out, want):
+            assert torch.equal(g, r)
+
+
+def test_autocast():
+    x, w, b = make((2, 32, 9, 9), torch.float32, 1), make((16, 32), torch.float32, 2), make((16,), torch.float32, 3)
+    g = make((32,), torch.float32, 4)
+    with torch.autocast("cuda", torch.bfloat16):
+        y = tvdcn.pointwise_conv(x, w, b, None, "gelu")
+        n = tvdcn.group_norm_act(y.new_ones(2, 32, 9), 4, g)
+        f = tvdcn.group_norm_act(x, 4, g)
+    bf = [t.bfloat16() for t in (x, w, b)]
+    assert y.dtype == torch.bfloat16 and torch.equal(y, tvdcn.pointwise_conv(*bf, None, "gelu"))
+    assert n.dtype == torch.bfloat16 and f.dtype == torch.float32 and torch.equal(f, tvdcn.group_norm_act(x, 4, g))
+
+
+def test_maps_beyond_32_bit_offsets():
+    """More than 2^31 values: the last rows of each result against float64, and the first."""
+    rows, c = 4200000, 520
+    gen = torch.Generator("cuda").manual_seed(1)
+    x = torch.randn(rows, c, generator=gen, device="cuda", dtype=torch.bfloat16)
+    w = torch.randn(24, c, generator=gen, device="cuda").mul_(c ** -0.5).bfloat16()
+    y = tvdcn.pointwise_conv(x, w)
+    for part in (slice(0, 300), slice(rows - 300, rows)):
+        check([y[part]], pointwise(x[part], w, None, None, "none"))
+    # the gradient of a wide map: the weight's is of a few rows that have one
+    dy = torch.zeros(rows, 24, device="cuda", dtype=torch.bfloat16)
+    dy[-200:] = torch.randn(200, 24, generator=gen, device="cuda").bfloat16()
+    xs, ws = leaf(x), leaf(w)
+    dx, dw = torch.autograd.grad(tvdcn.pointwise_conv(xs, ws), [xs, ws], dy)
+    want = pointwise(x[-200:], w, None, None, "none", dy[-200:])
+    check([dx[-200:], dw], want[1:3])
+    assert not dx[:-200].any()
+    del dx, y, xs
+    codes, exps = tvdcn.compress_activation(x)
+    part = slice(rows - 300, rows)
+    assert torch.equal(tvdcn.expand_activation(codes, exps, x.dtype)[part].double(), kept(x[part].double(), x.dtype))
+    del codes, exps
+    # rows as images of one pixel: each its own statistics
+    y = tvdcn.group_norm_act(x, 5)
+    for part in (slice(0, 100), slice(rows - 100, rows)):
+        check([y[part]], norm(x[part], 5, None, None, 1e-5, "none"))
+    # one image: the statistics of all of them
+    one = x.view(1, rows, c).movedim(-1, 1)
+    y = tvdcn.group_norm_act(one, 5)[0].t()
+    mean, var = (torch.zeros(5, 1, dtype=torch.float64, device="cuda") for _ in range(2))
+    for i in range(0, rows, 100000):
+        v = x[i:i + 100000].double().view(-1, 5, c // 5)
+        mean += v.sum((0, 2)).view(5, 1)
+        var += v.square().sum((0, 2)).view(5, 1)
+    n = rows * c // 5
+    mean, var = mean / n, var / n - (mean / n).square()
+    tail = x[-100:].double().view(-1, 5, c // 5)
+    ref = ((tail - mean) / (var + 1e-5).sqrt()).view(100, c)
+    # half a step of bfloat16, and the float32 statistics
+    assert ((y[-100:].double() - ref).abs() <= 2.0 ** -8 * ref.abs() + 1e-4).all()

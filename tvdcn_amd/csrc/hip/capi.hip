@@ -15,6 +15,7 @@
 #include <vector>
 
 #include "../../../include/tvdcn_hip.h"
+#include "capi.h"
 #include "kernels.h"
 
 using namespace tvdcn_hip;
@@ -967,6 +968,17 @@ tvdcn_status scratch_of_current_device(void **out) {
 }
 
 }  // namespace
+
+namespace tvdcn_hip {
+
+tvdcn_status api_fail(tvdcn_status st, const std::string &msg) { return fail(st, msg); }
+void api_clear_error() { g_last_error.clear(); }
+tvdcn_status api_launch(int family, hipStream_t s, const std::function<hipError_t()> &launch) {
+    TVDCN_LAUNCH(family, s, launch());
+    return TVDCN_STATUS_SUCCESS;
+}
+
+}  // namespace tvdcn_hip
 
 extern "C" {
 

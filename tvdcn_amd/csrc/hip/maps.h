@@ -1,0 +1,132 @@
+// Operators on channels-last maps, [rows][channels] with rows = batch x pixels: group normalisation with
+// activation, the pointwise convolution and 8-bit activations. Shared host and device definitions.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../../include/tvdcn_hip.h"
+
+namespace tvdcn_hip {
+
+typedef float fvec4 __attribute__((ext_vector_type(4)));
+
+// 8-bit maps: channels per block of one exponent, its bias in the stored byte, and the byte of a block that held a
+// value that is not finite
+constexpr int kKeptBlock = 32;
+constexpr int kKeptBias = 127;
+constexpr int kKeptNaN = 255;
+
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
+
+// ---- launchers (group_norm.hip, kept_maps.hip, pointwise.hip): asynchronous on `s`, nothing allocated ----
+
+struct NormArgs {
+    int dtype, act;
+    int64_t batch, pixels;   // pixels per image
+    int channels, groups;
+    float eps;
+    const void *x;           // [batch][pixels][channels], or null where the 8-bit form stands in for it
+    const int8_t *codes;
+    const uint8_t *exps;
+    const void *weight, *bias;   // [channels] or null
+    void *y;
+    float *mean, *rstd;          // [batch][groups]
+    const void *dy;
+    void *dx, *dweight, *dbias;
+    float *part;                 // workspace
+};
+int64_t norm_part_floats(const NormArgs &a, bool backward);
+hipError_t launch_norm_forward(const NormArgs &a, hipStream_t s);
+hipError_t launch_norm_backward(const NormArgs &a, hipStream_t s);
+
+hipError_t launch_compress(int dtype, int64_t rows, int channels, const void *x, int8_t *codes, uint8_t *exps,
+                           hipStream_t s);
+// the values into rows of `pitch` elements, zero beyond the channels; as_bf16: bfloat16 whatever the map's type
+hipError_t launch_expand(int dtype, bool as_bf16, int64_t rows, int channels, int64_t pitch, const int8_t *codes,
+                         const uint8_t *exps, void *y, hipStream_t s);
+
+struct PointwiseArgs {
+    int dtype, act;
+    int64_t rows;
+    int in, out;
+    const void *x, *weight, *bias, *residual;
+    void *y, *pre;               // pre: the activation's argument, kept for the backward (or null)
+    const void *dy;
+    const int8_t *codes;
+    const uint8_t *exps;
+    void *dx, *dweight, *dbias;
+    char *work;
+};
+size_t pointwise_forward_bytes(const PointwiseArgs &a);
+size_t pointwise_backward_bytes(const PointwiseArgs &a);
+hipError_t launch_pointwise_forward(const PointwiseArgs &a, hipStream_t s);
+hipError_t launch_pointwise_backward(const PointwiseArgs &a, hipStream_t s);
+
+// ---- device helpers ----
+
+typedef __bf16 bf16;
+typedef _Float16 f16;
+
+// N elements in one access (in 16-byte ones where they are more)
+template <typename T, int N> struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Pack {
+    T v[N];
+};
+
+// Activations. The argument is float32; ERF32: the error function to float32's last bits, otherwise to 1.5e-7
+// (Abramowitz and Stegun 7.1.26: erfc(u) = e^(-u^2) t (a1 + t (a2 + ...)), t = 1 / (1 + p u)), well under a half step
+// of the 16-bit types whose results it serves, at a third of the instructions.
+__device__ __forceinline__ float normal_cdf_poly(float z, float gauss) {   // gauss = e^(-z^2/2)
+    const float u = fabsf(z) * 0.70710678118654752f;
+    const float t = __frcp_rn(1.f + 0.3275911f * u);
+    const float tail =
+        0.5f * gauss * t *
+        (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+    return z < 0.f ? tail : 1.f - tail;
+}
+template <bool ERF32> __device__ __forceinline__ float normal_cdf(float z, float gauss) {
+    return ERF32 ? 0.5f * erfcf(-z * 0.70710678118654752f) : normal_cdf_poly(z, gauss);
+}
+template <bool PRECISE> __device__ __forceinline__ float exp32(float v) { return PRECISE ? expf(v) : __expf(v); }
+
+template <bool PRECISE> __device__ __forceinline__ float act_value(float z, int act) {
+    switch (act) {
+        case TVDCN_ACT_RELU: return z < 0.f ? 0.f : z;   // (a NaN stays one)
+        case TVDCN_ACT_SILU: return z / (1.f + exp32<PRECISE>(-z));
+        case TVDCN_ACT_GELU: return z * normal_cdf<PRECISE>(z, exp32<PRECISE>(-0.5f * z * z));
+        default: return z;
+    }
+}
+template <bool PRECISE> __device__ __forceinline__ float act_slope(float z, int act) {
+    switch (act) {
+        case TVDCN_ACT_RELU: return z > 0.f ? 1.f : 0.f;
+        case TVDCN_ACT_SILU: {
+            const float s = 1.f / (1.f + exp32<PRECISE>(-z));
+            return s * (1.f + z * (1.f - s));
+        }
+        case TVDCN_ACT_GELU: {
+            const float gauss = exp32<PRECISE>(-0.5f * z * z);
+            return normal_cdf<PRECISE>(z, gauss) + z * gauss * 0.39894228040143268f;
+        }
+        default: return 1.f;
+    }
+}
+
+template <typename T> constexpr bool is_f32() { return sizeof(T) == 4; }
+template <typename T> __device__ __forceinline__ float most() { return 0.f; }
+template <> __device__ __forceinline__ float most<float>() { return 3.402823466e38f; }
+template <> __device__ __forceinline__ float most<f16>() { return 65504.f; }
+template <> __device__ __forceinline__ float most<bf16>() { return 3.389531390e38f; }
+
+// What code q of exponent byte e stands for: q * 2^(e - bias) clamped to T's finite values (128 q' 2^k may pass them by
+// its rounding), NaN for a block that held a value that is not finite. The scaling is exact.
+template <typename T> __device__ __forceinline__ float kept_scale(uint8_t e) {
+    return e == kKeptNaN ? __builtin_nanf("") : __uint_as_float((uint32_t)e << 23);
+}
+template <typename T> __device__ __forceinline__ float kept_value(int8_t q, float scale) {
+    const float v = (float)q * scale;
+    return v != v ? v : fminf(fmaxf(v, -most<T>()), most<T>());
+}
+
+}  // namespace tvdcn_hip

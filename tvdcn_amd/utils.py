@@ -45,3 +45,16 @@ def _ints3(v: Union[int, Tuple[int, int, int]]) -> List[int]:
     if torch.jit.is_scripting():
         return [v[0], v[1], v[2]]
     return [int(e) for e in v]
+
+
+# the activation codes of the operators on channels-last maps (tvdcn_activation in include/tvdcn_hip.h)
+def _activation_code(activation: str) -> int:
+    if activation == "none":
+        return 0
+    if activation == "relu":
+        return 1
+    if activation == "silu":
+        return 2
+    if activation == "gelu":
+        return 3
+    raise ValueError("activation must be 'none', 'relu', 'silu' or 'gelu'. Got '{}'".format(activation))
