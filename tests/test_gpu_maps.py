@@ -108,6 +108,19 @@ def test_pointwise(shape, out, dtype):
             check([tvdcn.pointwise_conv(x, w, b, r, act)], want[:1])
 
 
+# outputs that fill the chip with the largest tiles, their last ones in part: rows, columns and reduction of all remainders
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,channels,out", [(20011, 72, 520), (33000, 264, 256), (9000, 1032, 2056), (70001, 8, 264),
+                                               (16384, 200, 1024), (40000, 520, 24)])
+def test_pointwise_of_many_pixels(rows, channels, out, dtype):
+    x = make((rows, channels), dtype, 1)
+    w = make((out, channels), dtype, 2, spread=channels ** -0.5)
+    b, r, dy = make((out,), dtype, 3), make((rows, out), dtype, 4), make((rows, out), dtype, 5)
+    check(run_pointwise(x, w, b, r, "silu", dy), pointwise(x, w, b, r, "silu", dy), (rows, channels, out))
+    with torch.no_grad():
+        check([tvdcn.pointwise_conv(x, w)], pointwise(x, w, None, None, "none"))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("shape,out", [((2, 64, 9, 7), 48), ((3, 71, 130), 33), ((1, 36, 5, 5), 8)])
 def test_pointwise_kept_in_8_bits(shape, out, dtype):

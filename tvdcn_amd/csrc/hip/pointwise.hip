@@ -1,7 +1,7 @@
 // The pointwise convolution over channels-last maps: y = act(x W^T + b) + r, and its gradients
 //   dz = dy act'(z),  dx = dz W,  dW = dz^T x,  db = sum dz.
 //
-// One matrix product kernel serves the three contractions, out[r][c] = sum_t R(r, t) C(c, t), on 16x16x32 MFMAs. An
+// Matrix product kernels serve the three contractions, out[r][c] = sum_t R(r, t) C(c, t), on 16x16x32 MFMAs. An
 // operand is either t-contiguous ([r][t]: x, W and dz in y and dx) or t-major ([t][r]: W in dx, dz and x in dW); a
 // t-major tile goes through LDS as it lies in memory and its fragments are transposed by the LDS read
 // (ds_read_b64_tr_b16), so no operand is ever transposed in memory. The operand of the output's contiguous side takes
@@ -16,6 +16,11 @@
 // float32 maps run as three bfloat16 pieces per value (exact) and the six products of pieces that reach
 // float32's precision, smallest first: 2^-24 relative to the operands' products, at a sixth of the 16-bit rate (2.6 times
 // the rate of the float32 MFMAs). An infinite operand may turn into a NaN where float32 would keep an infinity.
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
+
+#include "kernels.h"
 #include "maps.h"
 
 namespace tvdcn_hip {
@@ -28,7 +33,7 @@ typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef f16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int TB = 256;
-constexpr int BK = 64;   // reduction per staged tile
+constexpr int SHARE = 64;   // rows of the weight gradient's shares come in multiples of this
 
 __device__ __forceinline__ fvec4 mfma(const bf16x8 &a, const bf16x8 &b, const fvec4 &c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -52,7 +57,7 @@ struct Product {
     int npair;
     int8_t pr[6], pc[6];      // pieces of each product
     int rows, cols;           // of the output
-    int64_t share;            // reduction per workgroup (a multiple of BK, or all of it)
+    int64_t share;            // reduction per workgroup (a multiple of SHARE, or all of it)
     int tiles_r, tiles_c, splits;
     void *out;                // [rows][cols]; float32 sums [splits][rows][cols] where sums
     const void *bias, *residual;
@@ -71,34 +76,35 @@ __device__ __forceinline__ void load_to_lds(const u32x4 &rsrc, uint32_t offset, 
 
 template <int N> constexpr int log2_of() { return N <= 1 ? 0 : 1 + log2_of<N / 2>(); }
 
-// Stages tiles of an operand: B rows (columns of the output, or rows) x BK. Wave w of 4 issues B / 32 loads of 1 KB.
-//  t-contiguous: LDS row of 64 elements, 128 bytes, per output index; chunk j of row n at j ^ swz(n)
+// Stages tiles of an operand: B rows (columns of the output, or rows) x BK. The NW waves issue B BK / 512 loads of 1 KB.
+//  t-contiguous: LDS row of BK elements per output index; chunk j of row n at j ^ swz(n)
 //  t-major:      LDS row of B elements per t; chunk j of row t at j ^ 2 swz(t)
-template <bool TM, bool PERM, int B, int F> struct Stager {
-    static constexpr int LOADS = B / 32;
+template <bool TM, bool PERM, int B, int F, int BK, int NW> struct Stager {
+    static constexpr int LOADS = B * BK / 512 / NW, CH = (TM ? B : BK) / 8;   // chunks of an LDS row
+    static_assert(LOADS * 512 * NW == B * BK, "");
     uint32_t off[LOADS];
     bool in[LOADS];          // t-contiguous: the row exists; t-major: the columns do
     int at[LOADS];           // first reduction index of the lane's chunk
 
-    // which of 8 chunk positions a row is turned by: the 16 rows that one fragment read covers differ in it or in the
-    // row's parity (an LDS pass of 256 bytes covers two rows)
+    // Which chunk positions a row is turned by. t-contiguous: the 16 rows of one fragment read fall into different chunks
+    // of an LDS pass of 256 bytes (256 / (2 BK) rows); t-major: so do the eight rows of half a transposed read.
     static __device__ __forceinline__ int swz(int n) {
         if (TM) return (n & 3) | ((n >> 3) & 1) << 2;
+        if (BK == 32) return (PERM ? n >> log2_of<4 * F>() : n >> 2) & 3;
         if (PERM) return ((n >> 1) & 1) | ((n >> log2_of<4 * F>()) & 3) << 1;
         return (n >> 1) & 7;
     }
     __device__ __forceinline__ void init(const Operand &o, int64_t first, int wave, int lane) {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
-            const int idx = wave * LOADS + i;
+            const int e = (wave * LOADS + i) * 512 + lane * 8, row = e / (CH * 8), slot = e % (CH * 8) / 8;
             if (TM) {
-                constexpr int CH = B / 8;
-                const int t = idx * (512 / B) + lane / CH, chunk = (lane % CH) ^ ((2 * swz(t)) & (CH - 1));
-                off[i] = (uint32_t)(t * (int)o.ld + chunk * 8) * 2u;
+                const int chunk = slot ^ ((2 * swz(row)) & (CH - 1));
+                off[i] = (uint32_t)(row * (int)o.ld + chunk * 8) * 2u;
                 in[i] = first + chunk * 8 < o.width;
-                at[i] = t;
+                at[i] = row;
             } else {
-                const int row = idx * 8 + lane / 8, chunk = (lane % 8) ^ swz(row);
+                const int chunk = slot ^ swz(row);
                 off[i] = (uint32_t)(row * (int)o.ld + chunk * 8) * 2u;
                 in[i] = first + row < o.width;
                 at[i] = chunk * 8;
@@ -128,7 +134,7 @@ template <bool TM, bool PERM, int B, int F> struct Stager {
             for (int h = 0; h < 2; ++h) {
                 // 16 lanes read four rows t of 16 columns; the read hands lane r the column r of the four
                 const int t = kk * 32 + q * 8 + h * 4 + r / 4, c = origin + i * 16 + (r & 3) * 4;
-                const char *p = tile + t * (B * 2) + (((c >> 3) ^ ((2 * swz(t)) & (B / 8 - 1))) << 4) + (c & 7) * 2;
+                const char *p = tile + t * (B * 2) + (((c >> 3) ^ ((2 * swz(t)) & (CH - 1))) << 4) + (c & 7) * 2;
                 typedef __attribute__((address_space(3))) s16x4 *lds_t;
                 u.h[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)p);
             }
@@ -137,7 +143,7 @@ template <bool TM, bool PERM, int B, int F> struct Stager {
             // PERM: the MFMA's row r is output index (r / 4) 4F + 4i + r % 4, so that a lane's F fragments are 4F
             // neighbouring indexes
             const int n = origin + (PERM ? (r >> 2) * (4 * F) + i * 4 + (r & 3) : i * 16 + r);
-            return *reinterpret_cast<const typename Frag<E>::type *>(tile + n * 128 + (((kk * 4 + q) ^ swz(n)) << 4));
+            return *reinterpret_cast<const typename Frag<E>::type *>(tile + n * (BK * 2) + (((kk * 4 + q) ^ swz(n)) << 4));
         }
     }
 };
@@ -198,11 +204,11 @@ __device__ __forceinline__ void emit(const Product &p, int split, int row, int c
     }
 }
 
-// 4 waves as 2 x 2, each FR x FC fragments of 16 x 16: a tile of 32 FR rows x 32 FC columns
-template <typename E, typename T, bool RT, bool CT, int FR, int FC>
-__global__ void __launch_bounds__(TB) product_kernel(Product p) {
-    constexpr int BR = 32 * FR, BC = 32 * FC, TILE = (BR + BC) * BK * 2;
-    __shared__ __align__(1024) char smem[2 * TILE];
+// WR x WC waves, each FR x FC fragments of 16 x 16; STAGES tiles of BK along the reduction in LDS
+template <typename E, typename T, bool RT, bool CT, int WR, int WC, int FR, int FC, int BK, int STAGES, int BLOCKS>
+__global__ void __launch_bounds__(WR * WC * 64, BLOCKS * WR * WC / 4) product_kernel(Product p) {
+    constexpr int NW = WR * WC, BR = WR * 16 * FR, BC = WC * 16 * FC, TILE = (BR + BC) * BK * 2;
+    extern __shared__ __align__(1024) char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // Workgroups go to the 8 XCDs in turn; each XCD takes a run of neighbouring tiles, columns first, so that the
     // operand of the rows is read into one L2 only
@@ -215,15 +221,16 @@ __global__ void __launch_bounds__(TB) product_kernel(Product p) {
     const int64_t kbeg = split * p.share, kend = kbeg + p.share < kall ? kbeg + p.share : kall;
     const int nk = (int)((kend - kbeg + BK - 1) / BK), iters = nk * p.npair;
 
-    typedef Stager<RT, false, BR, FR> SR;
-    typedef Stager<CT, !CT, BC, FC> SC;
+    typedef Stager<RT, false, BR, FR, BK, NW> SR;
+    typedef Stager<CT, !CT, BC, FC, BK, NW> SC;
+    constexpr int LOADS = SR::LOADS + SC::LOADS;
     SR sr;
     SC sc;
     sr.init(p.R, row0, wave, lane);
     sc.init(p.C, col0, wave, lane);
     typedef __attribute__((address_space(3))) char *lds_t;
     const uint32_t lds = (uint32_t)(uintptr_t)(lds_t)smem;
-    const int wr = wave >> 1, wc = wave & 1;
+    const int wr = wave / WC, wc = wave % WC;
 
     fvec4 acc[FC][FR];
 #pragma unroll
@@ -231,19 +238,25 @@ __global__ void __launch_bounds__(TB) product_kernel(Product p) {
 #pragma unroll
         for (int j = 0; j < FR; ++j) acc[i][j] = fvec4{0.f, 0.f, 0.f, 0.f};
 
-    int pair = 0, step = 0;   // of the next tile to stage
-    auto stage = [&](int buf) {
+    int pair = 0, step = 0, to = 0, at = 0;   // the next tile to stage and its buffer; the buffer to read
+    auto stage = [&]() {
         const int64_t k0 = kbeg + (int64_t)step * BK;
-        sr.load(p.R, p.pr[pair], row0, k0, kend, lds + buf * TILE, wave);
-        sc.load(p.C, p.pc[pair], col0, k0, kend, lds + buf * TILE + BR * BK * 2, wave);
+        sr.load(p.R, p.pr[pair], row0, k0, kend, lds + to * TILE, wave);
+        sc.load(p.C, p.pc[pair], col0, k0, kend, lds + to * TILE + BR * BK * 2, wave);
         if (++step == nk) step = 0, ++pair;
+        if (++to == STAGES) to = 0;
     };
-    if (iters > 0) stage(0);
+    for (int it = 0; it < STAGES - 1 && it < iters; ++it) stage();
     for (int it = 0; it < iters; ++it) {
-        // this tile's loads have landed, and every wave has read the tile before it
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (it + 1 < iters) stage((it + 1) & 1);
-        const char *tr = smem + (it & 1) * TILE, *tc = tr + BR * BK * 2;
+        // this tile's loads have landed (those of the STAGES - 2 after it may be on their way), and every wave has read
+        // the tile before it
+        if (it + STAGES - 1 <= iters)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LOADS * (STAGES - 2)) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (it + STAGES - 1 < iters) stage();
+        const char *tr = smem + at * TILE, *tc = tr + BR * BK * 2;
+        if (++at == STAGES) at = 0;
 #pragma unroll
         for (int kk = 0; kk < BK / 32; ++kk) {
             typename Frag<E>::type a[FC], b[FR];
@@ -280,6 +293,314 @@ __global__ void __launch_bounds__(TB) product_kernel(Product p) {
                 emit<T, 4>(p, split, row, col0 + wc * 16 * FC + i * 16 + q * 4, v);
             }
         }
+    }
+}
+
+// The product in tiles of 256 x 256, for outputs that fill the chip with them: half the operand traffic of 128 x 128 tiles,
+// and that traffic, not the MFMAs, bounds those.
+//
+// Eight waves, 2 along the rows x 4 along the columns, 128 x 64 each. A stage of 64 along the reduction is cut into eight
+// sub-tiles of 8 KB (64 output indexes each), loaded by one 1 KB load per wave; LDS holds two stages. A stage is worked off
+// in four phases of 16 MFMAs: phase p takes two row fragments (rows 64 p .. 64 p + 63 of the tile, those of both wave rows)
+// against the four column fragments, which phase 0 reads and keeps in registers. A phase is a memory half (LDS reads, two
+// loads) and an MFMA half, a barrier behind each; the second wave row runs one half behind the first, so that each SIMD has
+// one wave multiplying while its other one reads.
+//
+// The loads of a stage are issued as soon as the phases that read the sub-tile's place are over, up to seven phases ahead:
+//   phase 1, 2 of stage i: columns of stage i + 2;  phase 3: rows 0..127 of stage i + 2;
+//   phase 0 of stage i + 1: rows 128..255 of stage i + 2
+// (both wave rows have then read the place: the one behind ends its reads a half before). At the end of phase 3's memory
+// half the loads issued after columns and rows 0..127 of the next stage are eight, at the end of phase 1's those after this
+// stage's rows 128..255 are ten: vmcnt(8) and vmcnt(10) there, a barrier before the first read.
+//
+// Workgroups are persistent: a tile's stages follow the last one's, the first loads of the next tile are under way while the
+// results are stored.
+template <bool TM, bool PERM> struct SubTile {
+    // the turn of an LDS row (128 bytes, 8 chunks): 16 rows of a fragment read, or the eight rows of half a transposed
+    // read, fall into different places of an LDS pass of 256 bytes
+    static __device__ __forceinline__ int swz(int n) {
+        if (TM) return (((n >> 1) & 1) | ((n >> 3) & 1) << 1) << 1;
+        if (PERM) return ((n >> 1) & 1) | ((n >> 3) & 3) << 1;
+        return (n >> 1) & 7;
+    }
+    // the byte offset of a lane's 16 bytes from the sub-tile's first element; `at`: its first reduction index
+    static __device__ __forceinline__ uint32_t offset(const Operand &o, int wave, int lane, int &at) {
+        const int row = wave * 8 + lane / 8, chunk = (lane & 7) ^ swz(row);
+        at = TM ? 0 : chunk * 8;
+        return (uint32_t)(row * (int)o.ld + chunk * 8) * 2u;
+    }
+    // 16 output indexes from `first`, reduction kk * 32 + (lane / 16) * 8 + 0..7. PERM: fragments 2i and 2i + 1 share 32, the
+    // MFMA's row r is (r / 4) 8 + r % 4 (+ 4): a lane then holds eight neighbouring indexes of theirs, four lanes 64 bytes of a
+    // 16-bit row
+    template <typename E>
+    static __device__ __forceinline__ typename Frag<E>::type frag(const char *tile, int first, int kk, int lane) {
+        const int q = lane >> 4, r = lane & 15;
+        if constexpr (TM) {
+            union {
+                s16x4 h[2];
+                typename Frag<E>::type f;
+            } u;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int t = kk * 32 + q * 8 + h * 4 + r / 4, c = first + (r & 3) * 4;
+                const char *p = tile + t * 128 + (((c >> 3) ^ swz(t)) << 4) + (c & 7) * 2;
+                typedef __attribute__((address_space(3))) s16x4 *lds_t;
+                u.h[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)p);
+            }
+            return u.f;
+        } else {
+            const int n = PERM ? (first & ~31) + (r >> 2) * 8 + (first & 16) / 4 + (r & 3) : first + r;
+            return *reinterpret_cast<const typename Frag<E>::type *>(tile + n * 128 + (((kk * 4 + q) ^ swz(n)) << 4));
+        }
+    }
+};
+
+// A workgroup's tiles: the XCD's run of neighbouring ones (columns first), its workgroups in turn
+struct WideTiles {
+    int first, step, count;
+    __device__ __forceinline__ WideTiles(const Product &p) {
+        const int total = p.tiles_r * p.tiles_c * p.splits, xcd = blockIdx.x % 8, slot = blockIdx.x / 8;
+        const int per = total / 8, extra = total % 8, run = per + (xcd < extra);
+        step = (gridDim.x + 7 - xcd) / 8;
+        first = xcd * per + min(xcd, extra) + slot;
+        count = run > slot ? (run - slot + step - 1) / step : 0;
+    }
+};
+// Tiles go through eight columns of them at a time, rows behind: a run of 32 (an XCD's workgroups) is then about as wide as it
+// is high, and shares most of what it reads.
+struct WideTile {
+    int split, row0, col0, nk;
+    int64_t kbeg;
+    __device__ __forceinline__ WideTile(const Product &p, int tile) {
+        const int plane = p.tiles_r * p.tiles_c;
+        split = tile / plane;
+        int t = tile - split * plane;
+        const int band = t / (p.tiles_r * 8), wide = min(8, p.tiles_c - band * 8);
+        t -= band * p.tiles_r * 8;
+        row0 = t / wide * 256, col0 = (band * 8 + t % wide) * 256;
+        const int64_t kall = p.R.lim > p.C.lim ? p.R.lim : p.C.lim;
+        kbeg = split * p.share;
+        const int64_t kend = kbeg + p.share < kall ? kbeg + p.share : kall;
+        nk = (int)((kend - kbeg + 63) / 64);
+    }
+};
+
+// Where a workgroup's loads of one operand are: the stage's base, and how many bytes from a sub-tile's first element on are
+// its own (rows, or columns of the last t, behind the edge are then read as zeros)
+template <bool TM> struct WideSource {
+    uint64_t base, step;     // of a stage; from sub-tile to sub-tile
+    int inside;              // output indexes from the tile's first one on
+    uint32_t rows;           // t-major: the bytes of the stage's t before the last one
+    uint32_t pitch;          // bytes
+    uint32_t off;            // the lane's offset, past the end where its reduction indexes are
+    int stages, tail;        // from this one to the operand's end, and the length of the last of them
+    __device__ __forceinline__ void trim(uint32_t lane_off, int lane_at) {
+        const int left = stages > 1 ? 64 : tail;
+        if (TM) rows = (uint32_t)(left - 1) * pitch, off = lane_off;
+        else off = lane_at < left ? lane_off : 0x80000000u;
+    }
+    __device__ __forceinline__ void enter(const Operand &o, int piece, int first, int64_t k0, uint32_t lane_off, int lane_at) {
+        base = (uint64_t)o.p + 2 * (uint64_t)(o.plane * piece + (TM ? k0 * o.ld + first : first * o.ld + k0));
+        inside = __builtin_amdgcn_readfirstlane((int)(o.width - first < 256 ? o.width - first : 256));
+        pitch = 2u * (uint32_t)o.ld;
+        step = TM ? 128 : 64 * (uint64_t)pitch;
+        const int64_t t = o.lim - k0, n = (t + 63) >> 6;
+        stages = __builtin_amdgcn_readfirstlane((int)(n < (1 << 30) ? n : 1 << 30));
+        tail = (((int)t - 1) & 63) + 1;
+        trim(lane_off, lane_at);
+    }
+    __device__ __forceinline__ void advance(uint32_t lane_off, int lane_at) {
+        base += TM ? 64 * (uint64_t)pitch : 128;
+        --stages;
+        trim(lane_off, lane_at);
+    }
+    __device__ __forceinline__ u32x4 descriptor(int q) const {
+        const uint64_t b = base + q * step;
+        const int n = min(max(inside - 64 * q, 0), 64);
+        const uint32_t bytes = TM ? (n ? rows + 2u * n : 0u) : (uint32_t)n * pitch;
+        // (uniform, which the compiler does not always see)
+        auto scalar = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
+        return u32x4{scalar((uint32_t)b), scalar((uint32_t)(b >> 32)), scalar(bytes), 0x00020000u};
+    }
+};
+
+template <typename E, typename T, bool RT, bool CT> __global__ void __launch_bounds__(512, 2) wide_product_kernel(Product p) {
+    constexpr int STAGE = 65536, COLS = 32768;   // bytes; the columns' sub-tiles follow the rows'
+    extern __shared__ __align__(1024) char smem[];
+    typedef SubTile<RT, false> SR;
+    typedef SubTile<CT, !CT> SC;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wr = wave >> 2, wc = wave & 3;
+    const WideTiles tiles(p);
+    if (tiles.count == 0) return;
+    typedef __attribute__((address_space(3))) char *lds_t;
+    const uint32_t lds = (uint32_t)(uintptr_t)(lds_t)smem + (uint32_t)wave * 1024u;
+
+    int at_r, at_c;
+    const uint32_t off_r = SR::offset(p.R, wave, lane, at_r), off_c = SC::offset(p.C, wave, lane, at_c);
+
+    // the stage to load next
+    int tile_n = 0, pair = 0, step = 0, buf = 0;
+    WideTile ahead(p, tiles.first);
+    WideSource<RT> rows;
+    WideSource<CT> cols;
+    auto enter = [&]() {
+        const int64_t k0 = ahead.kbeg + (int64_t)step * 64;
+        rows.enter(p.R, p.pr[pair], ahead.row0, k0, off_r, at_r);
+        cols.enter(p.C, p.pc[pair], ahead.col0, k0, off_c, at_c);
+        if (tile_n >= tiles.count) rows.inside = cols.inside = 0;   // past the last tile: loads that fetch nothing
+    };
+    auto next = [&]() {
+        buf ^= 1;
+        if (++step < ahead.nk) {
+            rows.advance(off_r, at_r);
+            cols.advance(off_c, at_c);
+            return;
+        }
+        step = 0;
+        if (++pair == p.npair) {
+            pair = 0;
+            if (++tile_n < tiles.count) ahead = WideTile(p, tiles.first + tile_n * tiles.step);
+        }
+        enter();
+    };
+    // two sub-tiles' loads, their descriptors made ahead (beside the MFMAs)
+    u32x4 d0, d1;
+    uint32_t to, off;
+    auto aim_rows = [&](int q) { d0 = rows.descriptor(q), d1 = rows.descriptor(q + 1), off = rows.off, to = lds + buf * STAGE + q * 8192; };
+    auto aim_cols = [&](int q) { d0 = cols.descriptor(q), d1 = cols.descriptor(q + 1), off = cols.off, to = lds + buf * STAGE + COLS + q * 8192; };
+    auto load = [&]() { load_to_lds(d0, off, to), load_to_lds(d1, off, to + 8192); };
+
+    enter();
+    aim_cols(0), load();
+    aim_cols(2), load();
+    aim_rows(0), load();
+    aim_rows(2), load();
+    next();
+    aim_cols(0), load();
+    aim_cols(2), load();
+    aim_rows(0), load();
+    aim_rows(2);
+    asm volatile("s_waitcnt vmcnt(8)\n\ts_barrier" ::: "memory");
+
+    int at = 0;
+    for (int n = 0; n < tiles.count; ++n) {
+        const WideTile tile(p, tiles.first + n * tiles.step);
+        const int iters = tile.nk * p.npair;
+        fvec4 acc[4][8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc[i][j] = fvec4{0.f, 0.f, 0.f, 0.f};
+        if (wr) asm volatile("s_barrier" ::: "memory");   // one half behind
+        for (int it = 0; it < iters; ++it) {
+            const char *tr = smem + at * STAGE, *tc = tr + COLS + wc * 8192;
+            at ^= 1;
+            typename Frag<E>::type a[2][4];
+            auto phase = [&](auto number) {
+                constexpr int ph = decltype(number)::value;
+                typename Frag<E>::type b[2][2];
+#pragma unroll
+                for (int kk = 0; kk < 2; ++kk) {
+                    if constexpr (ph == 0) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) a[kk][i] = SC::template frag<E>(tc, i * 16, kk, lane);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) b[kk][j] = SR::template frag<E>(tr + ph * 8192, j * 32 + wr * 16, kk, lane);
+                }
+                load();
+                if constexpr (ph == 1)
+                    asm volatile("s_waitcnt vmcnt(10) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                else if constexpr (ph == 3)
+                    asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                else
+                    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                __builtin_amdgcn_s_setprio(1);
+                if constexpr (ph == 0) next();
+#pragma unroll
+                for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) acc[i][ph * 2 + j] = mfma(a[kk][i], b[kk][j], acc[i][ph * 2 + j]);
+                if constexpr (ph == 0) aim_cols(0);
+                if constexpr (ph == 1) aim_cols(2);
+                if constexpr (ph == 2) aim_rows(0);
+                if constexpr (ph == 3) aim_rows(2);
+#pragma unroll
+                for (int m = 0; m < 16; ++m) {   // scalar work between the MFMAs
+                    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x4, 3, 0);
+                }
+                __builtin_amdgcn_s_setprio(0);
+                asm volatile("s_barrier" ::: "memory");
+            };
+            phase(std::integral_constant<int, 0>());
+            phase(std::integral_constant<int, 1>());
+            phase(std::integral_constant<int, 2>());
+            phase(std::integral_constant<int, 3>());
+        }
+        if (!wr) asm volatile("s_barrier" ::: "memory");   // level again
+        // Results: a lane's columns are the same in all its rows. What is read on the way comes ahead of its use: the bias once,
+        // the residual a row ahead of the stores.
+        constexpr int RUN = CT ? 4 : 8, RUNS = 16 / RUN;
+        typedef Pack<T, RUN> Run;
+        const int q = lane >> 4, colbase = tile.col0 + wc * 64 + q * RUN, first = tile.row0 + wr * 16 + (lane & 15);
+        auto col_of = [&](int r) { return colbase + r * 4 * RUN; };
+        Run bias[RUNS] = {}, ahead_r[RUNS] = {};
+        auto residual = [&](int row) {
+#pragma unroll
+            for (int r = 0; r < RUNS; ++r)
+                if (row < p.rows && col_of(r) < p.cols)
+                    ahead_r[r] = *reinterpret_cast<const Run *>((const T *)p.residual + (int64_t)row * p.cols + col_of(r));
+        };
+        if (p.bias)
+#pragma unroll
+            for (int r = 0; r < RUNS; ++r)
+                if (col_of(r) < p.cols) bias[r] = *reinterpret_cast<const Run *>((const T *)p.bias + col_of(r));
+        if (p.residual) residual(first);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int row = first + j * 32;
+            Run res[RUNS];
+#pragma unroll
+            for (int r = 0; r < RUNS; ++r) res[r] = ahead_r[r];
+            if (p.residual && j < 7) residual(row + 32);
+#pragma unroll
+            for (int r = 0; r < RUNS; ++r) {
+                const int col = col_of(r);
+                float v[RUN];
+#pragma unroll
+                for (int e = 0; e < RUN; ++e) v[e] = CT ? acc[r][j][e] : acc[r * 2 + e / 4][j][e % 4];
+                if (row >= p.rows || col >= p.cols) continue;
+                const int64_t at_o = (int64_t)row * p.cols + col;
+                if (p.sums) {
+                    float *o = (float *)p.out + (int64_t)tile.split * p.rows * p.cols + at_o;
+#pragma unroll
+                    for (int e = 0; e < RUN; e += 4) *reinterpret_cast<fvec4 *>(o + e) = fvec4{v[e], v[e + 1], v[e + 2], v[e + 3]};
+                    continue;
+                }
+                Run o;
+                if (p.bias)
+#pragma unroll
+                    for (int e = 0; e < RUN; ++e) v[e] += (float)bias[r].v[e];
+                if (p.pre) {
+#pragma unroll
+                    for (int e = 0; e < RUN; ++e) o.v[e] = (T)v[e];
+                    *reinterpret_cast<Run *>((T *)p.pre + at_o) = o;
+                }
+                act_values<is_f32<T>(), RUN>(v, p.act);
+                if (p.residual)
+#pragma unroll
+                    for (int e = 0; e < RUN; ++e) v[e] += (float)res[r].v[e];
+#pragma unroll
+                for (int e = 0; e < RUN; ++e) o.v[e] = (T)v[e];
+                *reinterpret_cast<Run *>((T *)p.out + at_o) = o;
+            }
+        }
+        // the loads' counts above are of loads alone
+        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
     }
 }
 
@@ -431,18 +752,50 @@ void set_pairs(Product &p, int nr, int nc) {
         if (s[0] < nr && s[1] < nc) p.pr[p.npair] = s[0], p.pc[p.npair] = s[1], ++p.npair;
 }
 
-template <typename E, typename T, bool RT, bool CT, int F> hipError_t launch_tiles(Product &p, hipStream_t s) {
-    p.tiles_r = (int)ceil_div(p.rows, 32 * F);
-    p.tiles_c = (int)ceil_div(p.cols, 32 * F);
-    product_kernel<E, T, RT, CT, F, F><<<(unsigned)(p.tiles_r * p.tiles_c * p.splits), TB, 0, s>>>(p);
+template <typename E, typename T, bool RT, bool CT, int WR, int WC, int FR, int FC, int BK, int STAGES, int BLOCKS>
+hipError_t launch_tiles(Product &p, hipStream_t s) {
+    constexpr int BR = WR * 16 * FR, BC = WC * 16 * FC, LDS = STAGES * (BR + BC) * BK * 2;
+    static std::atomic<unsigned long long> done{0};
+    const auto kernel = product_kernel<E, T, RT, CT, WR, WC, FR, FC, BK, STAGES, BLOCKS>;
+    if (hipError_t e = raise_lds_limit((const void *)kernel, done)) return e;
+    p.tiles_r = (int)ceil_div(p.rows, BR);
+    p.tiles_c = (int)ceil_div(p.cols, BC);
+    kernel<<<(unsigned)(p.tiles_r * p.tiles_c * p.splits), WR * WC * 64, LDS, s>>>(p);
     return hipGetLastError();
 }
 
-// 128 x 128 tiles where they fill the 256 CUs, else 64 x 64
-bool big_tiles(int64_t rows, int64_t cols, int64_t splits) { return ceil_div(rows, 128) * ceil_div(cols, 128) * splits >= 256; }
+template <typename E, typename T, bool RT, bool CT> hipError_t launch_wide(Product &p, hipStream_t s) {
+    static std::atomic<unsigned long long> done{0};
+    const auto kernel = wide_product_kernel<E, T, RT, CT>;
+    if (hipError_t e = raise_lds_limit((const void *)kernel, done)) return e;
+    p.tiles_r = (int)ceil_div(p.rows, 256);
+    p.tiles_c = (int)ceil_div(p.cols, 256);
+    const int64_t tiles = (int64_t)p.tiles_r * p.tiles_c * p.splits;
+    kernel<<<(unsigned)(tiles < 256 ? tiles : 256), 512, 131072, s>>>(p);
+    return hipGetLastError();
+}
 
-template <typename E, typename T, bool RT, bool CT> hipError_t launch_product(Product p, hipStream_t s) {
-    return big_tiles(p.rows, p.cols, p.splits) ? launch_tiles<E, T, RT, CT, 4>(p, s) : launch_tiles<E, T, RT, CT, 2>(p, s);
+// Which tiles an output takes: 256 x 256 (of whole eights of columns), one workgroup per CU; 128 x 128, two per CU; or
+// 64 x 64 where those leave CUs idle. What a step of 64 along the reduction takes with all CUs at work: 2.1 us in 256 x 256
+// tiles, 1.95 us in twice 128 x 128 (65536 x 512 from 2048, bfloat16), so the rounds decide.
+enum Tiles { WIDE, BIG, SMALL };
+double wide_cost(int64_t rows, int64_t cols, int64_t splits) {
+    return 2.1 * (double)ceil_div(ceil_div(rows, 256) * ceil_div(cols, 256) * splits, 256);
+}
+double big_cost(int64_t rows, int64_t cols, int64_t splits) {
+    return 1.95 * (double)ceil_div(ceil_div(rows, 128) * ceil_div(cols, 128) * splits, 512);
+}
+Tiles choose_tiles(int64_t rows, int64_t cols) {
+    if (cols % 8 == 0 && wide_cost(rows, cols, 1) < big_cost(rows, cols, 1)) return WIDE;
+    return ceil_div(rows, 128) * ceil_div(cols, 128) >= 256 ? BIG : SMALL;
+}
+
+template <typename E, typename T, bool RT, bool CT> hipError_t launch_product(Product p, Tiles tiles, hipStream_t s) {
+    switch (tiles) {
+        case WIDE: return launch_wide<E, T, RT, CT>(p, s);
+        case BIG: return launch_tiles<E, T, RT, CT, 2, 2, 4, 4, 64, 2, 2>(p, s);
+        default: return launch_tiles<E, T, RT, CT, 2, 2, 2, 2, 64, 3, 2>(p, s);
+    }
 }
 
 // y or dx: rows in runs whose workgroups HIP takes in one launch
@@ -459,7 +812,7 @@ template <typename E, typename T, bool CT> hipError_t launch_rows(Product p, int
         p.out = out + first * p.cols;
         p.pre = pre ? pre + first * p.cols : nullptr;
         p.residual = res ? res + first * p.cols : nullptr;
-        if (hipError_t e = launch_product<E, T, false, CT>(p, s)) return e;
+        if (hipError_t e = launch_product<E, T, false, CT>(p, choose_tiles(p.rows, p.cols), s)) return e;
     }
     return hipSuccess;
 }
@@ -479,7 +832,8 @@ struct Plan {
     size_t x_at, w_at, dz_at, part_at, sums_at, forward, backward;
     int cols, chunks;                  // bias gradient: lanes of channels, chunks of rows
     int64_t chunk;
-    int splits;                        // weight gradient: shares of the rows
+    Tiles tiles;                       // weight gradient: its tiles, and shares of the rows
+    int splits;
     int64_t share;
 };
 
@@ -519,13 +873,19 @@ Plan make_plan(const PointwiseArgs &a) {
     k.chunk = ceil_div(a.rows, chunks < 1 ? 1 : chunks);
     k.chunks = (int)ceil_div(a.rows, k.chunk < 1 ? 1 : k.chunk);
     k.part_at = take((size_t)k.chunks * a.out * 4);
-    // shares of the rows: two 128 x 128 workgroups per CU, each at least four steps
-    const int64_t tiles = ceil_div(a.out, 128) * ceil_div(a.in, 128);
-    int64_t splits = ceil_div(512, tiles);
-    const int64_t most_splits = ceil_div(a.rows, 4 * BK);
-    splits = splits < most_splits ? splits : most_splits;
-    k.share = round_up(ceil_div(a.rows, splits < 1 ? 1 : splits), BK);
+    // shares of the rows: as many as give every CU its workgroups, each share at least four steps. The shares' sums are
+    // written and read again: 8 bytes per output and share, at about 4 TB/s.
+    const int64_t most_splits = std::max<int64_t>(1, a.rows / (4 * SHARE));
+    auto cost = [&](int64_t splits, double per_step) {
+        return per_step * (double)ceil_div(ceil_div(a.rows, splits), SHARE) + (splits > 1 ? (double)(splits * a.out) * a.in * 2e-6 : 0.0);
+    };
+    const int64_t t256 = ceil_div(a.out, 256) * ceil_div(a.in, 256), t128 = ceil_div(a.out, 128) * ceil_div(a.in, 128);
+    const int64_t s256 = std::min(std::max<int64_t>(1, 256 / t256), most_splits), s128 = std::min(std::max<int64_t>(1, 512 / t128), most_splits);
+    const bool wide256 = a.in % 8 == 0 && cost(s256, wide_cost(a.out, a.in, s256)) < cost(s128, big_cost(a.out, a.in, s128));
+    const int64_t splits = wide256 ? s256 : s128;
+    k.share = round_up(ceil_div(a.rows, splits), SHARE);
     k.splits = (int)ceil_div(a.rows, k.share < 1 ? 1 : k.share);
+    k.tiles = wide256 ? WIDE : t128 * k.splits >= 256 ? BIG : SMALL;
     k.sums_at = k.splits > 1 ? take((size_t)k.splits * a.out * a.in * 4) : 0;
     k.backward = off;
     return k;
@@ -603,7 +963,7 @@ template <typename T, typename E, int NP> hipError_t backward(const PointwiseArg
         p.share = k.share;
         p.sums = k.splits > 1;
         p.out = p.sums ? (void *)(a.work + k.sums_at) : a.dweight;
-        if (hipError_t e = launch_product<E, T, true, true>(p, s)) return e;
+        if (hipError_t e = launch_product<E, T, true, true>(p, k.tiles, s)) return e;
     }
     // (no rows: zeros, the sum of nothing)
     const bool sum_w = a.dweight && (k.splits > 1 || a.rows == 0);
