@@ -222,9 +222,12 @@ __global__ void __launch_bounds__(TB) norm_apply_kernel(const T *__restrict__ x,
             for (int u = 0; u < UNROLL; ++u) {
                 const int64_t ru = r + (int64_t)u * k.lanes_r;
                 if (ru >= last) break;
+                float z[VEC];
 #pragma unroll
-                for (int v = 0; v < VEC; ++v)
-                    p[u].v[v] = (T)act_value<is_f32<T>()>(fmaf((float)p[u].v[v] - mu[v], sc[v], bv[v]), act);
+                for (int v = 0; v < VEC; ++v) z[v] = fmaf((float)p[u].v[v] - mu[v], sc[v], bv[v]);
+                act_values<is_f32<T>(), VEC>(z, act);
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) p[u].v[v] = (T)z[v];
                 *reinterpret_cast<Pack<T, VEC> *>(y + base + ru * C) = p[u];
             }
         }
@@ -276,12 +279,18 @@ __global__ void __launch_bounds__(TB) norm_sums_kernel(Source<T, VEC, KEPT> src,
 #pragma unroll
                 for (int u = 0; u < UNROLL; ++u) {
                     if (r + (int64_t)u * k.lanes_r >= last) break;
+                    float z[VEC], dz[VEC];
 #pragma unroll
                     for (int v = 0; v < VEC; ++v) {
-                        const float n = (f[u][v] - mu[v]) * rs[v];
-                        const float dz = (float)d[u].v[v] * act_slope<is_f32<T>()>(fmaf(n, wv[v], bv[v]), act);
-                        s[v] += dz;
-                        q[v] = fmaf(dz, n, q[v]);
+                        f[u][v] = (f[u][v] - mu[v]) * rs[v];
+                        z[v] = fmaf(f[u][v], wv[v], bv[v]);
+                        dz[v] = (float)d[u].v[v];
+                    }
+                    act_slopes<is_f32<T>(), VEC>(dz, z, act);
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v) {
+                        s[v] += dz[v];
+                        q[v] = fmaf(dz[v], f[u][v], q[v]);
                     }
                 }
             }
@@ -293,22 +302,24 @@ __global__ void __launch_bounds__(TB) norm_sums_kernel(Source<T, VEC, KEPT> src,
     }
 }
 
-// The first BG workgroups: avg(dn) and avg(dn n) of a (batch, group) into avg. The others: 64 channels of dw and db
-// each, four waves along the chunks.
+constexpr int FIN = 1024;   // lanes of the step that adds up the chunks' sums: 4 loads each in flight cover 256 chunks in one go
+
+// The first BG workgroups: avg(dn) and avg(dn n) of a (batch, group) into avg. The others: 16 channels of dw and db each, 64
+// lanes along the chunks of all images.
 template <typename T>
-__global__ void __launch_bounds__(TB) norm_bwd_finish_kernel(const float2 *__restrict__ part, const void *__restrict__ w,
-                                                             float2 *__restrict__ avg, T *__restrict__ dw,
-                                                             T *__restrict__ db, int64_t BG, int64_t P, int C, int G,
-                                                             int Cg, int chunks, int64_t units) {
-    __shared__ float2 red[TB];
+__global__ void __launch_bounds__(FIN) norm_bwd_finish_kernel(const float2 *__restrict__ part, const void *__restrict__ w,
+                                                              float2 *__restrict__ avg, T *__restrict__ dw,
+                                                              T *__restrict__ db, int64_t BG, int64_t P, int C, int G,
+                                                              int Cg, int chunks, int64_t units) {
+    __shared__ float2 red[FIN];
     const int t = threadIdx.x;
-    const int64_t jobs = BG + (dw || db ? (C + 63) / 64 : 0);
+    const int64_t jobs = BG + (dw || db ? (C + 15) / 16 : 0);
     for (int64_t job = blockIdx.x; job < jobs; job += gridDim.x) {
         float s = 0.f, q = 0.f;
         if (job < BG) {
             const int64_t b = job / G;
             const int g = (int)(job - b * G);
-            for (int64_t i = t; i < (int64_t)chunks * Cg; i += TB) {
+            for (int64_t i = t; i < (int64_t)chunks * Cg; i += FIN) {
                 const int64_t chunk = i / Cg;
                 const int c = g * Cg + (int)(i - chunk * Cg);
                 const float2 v = part[(b * chunks + chunk) * C + c];
@@ -320,24 +331,37 @@ __global__ void __launch_bounds__(TB) norm_bwd_finish_kernel(const float2 *__res
             q = wave_sum(q);
             if ((t & 63) == 0) red[t >> 6] = make_float2(s, q);
             __syncthreads();
-            if (t == 0) {
+            if (t < 64) {
+                const float2 v = t < FIN / 64 ? red[t] : make_float2(0.f, 0.f);
                 const float n = (float)((double)P * Cg);
-                avg[job] = make_float2((red[0].x + red[1].x + red[2].x + red[3].x) / n,
-                                       (red[0].y + red[1].y + red[2].y + red[3].y) / n);
+                s = wave_sum(v.x) / n;
+                q = wave_sum(v.y) / n;
+                if (t == 0) avg[job] = make_float2(s, q);
             }
         } else {
-            const int c = (int)(job - BG) * 64 + (t & 63);
+            const int c = (int)(job - BG) * 16 + (t & 15);
             if (c < C)
-                for (int64_t u = t >> 6; u < units; u += TB / 64) {
-                    const float2 v = part[u * C + c];
-                    s += v.x;
-                    q += v.y;
+                for (int64_t u = t >> 4; u < units; u += 4 * (FIN / 16)) {
+                    float2 v[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int64_t uk = u + k * (FIN / 16);
+                        v[k] = uk < units ? part[uk * C + c] : make_float2(0.f, 0.f);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) s += v[k].x, q += v[k].y;
                 }
             red[t] = make_float2(s, q);
             __syncthreads();
-            if (t < 64 && c < C) {
-                if (db) db[c] = (T)(red[t].x + red[t + 64].x + red[t + 128].x + red[t + 192].x);
-                if (dw) dw[c] = (T)(red[t].y + red[t + 64].y + red[t + 128].y + red[t + 192].y);
+            if (t < 64) {   // four lanes a channel, 16 rows each
+                float2 a = red[t];
+                for (int k = 64; k < FIN; k += 64) a.x += red[t + k].x, a.y += red[t + k].y;
+                a.x += __shfl_xor(a.x, 16), a.y += __shfl_xor(a.y, 16);
+                a.x += __shfl_xor(a.x, 32), a.y += __shfl_xor(a.y, 32);
+                if (t < 16 && c < C) {
+                    if (db) db[c] = (T)a.x;
+                    if (dw) dw[c] = (T)a.y;
+                }
             }
         }
         __syncthreads();
@@ -383,12 +407,16 @@ __global__ void __launch_bounds__(TB) norm_dx_kernel(Source<T, VEC, KEPT> src, c
             for (int u = 0; u < UNROLL; ++u) {
                 const int64_t ru = r + (int64_t)u * k.lanes_r;
                 if (ru >= last) break;
+                float z[VEC], dz[VEC];
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) {
-                    const float n = (f[u][v] - mu[v]) * rs[v];
-                    const float dn = (float)d[u].v[v] * act_slope<is_f32<T>()>(fmaf(n, wv[v], bv[v]), act) * wv[v];
-                    d[u].v[v] = (T)(rs[v] * (dn - a1[v] - n * a2[v]));
+                    f[u][v] = (f[u][v] - mu[v]) * rs[v];
+                    z[v] = fmaf(f[u][v], wv[v], bv[v]);
+                    dz[v] = (float)d[u].v[v];
                 }
+                act_slopes<is_f32<T>(), VEC>(dz, z, act);
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) d[u].v[v] = (T)(rs[v] * (dz[v] * wv[v] - a1[v] - f[u][v] * a2[v]));
                 *reinterpret_cast<Pack<T, VEC> *>(dx + base + ru * C) = d[u];
             }
         }
@@ -420,7 +448,7 @@ template <typename T, int VEC, bool KEPT> hipError_t backward(const NormArgs &a,
     const int C = a.channels, G = a.groups, Cg = C / G;
     if (a.batch == 0 || a.pixels == 0) {   // sums of nothing
         if (a.dweight || a.dbias)
-            norm_bwd_finish_kernel<T><<<grid_1d(ceil_div(C, 64)), TB, 0, s>>>(nullptr, a.weight, nullptr, (T *)a.dweight,
+            norm_bwd_finish_kernel<T><<<grid_1d(ceil_div(C, 16)), FIN, 0, s>>>(nullptr, a.weight, nullptr, (T *)a.dweight,
                                                                              (T *)a.dbias, 0, 0, C, G, Cg, 0, 0);
         return hipGetLastError();
     }
@@ -431,7 +459,7 @@ template <typename T, int VEC, bool KEPT> hipError_t backward(const NormArgs &a,
     norm_sums_kernel<T, VEC, KEPT><<<grid_of(k), TB, 0, s>>>(src, (const T *)a.dy, a.weight, a.bias, a.mean, a.rstd,
                                                              part, a.pixels, C, G, Cg, a.act, k);
     if (hipError_t e = hipGetLastError()) return e;
-    norm_bwd_finish_kernel<T><<<grid_1d(BG + ceil_div(C, 64)), TB, 0, s>>>(
+    norm_bwd_finish_kernel<T><<<grid_1d(BG + ceil_div(C, 16)), FIN, 0, s>>>(
         part, a.weight, avg, (T *)a.dweight, (T *)a.dbias, BG, a.pixels, C, G, Cg, k.chunks, k.units);
     if (hipError_t e = hipGetLastError()) return e;
     if (a.dx)

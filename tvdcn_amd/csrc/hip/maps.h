@@ -131,6 +131,21 @@ template <bool PRECISE> __device__ __forceinline__ float act_slope(float z, int 
     }
 }
 
+// d *= slope(z)
+template <bool PRECISE, int N> __device__ __forceinline__ void act_slopes(float *d, const float *z, int act) {
+    if (act == TVDCN_ACT_NONE) return;
+    if (act == TVDCN_ACT_RELU) {
+#pragma unroll
+        for (int v = 0; v < N; ++v) d[v] *= act_slope<PRECISE>(z[v], TVDCN_ACT_RELU);
+    } else if (act == TVDCN_ACT_SILU) {
+#pragma unroll
+        for (int v = 0; v < N; ++v) d[v] *= act_slope<PRECISE>(z[v], TVDCN_ACT_SILU);
+    } else {
+#pragma unroll
+        for (int v = 0; v < N; ++v) d[v] *= act_slope<PRECISE>(z[v], TVDCN_ACT_GELU);
+    }
+}
+
 template <typename T> constexpr bool is_f32() { return sizeof(T) == 4; }
 template <typename T> __device__ __forceinline__ float most() { return 0.f; }
 template <> __device__ __forceinline__ float most<float>() { return 3.402823466e38f; }

@@ -675,24 +675,31 @@ __global__ void __launch_bounds__(TB) slope_kernel(const T *__restrict__ dy, con
     float s[8];
 #pragma unroll
     for (int v = 0; v < 8; ++v) s[v] = 0.f;
+    constexpr int UNROLL = 4;   // rows of a lane in flight
     if (active)
-        for (int64_t r = first + rl; r < last; r += lanes_r) {
-            float d[8], z[8];
-            load8(dy + r * C, c, C, vec, d);
-            if (act != TVDCN_ACT_NONE) {
-                load8(pre + r * C, c, C, vec, z);
+        for (int64_t r0 = first + rl; r0 < last; r0 += (int64_t)lanes_r * UNROLL) {
+            float d[UNROLL][8], z[UNROLL][8];
 #pragma unroll
-                for (int v = 0; v < 8; ++v) d[v] *= act_slope<is_f32<T>()>(z[v], act);
+            for (int u = 0; u < UNROLL; ++u) {
+                const int64_t ru = r0 + (int64_t)u * lanes_r, r = ru < last ? ru : first;
+                load8(dy + r * C, c, C, vec, d[u]);
+                if (act != TVDCN_ACT_NONE) load8(pre + r * C, c, C, vec, z[u]);
             }
 #pragma unroll
-            for (int v = 0; v < 8; ++v) s[v] += d[v];
-            if (dz) {
-                Pack<E, 8> o[NP];
+            for (int u = 0; u < UNROLL; ++u) {
+                const int64_t r = r0 + (int64_t)u * lanes_r;
+                if (r >= last) break;
+                act_slopes<is_f32<T>(), 8>(d[u], z[u], act);
 #pragma unroll
-                for (int v = 0; v < 8; ++v) split_pack<E, NP>(d[v], v, o);
+                for (int v = 0; v < 8; ++v) s[v] += d[u][v];
+                if (dz) {
+                    Pack<E, 8> o[NP];
 #pragma unroll
-                for (int n = 0; n < NP; ++n)
-                    *reinterpret_cast<Pack<E, 8> *>(dz + n * plane + (r * lanes_row + j) * 8) = o[n];
+                    for (int v = 0; v < 8; ++v) split_pack<E, NP>(d[u][v], v, o);
+#pragma unroll
+                    for (int n = 0; n < NP; ++n)
+                        *reinterpret_cast<Pack<E, 8> *>(dz + n * plane + (r * lanes_row + j) * 8) = o[n];
+                }
             }
         }
     if (!part) return;
@@ -708,29 +715,49 @@ __global__ void __launch_bounds__(TB) slope_kernel(const T *__restrict__ dy, con
     }
 }
 
-// dW = the sum of its shares; db = the sum of its chunks (64 channels per workgroup, four waves along the chunks)
+constexpr int FIN = 1024;
+
+// dW = the sum of its shares (eight loads in flight per lane); db = the sum of its chunks (16 channels per workgroup, 64
+// lanes along the chunks)
 template <typename T>
-__global__ void __launch_bounds__(TB) finish_kernel(const float *__restrict__ sums, T *__restrict__ dw, int64_t n,
-                                                    int splits, int w_blocks, const float *__restrict__ part,
-                                                    T *__restrict__ db, int C, int chunks) {
-    __shared__ float red[TB];
+__global__ void __launch_bounds__(FIN) finish_kernel(const float *__restrict__ sums, T *__restrict__ dw, int64_t n,
+                                                     int splits, int w_blocks, const float *__restrict__ part,
+                                                     T *__restrict__ db, int C, int chunks) {
+    __shared__ float red[FIN];
     const int t = threadIdx.x;
     if ((int)blockIdx.x < w_blocks) {
-        const int64_t stride = (int64_t)w_blocks * TB;
-        for (int64_t i = (int64_t)blockIdx.x * TB + t; i < n; i += stride) {
+        const int64_t stride = (int64_t)w_blocks * FIN;
+        for (int64_t i = (int64_t)blockIdx.x * FIN + t; i < n; i += stride) {
             float a = 0.f;
-            for (int k = 0; k < splits; ++k) a += sums[k * n + i];
+            for (int k = 0; k < splits; k += 8) {
+                float v[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) v[u] = k + u < splits ? sums[(k + u) * n + i] : 0.f;
+#pragma unroll
+                for (int u = 0; u < 8; ++u) a += v[u];
+            }
             dw[i] = (T)a;
         }
         return;
     }
-    const int c = ((int)blockIdx.x - w_blocks) * 64 + (t & 63);
+    const int c = ((int)blockIdx.x - w_blocks) * 16 + (t & 15);
     float a = 0.f;
     if (c < C)
-        for (int u = t >> 6; u < chunks; u += TB / 64) a += part[(int64_t)u * C + c];
+        for (int u = t >> 4; u < chunks; u += 4 * (FIN / 16)) {
+            float v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = u + k * (FIN / 16) < chunks ? part[(int64_t)(u + k * (FIN / 16)) * C + c] : 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) a += v[k];
+        }
     red[t] = a;
     __syncthreads();
-    if (t < 64 && c < C) db[c] = (T)(red[t] + red[t + 64] + red[t + 128] + red[t + 192]);
+    if (t < 64) {   // four lanes a channel, 16 rows each
+        for (int k = 64; k < FIN; k += 64) a += red[t + k];
+        a += __shfl_xor(a, 16);
+        a += __shfl_xor(a, 32);
+        if (t < 16 && c < C) db[c] = (T)a;
+    }
 }
 
 // ---- host ----
@@ -968,9 +995,9 @@ template <typename T, typename E, int NP> hipError_t backward(const PointwiseArg
     // (no rows: zeros, the sum of nothing)
     const bool sum_w = a.dweight && (k.splits > 1 || a.rows == 0);
     const int64_t n = (int64_t)a.out * a.in;
-    const int w_blocks = sum_w ? (int)strided_grid(n) : 0, b_blocks = a.dbias ? (int)ceil_div(a.out, 64) : 0;
+    const int w_blocks = sum_w ? (int)std::min<int64_t>(ceil_div(n, FIN), 4096) : 0, b_blocks = a.dbias ? (int)ceil_div(a.out, 16) : 0;
     if (w_blocks + b_blocks == 0) return hipSuccess;
-    finish_kernel<T><<<(unsigned)(w_blocks + b_blocks), TB, 0, s>>>((const float *)(a.work + k.sums_at), (T *)a.dweight, n,
+    finish_kernel<T><<<(unsigned)(w_blocks + b_blocks), FIN, 0, s>>>((const float *)(a.work + k.sums_at), (T *)a.dweight, n,
                                                                    a.rows ? k.splits : 0, w_blocks, part, (T *)a.dbias,
                                                                    a.out, a.rows ? k.chunks : 0);
     return hipGetLastError();
