@@ -18,6 +18,7 @@
 // the rate of the float32 MFMAs). An infinite operand may turn into a NaN where float32 would keep an infinity.
 #include <algorithm>
 #include <atomic>
+#include <tuple>
 #include <type_traits>
 
 #include "kernels.h"
@@ -296,22 +297,23 @@ __global__ void __launch_bounds__(WR * WC * 64, BLOCKS * WR * WC / 4) product_ke
     }
 }
 
-// The product in tiles of 256 x 256, for outputs that fill the chip with them: half the operand traffic of 128 x 128 tiles,
-// and that traffic, not the MFMAs, bounds those.
+// The product in tiles of 256 x 256 (or 256 x 128), for outputs that fill the chip with them: half the operand traffic of 128 x
+// 128 tiles (three quarters), and that traffic, not the MFMAs, bounds those.
 //
-// Eight waves, 2 along the rows x 4 along the columns, 128 x 64 each. A stage of 64 along the reduction is cut into eight
-// sub-tiles of 8 KB (64 output indexes each), loaded by one 1 KB load per wave; LDS holds two stages. A stage is worked off
-// in four phases of 16 MFMAs: phase p takes two row fragments (rows 64 p .. 64 p + 63 of the tile, those of both wave rows)
-// against the four column fragments, which phase 0 reads and keeps in registers. A phase is a memory half (LDS reads, two
+// Eight waves, 2 along the rows x 4 along the columns, 128 x 64 each (128 x 32: FC = 2 column fragments instead of 4). A stage
+// of 64 along the reduction is cut into sub-tiles of 8 KB (64 output indexes each), loaded by one 1 KB load per wave; LDS holds
+// two stages. A stage is worked off in four phases of 4 FC MFMAs: phase p takes two row fragments (rows 64 p .. 64 p + 63 of the
+// tile, those of both wave rows) against the column fragments, which phase 0 reads and keeps in registers. A phase is a memory half (LDS reads, two
 // loads) and an MFMA half, a barrier behind each; the second wave row runs one half behind the first, so that each SIMD has
 // one wave multiplying while its other one reads.
 //
 // The loads of a stage are issued as soon as the phases that read the sub-tile's place are over, up to seven phases ahead:
-//   phase 1, 2 of stage i: columns of stage i + 2;  phase 3: rows 0..127 of stage i + 2;
+//   phase 1, 2 of stage i: columns of stage i + 2 (FC = 2: all in phase 1);  phase 3: rows 0..127 of stage i + 2;
 //   phase 0 of stage i + 1: rows 128..255 of stage i + 2
 // (both wave rows have then read the place: the one behind ends its reads a half before). At the end of phase 3's memory
-// half the loads issued after columns and rows 0..127 of the next stage are eight, at the end of phase 1's those after this
-// stage's rows 128..255 are ten: vmcnt(8) and vmcnt(10) there, a barrier before the first read.
+// half the loads issued after columns and rows 0..127 of the next stage are 4 + FC (rows 128..255 of it; columns and rows 0..127
+// of the one behind it), at the end of phase 1's those after this stage's rows 128..255 are 6 + FC (the next stage's FC + 4, and
+// two columns): vmcnt to those counts, a barrier before the first read.
 //
 // Workgroups are persistent: a tile's stages follow the last one's, the first loads of the next tile are under way while the
 // results are stored.
@@ -368,7 +370,7 @@ struct WideTiles {
 };
 // Tiles go through eight columns of them at a time, rows behind: a run of 32 (an XCD's workgroups) is then about as wide as it
 // is high, and shares most of what it reads.
-struct WideTile {
+template <int BC> struct WideTile {
     int split, row0, col0, nk;
     int64_t kbeg;
     __device__ __forceinline__ WideTile(const Product &p, int tile) {
@@ -377,7 +379,7 @@ struct WideTile {
         int t = tile - split * plane;
         const int band = t / (p.tiles_r * 8), wide = min(8, p.tiles_c - band * 8);
         t -= band * p.tiles_r * 8;
-        row0 = t / wide * 256, col0 = (band * 8 + t % wide) * 256;
+        row0 = t / wide * 256, col0 = (band * 8 + t % wide) * BC;
         const int64_t kall = p.R.lim > p.C.lim ? p.R.lim : p.C.lim;
         kbeg = split * p.share;
         const int64_t kend = kbeg + p.share < kall ? kbeg + p.share : kall;
@@ -387,7 +389,7 @@ struct WideTile {
 
 // Where a workgroup's loads of one operand are: the stage's base, and how many bytes from a sub-tile's first element on are
 // its own (rows, or columns of the last t, behind the edge are then read as zeros)
-template <bool TM> struct WideSource {
+template <bool TM, int B> struct WideSource {
     uint64_t base, step;     // of a stage; from sub-tile to sub-tile
     int inside;              // output indexes from the tile's first one on
     uint32_t rows;           // t-major: the bytes of the stage's t before the last one
@@ -401,7 +403,7 @@ template <bool TM> struct WideSource {
     }
     __device__ __forceinline__ void enter(const Operand &o, int piece, int first, int64_t k0, uint32_t lane_off, int lane_at) {
         base = (uint64_t)o.p + 2 * (uint64_t)(o.plane * piece + (TM ? k0 * o.ld + first : first * o.ld + k0));
-        inside = __builtin_amdgcn_readfirstlane((int)(o.width - first < 256 ? o.width - first : 256));
+        inside = __builtin_amdgcn_readfirstlane((int)(o.width - first < B ? o.width - first : B));
         pitch = 2u * (uint32_t)o.ld;
         step = TM ? 128 : 64 * (uint64_t)pitch;
         const int64_t t = o.lim - k0, n = (t + 63) >> 6;
@@ -424,8 +426,8 @@ template <bool TM> struct WideSource {
     }
 };
 
-template <typename E, typename T, bool RT, bool CT> __global__ void __launch_bounds__(512, 2) wide_product_kernel(Product p) {
-    constexpr int STAGE = 65536, COLS = 32768;   // bytes; the columns' sub-tiles follow the rows'
+template <typename E, typename T, bool RT, bool CT, int FC> __global__ void __launch_bounds__(512, 2) wide_product_kernel(Product p) {
+    constexpr int BC = 64 * FC, COLS = 32768, STAGE = COLS + BC * 128;   // bytes; the columns' sub-tiles follow the rows'
     extern __shared__ __align__(1024) char smem[];
     typedef SubTile<RT, false> SR;
     typedef SubTile<CT, !CT> SC;
@@ -441,9 +443,9 @@ template <typename E, typename T, bool RT, bool CT> __global__ void __launch_bou
 
     // the stage to load next
     int tile_n = 0, pair = 0, step = 0, buf = 0;
-    WideTile ahead(p, tiles.first);
-    WideSource<RT> rows;
-    WideSource<CT> cols;
+    WideTile<BC> ahead(p, tiles.first);
+    WideSource<RT, 256> rows;
+    WideSource<CT, BC> cols;
     auto enter = [&]() {
         const int64_t k0 = ahead.kbeg + (int64_t)step * 64;
         rows.enter(p.R, p.pr[pair], ahead.row0, k0, off_r, at_r);
@@ -460,7 +462,7 @@ template <typename E, typename T, bool RT, bool CT> __global__ void __launch_bou
         step = 0;
         if (++pair == p.npair) {
             pair = 0;
-            if (++tile_n < tiles.count) ahead = WideTile(p, tiles.first + tile_n * tiles.step);
+            if (++tile_n < tiles.count) ahead = WideTile<BC>(p, tiles.first + tile_n * tiles.step);
         }
         enter();
     };
@@ -473,30 +475,30 @@ template <typename E, typename T, bool RT, bool CT> __global__ void __launch_bou
 
     enter();
     aim_cols(0), load();
-    aim_cols(2), load();
+    if (FC == 4) aim_cols(2), load();
     aim_rows(0), load();
     aim_rows(2), load();
     next();
     aim_cols(0), load();
-    aim_cols(2), load();
+    if (FC == 4) aim_cols(2), load();
     aim_rows(0), load();
     aim_rows(2);
-    asm volatile("s_waitcnt vmcnt(8)\n\ts_barrier" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(4 + FC) : "memory");
 
     int at = 0;
     for (int n = 0; n < tiles.count; ++n) {
-        const WideTile tile(p, tiles.first + n * tiles.step);
+        const WideTile<BC> tile(p, tiles.first + n * tiles.step);
         const int iters = tile.nk * p.npair;
-        fvec4 acc[4][8];
+        fvec4 acc[FC][8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < FC; ++i)
 #pragma unroll
             for (int j = 0; j < 8; ++j) acc[i][j] = fvec4{0.f, 0.f, 0.f, 0.f};
         if (wr) asm volatile("s_barrier" ::: "memory");   // one half behind
         for (int it = 0; it < iters; ++it) {
-            const char *tr = smem + at * STAGE, *tc = tr + COLS + wc * 8192;
+            const char *tr = smem + at * STAGE, *tc = tr + COLS + wc * FC / 4 * 8192;
             at ^= 1;
-            typename Frag<E>::type a[2][4];
+            typename Frag<E>::type a[2][FC];
             auto phase = [&](auto number) {
                 constexpr int ph = decltype(number)::value;
                 typename Frag<E>::type b[2][2];
@@ -504,16 +506,16 @@ template <typename E, typename T, bool RT, bool CT> __global__ void __launch_bou
                 for (int kk = 0; kk < 2; ++kk) {
                     if constexpr (ph == 0) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) a[kk][i] = SC::template frag<E>(tc, i * 16, kk, lane);
+                        for (int i = 0; i < FC; ++i) a[kk][i] = SC::template frag<E>(tc, wc * FC % 4 * 16 + i * 16, kk, lane);
                     }
 #pragma unroll
                     for (int j = 0; j < 2; ++j) b[kk][j] = SR::template frag<E>(tr + ph * 8192, j * 32 + wr * 16, kk, lane);
                 }
-                load();
+                if constexpr (FC == 4 || ph != 2) load();
                 if constexpr (ph == 1)
-                    asm volatile("s_waitcnt vmcnt(10) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(FC == 4 ? 10 : 8) : "memory");
                 else if constexpr (ph == 3)
-                    asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(4 + FC) : "memory");
                 else
                     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
                 __builtin_amdgcn_s_setprio(1);
@@ -521,15 +523,15 @@ template <typename E, typename T, bool RT, bool CT> __global__ void __launch_bou
 #pragma unroll
                 for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
+                    for (int i = 0; i < FC; ++i)
 #pragma unroll
                         for (int j = 0; j < 2; ++j) acc[i][ph * 2 + j] = mfma(a[kk][i], b[kk][j], acc[i][ph * 2 + j]);
                 if constexpr (ph == 0) aim_cols(0);
-                if constexpr (ph == 1) aim_cols(2);
+                if constexpr (ph == 1 && FC == 4) aim_cols(2);
                 if constexpr (ph == 2) aim_rows(0);
                 if constexpr (ph == 3) aim_rows(2);
 #pragma unroll
-                for (int m = 0; m < 16; ++m) {   // scalar work between the MFMAs
+                for (int m = 0; m < 4 * FC; ++m) {   // scalar work between the MFMAs
                     __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
                     __builtin_amdgcn_sched_group_barrier(0x4, 3, 0);
                 }
@@ -544,9 +546,9 @@ template <typename E, typename T, bool RT, bool CT> __global__ void __launch_bou
         if (!wr) asm volatile("s_barrier" ::: "memory");   // level again
         // Results: a lane's columns are the same in all its rows. What is read on the way comes ahead of its use: the bias once,
         // the residual a row ahead of the stores.
-        constexpr int RUN = CT ? 4 : 8, RUNS = 16 / RUN;
+        constexpr int RUN = CT ? 4 : 8, RUNS = 4 * FC / RUN;
         typedef Pack<T, RUN> Run;
-        const int q = lane >> 4, colbase = tile.col0 + wc * 64 + q * RUN, first = tile.row0 + wr * 16 + (lane & 15);
+        const int q = lane >> 4, colbase = tile.col0 + wc * 16 * FC + q * RUN, first = tile.row0 + wr * 16 + (lane & 15);
         auto col_of = [&](int r) { return colbase + r * 4 * RUN; };
         Run bias[RUNS] = {}, ahead_r[RUNS] = {};
         auto residual = [&](int row) {
@@ -791,35 +793,42 @@ hipError_t launch_tiles(Product &p, hipStream_t s) {
     return hipGetLastError();
 }
 
-template <typename E, typename T, bool RT, bool CT> hipError_t launch_wide(Product &p, hipStream_t s) {
+template <typename E, typename T, bool RT, bool CT, int FC> hipError_t launch_wide(Product &p, hipStream_t s) {
     static std::atomic<unsigned long long> done{0};
-    const auto kernel = wide_product_kernel<E, T, RT, CT>;
+    const auto kernel = wide_product_kernel<E, T, RT, CT, FC>;
     if (hipError_t e = raise_lds_limit((const void *)kernel, done)) return e;
     p.tiles_r = (int)ceil_div(p.rows, 256);
-    p.tiles_c = (int)ceil_div(p.cols, 256);
+    p.tiles_c = (int)ceil_div(p.cols, 64 * FC);
     const int64_t tiles = (int64_t)p.tiles_r * p.tiles_c * p.splits;
-    kernel<<<(unsigned)(tiles < 256 ? tiles : 256), 512, 131072, s>>>(p);
+    kernel<<<(unsigned)(tiles < 256 ? tiles : 256), 512, 2 * (32768 + 64 * FC * 128), s>>>(p);
     return hipGetLastError();
 }
 
-// Which tiles an output takes: 256 x 256 (of whole eights of columns), one workgroup per CU; 128 x 128, two per CU; or
-// 64 x 64 where those leave CUs idle. What a step of 64 along the reduction takes with all CUs at work: 2.1 us in 256 x 256
-// tiles, 1.95 us in twice 128 x 128 (65536 x 512 from 2048, bfloat16), so the rounds decide.
-enum Tiles { WIDE, BIG, SMALL };
-double wide_cost(int64_t rows, int64_t cols, int64_t splits) {
-    return 2.1 * (double)ceil_div(ceil_div(rows, 256) * ceil_div(cols, 256) * splits, 256);
+// Which tiles an output takes: 256 x 256 or 256 x 128 (of whole eights of columns), one workgroup per CU; 128 x 128 or 64 x 64,
+// two per CU. The least of what they take, in microseconds: launch, first loads and results, and so much per step of 64 along
+// the reduction and round of workgroups. Measured in bfloat16, 16 steps: 2048 x 1024 takes 33.6 / 23.7 / 21.1 / 15.6 us in the
+// four; 24 steps, 32768 x 256: 47.8 / 35.0 / 43.3 / 79.7; 32 steps, 65536 x 512: 130 / 166 / 253 / -.
+enum Tiles { WIDE, HALF, BIG, SMALL };
+double tiles_cost(Tiles t, int64_t rows, int64_t cols, int64_t splits, double steps) {
+    auto count = [&](int64_t r, int64_t c) { return ceil_div(rows, r) * ceil_div(cols, c) * splits; };
+    switch (t) {
+        case WIDE: return 10 + 1.75 * steps * (double)ceil_div(count(256, 256), 256);
+        case HALF: return 7 + 1.2 * steps * (double)ceil_div(count(256, 128), 256);
+        case BIG: return 6 + steps * (count(128, 128) <= 256 ? 0.95 : 1.7 * (double)ceil_div(count(128, 128), 512));
+        default: return 4 + steps * (count(64, 64) <= 256 ? 0.55 : 0.75 * (double)ceil_div(count(64, 64), 512));
+    }
 }
-double big_cost(int64_t rows, int64_t cols, int64_t splits) {
-    return 1.95 * (double)ceil_div(ceil_div(rows, 128) * ceil_div(cols, 128) * splits, 512);
-}
-Tiles choose_tiles(int64_t rows, int64_t cols) {
-    if (cols % 8 == 0 && wide_cost(rows, cols, 1) < big_cost(rows, cols, 1)) return WIDE;
-    return ceil_div(rows, 128) * ceil_div(cols, 128) >= 256 ? BIG : SMALL;
+Tiles choose_tiles(int64_t rows, int64_t cols, double steps) {
+    Tiles best = SMALL;
+    for (Tiles t : {BIG, HALF, WIDE})
+        if ((t == BIG || cols % 8 == 0) && tiles_cost(t, rows, cols, 1, steps) < tiles_cost(best, rows, cols, 1, steps)) best = t;
+    return best;
 }
 
 template <typename E, typename T, bool RT, bool CT> hipError_t launch_product(Product p, Tiles tiles, hipStream_t s) {
     switch (tiles) {
-        case WIDE: return launch_wide<E, T, RT, CT>(p, s);
+        case WIDE: return launch_wide<E, T, RT, CT, 4>(p, s);
+        case HALF: return launch_wide<E, T, RT, CT, 2>(p, s);
         case BIG: return launch_tiles<E, T, RT, CT, 2, 2, 4, 4, 64, 2, 2>(p, s);
         default: return launch_tiles<E, T, RT, CT, 2, 2, 2, 2, 64, 3, 2>(p, s);
     }
@@ -830,6 +839,7 @@ template <typename E, typename T, bool CT> hipError_t launch_rows(Product p, int
     const int64_t run = (int64_t)(1 << 22) / ceil_div(p.cols, 64) * 64;
     const char *r = (const char *)p.R.p;
     const int64_t ld = p.R.ld;
+    const double steps = (double)ceil_div(p.share, 64) * p.npair;
     T *out = (T *)p.out, *pre = (T *)p.pre;
     const T *res = (const T *)p.residual;
     for (int64_t first = 0; first < rows; first += run) {
@@ -839,7 +849,7 @@ template <typename E, typename T, bool CT> hipError_t launch_rows(Product p, int
         p.out = out + first * p.cols;
         p.pre = pre ? pre + first * p.cols : nullptr;
         p.residual = res ? res + first * p.cols : nullptr;
-        if (hipError_t e = launch_product<E, T, false, CT>(p, choose_tiles(p.rows, p.cols), s)) return e;
+        if (hipError_t e = launch_product<E, T, false, CT>(p, choose_tiles(p.rows, p.cols, steps), s)) return e;
     }
     return hipSuccess;
 }
@@ -903,16 +913,18 @@ Plan make_plan(const PointwiseArgs &a) {
     // shares of the rows: as many as give every CU its workgroups, each share at least four steps. The shares' sums are
     // written and read again: 8 bytes per output and share, at about 4 TB/s.
     const int64_t most_splits = std::max<int64_t>(1, a.rows / (4 * SHARE));
-    auto cost = [&](int64_t splits, double per_step) {
-        return per_step * (double)ceil_div(ceil_div(a.rows, splits), SHARE) + (splits > 1 ? (double)(splits * a.out) * a.in * 2e-6 : 0.0);
-    };
-    const int64_t t256 = ceil_div(a.out, 256) * ceil_div(a.in, 256), t128 = ceil_div(a.out, 128) * ceil_div(a.in, 128);
-    const int64_t s256 = std::min(std::max<int64_t>(1, 256 / t256), most_splits), s128 = std::min(std::max<int64_t>(1, 512 / t128), most_splits);
-    const bool wide256 = a.in % 8 == 0 && cost(s256, wide_cost(a.out, a.in, s256)) < cost(s128, big_cost(a.out, a.in, s128));
-    const int64_t splits = wide256 ? s256 : s128;
+    double least = 0;
+    int64_t splits = 0;
+    for (const auto &[t, r, c, slots] : {std::tuple<Tiles, int, int, int>{SMALL, 64, 64, 512}, {BIG, 128, 128, 256},
+                                         {BIG, 128, 128, 512}, {HALF, 256, 128, 256}, {WIDE, 256, 256, 256}}) {
+        if (t <= HALF && a.in % 8 != 0) continue;
+        const int64_t n = std::min(std::max<int64_t>(1, slots / (ceil_div(a.out, r) * ceil_div(a.in, c))), most_splits);
+        const double steps = (double)ceil_div(ceil_div(a.rows, n), SHARE) * k.np * (k.npx == 3 ? 2 : 1);
+        const double cost = tiles_cost(t, a.out, a.in, n, steps) + (n > 1 ? (double)(n * a.out) * a.in * 2e-6 : 0.0);
+        if (splits == 0 || cost < least) least = cost, splits = n, k.tiles = t;
+    }
     k.share = round_up(ceil_div(a.rows, splits), SHARE);
     k.splits = (int)ceil_div(a.rows, k.share < 1 ? 1 : k.share);
-    k.tiles = wide256 ? WIDE : t128 * k.splits >= 256 ? BIG : SMALL;
     k.sums_at = k.splits > 1 ? take((size_t)k.splits * a.out * a.in * 4) : 0;
     k.backward = off;
     return k;
