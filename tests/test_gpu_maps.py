@@ -41,7 +41,8 @@ def norm_case(shape, dtype, seed=0, **kw):
 NORM_SHAPES = [
     ((2, 8, 5, 3), 2), ((1, 3, 7), 1), ((3, 63, 11, 13), 7), ((2, 72, 9, 9), 9), ((1, 256, 33, 31), 32), ((37, 48), 3),
     ((1, 40, 1), 1), ((2, 5, 3, 2, 7), 5), ((1, 2064, 3, 2), 3), ((2, 2100, 5), 2), ((1, 1, 600), 1), ((5, 260, 70), 130),
-    ((1000, 16, 2), 2),
+    ((1000, 16, 2), 2), ((2, 64, 100, 110), 2), ((1, 33, 70, 80), 3), ((3, 256, 64, 64), 32), ((2, 128, 40, 41), 32),
+    ((1, 24, 2100), 3), ((4, 512, 4), 512), ((300, 96, 1, 1), 4),
 ]
 
 

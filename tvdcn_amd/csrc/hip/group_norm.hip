@@ -3,11 +3,13 @@
 //   n = (x - mean) rstd,  z = w n + b,  y = act(z);  mean and variance over the pixels and the Cg channels of a
 //   (batch, group);  dz = dy act'(z),  dn = w dz,  dx = rstd (dn - avg(dn) - n avg(dn n)),  dw = sum dz n,  db = sum dz
 //
-// Bound by memory. Forward: the statistics read x once, the second pass reads it again (from the 256 MB last-level
-// cache where it fits) and writes y. A workgroup takes a run of pixels of one image and all channels (in tiles of 256
+// Bound by memory. Groups that a workgroup can hold in registers are read once, in one launch (below). For larger ones the
+// statistics read x once, the second pass reads it again (from the 256 MB last-level cache where it fits) and writes y. A
+// workgroup takes a run of pixels of one image and all channels (in tiles of 256
 // lanes), so every access is a run of whole rows; a lane keeps its 16 bytes of channels over all its pixels, and with
 // them the parameters of those channels. Sums are float32, of deviations from the group's first value (large means
 // against small spreads do not cancel), combined in a fixed order.
+
 #include "maps.h"
 
 namespace tvdcn_hip {
@@ -423,15 +425,277 @@ __global__ void __launch_bounds__(TB) norm_dx_kernel(Source<T, VEC, KEPT> src, c
     }
 }
 
+// ---- whole groups: a group's values stay in registers between the sums and the results, so a map is read once and one launch
+// does it. TG lanes per group (several groups to a workgroup of 256 where TG < 256), NV accesses of VEC channels per lane. ----
+
+constexpr int block_of(int TG) { return TG > 256 ? TG : 256; }
+
+// Workgroups go to the 8 XCDs in turn: each gets a run of neighbouring groups, which share lines of the map in one L2
+__device__ __forceinline__ int64_t xcd_run(int64_t id, int64_t total) {
+    const int64_t per = total / 8, extra = total % 8, xcd = id % 8;
+    return xcd * per + (xcd < extra ? xcd : extra) + id / 8;
+}
+
+template <int TG> __device__ __forceinline__ float group_sum(float v, float *red, int t) {
+    constexpr int W = TG < 64 ? TG : 64;
+#pragma unroll
+    for (int m = 1; m < W; m <<= 1) v += __shfl_xor(v, m);
+    if constexpr (TG > 64) {
+        __syncthreads();   // (the last sum's values have been read)
+        if ((t & 63) == 0) red[t >> 6] = v;
+        __syncthreads();
+        v = 0.f;
+#pragma unroll
+        for (int w = 0; w < TG / 64; ++w) v += red[t / TG * (TG / 64) + w];
+    }
+    return v;
+}
+
+// A lane's place: group, first channel of its accesses, and its pixels first, first + rows, ...
+template <int TG, int VEC> struct Place {
+    int64_t bg, b;
+    int g, c0, first, rows, cv;
+    bool on;   // lanes beyond the last whole row of accesses, or beyond the groups, hold nothing
+    __device__ __forceinline__ Place(int64_t groups, int64_t blocks, int G, int Cg, int64_t P) {
+        const int t = threadIdx.x, l = t % TG;
+        bg = xcd_run(blockIdx.x, blocks) * (block_of(TG) / TG) + t / TG;
+        on = bg < groups;
+        if (!on) bg = groups - 1;
+        b = bg / G;
+        g = (int)(bg - b * G);
+        cv = Cg / VEC;
+        rows = TG / cv;
+        first = l / cv;
+        c0 = g * Cg + (l - first * cv) * VEC;
+        on = on && first < rows;
+        if (!on) first = (int)P;
+    }
+};
+
+template <typename T, int VEC, int TG, int NV>
+__global__ void __launch_bounds__(block_of(TG)) norm_group_kernel(const T *__restrict__ x, const void *__restrict__ w,
+                                                                  const void *__restrict__ bias, T *__restrict__ y,
+                                                                  float *__restrict__ mean, float *__restrict__ rstd,
+                                                                  int64_t groups, int64_t blocks, int64_t P, int C, int G, int Cg,
+                                                                  float eps, int act) {
+    __shared__ float red[block_of(TG) / 64];
+    const int t = threadIdx.x;
+    const Place<TG, VEC> at(groups, blocks, G, Cg, P);
+    const int64_t base = at.b * P * C + at.c0;
+    Pack<T, VEC> p[NV];
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int r = at.first + i * at.rows;
+        if (r < P) p[i] = *reinterpret_cast<const Pack<T, VEC> *>(x + base + (int64_t)r * C);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (at.first + i * at.rows < P)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) s += (float)p[i].v[v];
+    const float n = (float)(P * Cg), mu = group_sum<TG>(s, red, t) / n;
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (at.first + i * at.rows < P)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                const float d = (float)p[i].v[v] - mu;
+                s = fmaf(d, d, s);
+            }
+    const float rs = 1.f / sqrtf(group_sum<TG>(s, red, t) / n + eps);
+    if (!at.on) return;
+    if (t % TG == 0) mean[at.bg] = mu, rstd[at.bg] = rs;
+    float sc[VEC], bv[VEC];
+    params<T, VEC>(w, at.c0, sc, 1.f);
+    params<T, VEC>(bias, at.c0, bv, 0.f);
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) sc[v] *= rs;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int r = at.first + i * at.rows;
+        if (r >= P) break;
+        float z[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) z[v] = fmaf((float)p[i].v[v] - mu, sc[v], bv[v]);
+        act_values<is_f32<T>(), VEC>(z, act);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) p[i].v[v] = (T)z[v];
+        *reinterpret_cast<Pack<T, VEC> *>(y + base + (int64_t)r * C) = p[i];
+    }
+}
+
+// dx, and the group's sums of dz and dz n per channel: part[b * C + c], or dw and db themselves where there is one image. n and
+// dz stay in registers too, so these are smaller groups.
+template <typename T, int VEC, int TG, int NV, bool KEPT>
+__global__ void __launch_bounds__(block_of(TG))
+    norm_group_bwd_kernel(Source<T, VEC, KEPT> src, const T *__restrict__ dy, const void *__restrict__ w,
+                          const void *__restrict__ bias, const float *__restrict__ mean, const float *__restrict__ rstd,
+                          T *__restrict__ dx, float2 *__restrict__ part, T *__restrict__ dw, T *__restrict__ db,
+                          int64_t groups, int64_t blocks, int64_t P, int C, int G, int Cg, int act) {
+    __shared__ float2 sums[block_of(TG) * VEC];
+    float *red = (float *)sums;   // (before the sums)
+    const int t = threadIdx.x;
+    const Place<TG, VEC> at(groups, blocks, G, Cg, P);
+    const int64_t base = at.b * P * C + at.c0;
+    const float mu = mean[at.bg], rs = rstd[at.bg];
+    float wv[VEC], bv[VEC], s[VEC], q[VEC];
+    params<T, VEC>(w, at.c0, wv, 1.f);
+    params<T, VEC>(bias, at.c0, bv, 0.f);
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) s[v] = q[v] = 0.f;
+    float f[NV][VEC], d[NV][VEC];   // x, then n; dy, then dz
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int r = at.first + i * at.rows;
+        if (r < P) {
+            src.get(at.b * P + r, at.c0, f[i]);
+            const Pack<T, VEC> g = *reinterpret_cast<const Pack<T, VEC> *>(dy + base + (int64_t)r * C);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) d[i][v] = (float)g.v[v];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (at.first + i * at.rows < P) {
+            float z[VEC];
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                f[i][v] = (f[i][v] - mu) * rs;
+                z[v] = fmaf(f[i][v], wv[v], bv[v]);
+            }
+            act_slopes<is_f32<T>(), VEC>(d[i], z, act);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                s[v] += d[i][v];
+                q[v] = fmaf(d[i][v], f[i][v], q[v]);
+            }
+        }
+    float a1 = 0.f, a2 = 0.f;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) a1 = fmaf(s[v], wv[v], a1), a2 = fmaf(q[v], wv[v], a2);
+    const float n = (float)(P * Cg);
+    a1 = group_sum<TG>(a1, red, t) / n;
+    a2 = group_sum<TG>(a2, red, t) / n;
+    if (dx)
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int r = at.first + i * at.rows;
+            if (r >= P) break;
+            Pack<T, VEC> p;
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) p.v[v] = (T)(rs * (d[i][v] * wv[v] - a1 - f[i][v] * a2));
+            *reinterpret_cast<Pack<T, VEC> *>(dx + base + (int64_t)r * C) = p;
+        }
+    if (!part && !dw && !db) return;
+    // per channel: the lanes of its accesses, added up by one wave (or by the group's lanes) per channel
+    const int l = t % TG, own = t / TG * TG * VEC;
+    __syncthreads();
+    if (at.on)
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) sums[own + l * VEC + v] = make_float2(s[v], q[v]);
+    __syncthreads();
+    const int used = min(at.rows, (int)(P < TG ? P : TG));   // lanes along the pixels that held any
+    auto write = [&](int c, float sc, float qc) {
+        const int64_t to = at.b * C + at.g * Cg + c;
+        if (part) part[to] = make_float2(sc, qc);
+        if (!part && db) db[to] = (T)sc;
+        if (!part && dw) dw[to] = (T)qc;
+    };
+    const bool there = xcd_run(blockIdx.x, blocks) * (block_of(TG) / TG) + t / TG < groups;
+    if constexpr (TG > 64) {
+        for (int c = l >> 6; c < Cg; c += TG / 64) {
+            float sc = 0.f, qc = 0.f;
+            for (int r = l & 63; r < used; r += 64) {
+                const float2 a = sums[own + r * Cg + c];
+                sc += a.x, qc += a.y;
+            }
+            sc = wave_sum(sc);
+            qc = wave_sum(qc);
+            if ((l & 63) == 0 && there) write(c, sc, qc);
+        }
+    } else if (there) {
+        for (int c = l; c < Cg; c += TG) {
+            float sc = 0.f, qc = 0.f;
+            for (int r = 0; r < used; ++r) {
+                const float2 a = sums[own + r * Cg + c];
+                sc += a.x, qc += a.y;
+            }
+            write(c, sc, qc);
+        }
+    }
+}
+
+constexpr int64_t MOST_GROUPS = 1 << 22;   // a workgroup each: HIP takes fewer than 2^32 threads along x
+
+// What a group takes: lanes, and accesses per lane (0: a workgroup does not hold it, or not at a gain). Forward, groups of up to 64
+// / 512 / 4096 / 16384 / 65536 values of 16 bits whose channels come in eights (half as many float32 ones in fours; an eighth to
+// a half of that one by one): (8, 256, 64 x 64) in 32 groups 17.8 us instead of 25.5, (16, 512, 4096) 35.7 instead of 46.4,
+// bfloat16. Backward, up to 16384 (2048 one by one): (8, 256, 32 x 32) 13.7 us instead of 17.4; four times that does not fit
+// beside the sums and takes 35.3 instead of 33.1 read twice.
+struct Whole {
+    int TG, NV;
+};
+template <int VEC> Whole whole_of(const NormArgs &a, bool backward) {
+    const int Cg = a.channels / a.groups, cv = Cg / VEC;
+    if (Cg % VEC || a.batch * a.groups >= MOST_GROUPS) return {0, 0};
+    constexpr int FEW = VEC > 1 ? 2 : 8, MANY = VEC > 1 ? 8 : 32;
+    for (const Whole &k : {Whole{4, FEW}, Whole{32, FEW}, Whole{256, FEW}, Whole{256, MANY}, Whole{1024, MANY}}) {
+        if (backward && (k.TG == 1024 || k.NV == 32)) break;
+        if (cv <= k.TG && a.pixels <= (int64_t)(k.TG / cv) * k.NV) return k;
+    }
+    return {0, 0};
+}
+
 constexpr int64_t MOST_BLOCKS = 1 << 20;   // (HIP takes fewer than 2^32 threads along x; the kernels stride)
 dim3 grid_of(const Cut &k) { return dim3((unsigned)(k.units < MOST_BLOCKS ? k.units : MOST_BLOCKS), (unsigned)k.tiles); }
 unsigned grid_1d(int64_t n) { return (unsigned)(n < MOST_BLOCKS ? n : MOST_BLOCKS); }
 
-template <typename T> int vec_of(const NormArgs &a) { return a.channels % (16 / sizeof(T)) == 0 ? 16 / sizeof(T) : 1; }
-int vec_of(const NormArgs &a) { return a.dtype == TVDCN_DTYPE_FLOAT32 ? vec_of<float>(a) : vec_of<f16>(a); }
+// Channels per access: 16 bytes where the rows allow it. (Where the rows do and the groups do not, whole groups go one by one if
+// they fit, else the rows in whole accesses.)
+template <typename T> int vec_of(const NormArgs &a, bool backward) {
+    constexpr int V = 16 / sizeof(T);
+    if (a.channels % V) return 1;
+    return a.channels / a.groups % V && whole_of<1>(a, backward).TG ? 1 : V;
+}
+int vec_of(const NormArgs &a, bool backward) {
+    return a.dtype == TVDCN_DTYPE_FLOAT32 ? vec_of<float>(a, backward) : vec_of<f16>(a, backward);
+}
+
+template <typename T, int VEC, int TG, int NV> hipError_t forward_groups(const NormArgs &a, hipStream_t s) {
+    const int64_t groups = a.batch * a.groups, blocks = ceil_div(groups, block_of(TG) / TG);
+    norm_group_kernel<T, VEC, TG, NV><<<(unsigned)blocks, block_of(TG), 0, s>>>(
+        (const T *)a.x, a.weight, a.bias, (T *)a.y, a.mean, a.rstd, groups, blocks, a.pixels, a.channels, a.groups,
+        a.channels / a.groups, a.eps, a.act);
+    return hipGetLastError();
+}
+
+template <typename T, int VEC, int TG, int NV, bool KEPT> hipError_t backward_groups(const NormArgs &a, hipStream_t s) {
+    const int C = a.channels;
+    const int64_t groups = a.batch * a.groups, blocks = ceil_div(groups, block_of(TG) / TG);
+    const bool params = a.dweight || a.dbias, one = a.batch == 1;
+    float2 *part = params && !one ? (float2 *)a.part : nullptr;
+    const Source<T, VEC, KEPT> src{(const T *)a.x, a.codes, a.exps, C, (int)ceil_div(C, kKeptBlock)};
+    norm_group_bwd_kernel<T, VEC, TG, NV, KEPT><<<(unsigned)blocks, block_of(TG), 0, s>>>(
+        src, (const T *)a.dy, a.weight, a.bias, a.mean, a.rstd, (T *)a.dx, part, one ? (T *)a.dweight : nullptr,
+        one ? (T *)a.dbias : nullptr, groups, blocks, a.pixels, C, a.groups, C / a.groups, a.act);
+    if (hipError_t e = hipGetLastError()) return e;
+    if (part)
+        norm_bwd_finish_kernel<T><<<grid_1d(ceil_div(C, 16)), FIN, 0, s>>>(part, a.weight, nullptr, (T *)a.dweight, (T *)a.dbias,
+                                                                          0, 0, C, a.groups, C / a.groups, 0, a.batch);
+    return hipGetLastError();
+}
 
 template <typename T, int VEC> hipError_t forward(const NormArgs &a, hipStream_t s) {
     const int C = a.channels, G = a.groups, Cg = C / G;
+    constexpr int FEW = VEC > 1 ? 2 : 8, MANY = VEC > 1 ? 8 : 32;
+    if (const Whole k = whole_of<VEC>(a, false); k.TG) {
+        if (k.TG == 4) return forward_groups<T, VEC, 4, FEW>(a, s);
+        if (k.TG == 32) return forward_groups<T, VEC, 32, FEW>(a, s);
+        if (k.TG == 1024) return forward_groups<T, VEC, 1024, MANY>(a, s);
+        return k.NV == FEW ? forward_groups<T, VEC, 256, FEW>(a, s) : forward_groups<T, VEC, 256, MANY>(a, s);
+    }
     const Cut k = make_cut(a.batch, a.pixels, C, VEC);
     const T *x = (const T *)a.x;
     norm_stats_kernel<T, VEC><<<grid_of(k), TB, 0, s>>>(x, (float2 *)a.part, a.pixels, C, G, Cg, k);
@@ -452,6 +716,12 @@ template <typename T, int VEC, bool KEPT> hipError_t backward(const NormArgs &a,
                                                                              (T *)a.dbias, 0, 0, C, G, Cg, 0, 0);
         return hipGetLastError();
     }
+    constexpr int FEW = VEC > 1 ? 2 : 8;
+    if (const Whole k = whole_of<VEC>(a, true); k.TG) {
+        if (k.TG == 4) return backward_groups<T, VEC, 4, FEW, KEPT>(a, s);
+        if (k.TG == 32) return backward_groups<T, VEC, 32, FEW, KEPT>(a, s);
+        return k.NV == FEW ? backward_groups<T, VEC, 256, FEW, KEPT>(a, s) : backward_groups<T, VEC, 256, 8, KEPT>(a, s);
+    }
     const Cut k = make_cut(a.batch, a.pixels, C, VEC);
     const int64_t BG = a.batch * G;
     float2 *avg = (float2 *)a.part, *part = avg + BG;
@@ -470,18 +740,21 @@ template <typename T, int VEC, bool KEPT> hipError_t backward(const NormArgs &a,
 
 template <typename T> hipError_t forward_of(const NormArgs &a, hipStream_t s) {
     constexpr int V = 16 / sizeof(T);
-    return vec_of<T>(a) == V ? forward<T, V>(a, s) : forward<T, 1>(a, s);
+    return vec_of<T>(a, false) == V ? forward<T, V>(a, s) : forward<T, 1>(a, s);
 }
 template <typename T> hipError_t backward_of(const NormArgs &a, hipStream_t s) {
     constexpr int V = 16 / sizeof(T);
-    if (vec_of<T>(a) == V) return a.codes ? backward<T, V, true>(a, s) : backward<T, V, false>(a, s);
+    if (vec_of<T>(a, true) == V) return a.codes ? backward<T, V, true>(a, s) : backward<T, V, false>(a, s);
     return a.codes ? backward<T, 1, true>(a, s) : backward<T, 1, false>(a, s);
 }
 
 }  // namespace
 
 int64_t norm_part_floats(const NormArgs &a, bool backward) {
-    const Cut k = make_cut(a.batch, a.pixels, a.channels, vec_of(a));
+    const int vec = vec_of(a, backward);
+    const Whole whole = vec == 1 ? whole_of<1>(a, backward) : vec == 4 ? whole_of<4>(a, backward) : whole_of<8>(a, backward);
+    if (whole.TG) return backward && a.batch > 1 ? 2 * a.batch * a.channels : 0;
+    const Cut k = make_cut(a.batch, a.pixels, a.channels, vec);
     return backward ? 2 * (a.batch * a.groups + k.units * a.channels) : 2 * k.units * k.tiles * a.groups;
 }
 

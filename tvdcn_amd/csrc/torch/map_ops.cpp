@@ -66,13 +66,37 @@ void check_activation(int64_t activation, const char *name) {
     TORCH_CHECK(activation >= TVDCN_ACT_NONE && activation <= TVDCN_ACT_GELU, name, ": unknown activation ", activation);
 }
 
-// [batch, *size, channels], contiguous and 16-byte aligned
-Tensor to_rows(const Tensor &x) {
-    Tensor r = x.dim() == 2 ? x.contiguous() : x.movedim(1, -1).contiguous();
-    if (r.is_meta() || (reinterpret_cast<uintptr_t>(r.data_ptr()) & 15) == 0) return r;
-    return r.clone();
+// Dense channels-last memory: the last axes' strides under a channel stride of one
+bool is_rows(const Tensor &x) {
+    const auto sizes = x.sizes(), strides = x.strides();
+    const int64_t n = x.dim();
+    int64_t run = sizes[1];
+    if (sizes[1] > 1 && strides[1] != 1) return false;
+    for (int64_t i = n - 1; i >= 2; --i) {
+        if (sizes[i] > 1 && strides[i] != run) return false;
+        run *= sizes[i];
+    }
+    return sizes[0] <= 1 || strides[0] == run || x.numel() == 0;
 }
-Tensor to_rows(MaybeTensor x) { return has(x) ? to_rows(*x) : Tensor(); }
+bool is_aligned(const Tensor &x) { return x.is_meta() || (reinterpret_cast<uintptr_t>(x.data_ptr()) & 15) == 0; }
+// an empty map of these sizes in channels-last memory
+Tensor new_map(at::IntArrayRef sizes, const at::TensorOptions &options) {
+    const size_t n = sizes.size();
+    c10::SmallVector<int64_t, 6> strides(n);
+    int64_t run = 1;
+    strides[1] = run, run *= std::max<int64_t>(sizes[1], 1);
+    for (size_t i = n - 1; i >= 2; --i) strides[i] = run, run *= std::max<int64_t>(sizes[i], 1);
+    strides[0] = run;
+    return at::empty_strided(sizes, strides, options);
+}
+// the map with its channels contiguous per pixel, 16-byte aligned: itself, or a copy
+Tensor rows_of(const Tensor &x) {
+    if (is_rows(x) && is_aligned(x)) return x;
+    return new_map(x.sizes(), x.options()).copy_(x);
+}
+Tensor rows_of(MaybeTensor x) { return has(x) ? rows_of(*x) : Tensor(); }
+// [batch, *size, channels] (host kernels)
+Tensor to_rows(const Tensor &x) { return x.dim() == 2 ? x.contiguous() : x.movedim(1, -1).contiguous(); }
 Tensor flat(MaybeTensor v) {   // a parameter, contiguous and 16-byte aligned
     if (!has(v)) return Tensor();
     Tensor r = v->contiguous();
@@ -133,36 +157,35 @@ void check_expand(const Tensor &codes, const Tensor &exponents, at::ScalarType d
 Two compress_hip(const Tensor &x) {
     check_compress(x);
     c10::DeviceGuard guard(x.device());
-    const Tensor r = to_rows(x);
+    const Tensor r = rows_of(x);
     const int64_t C = x.size(1);
-    Tensor codes = new_rows(x, C, x.options().dtype(at::kChar));
-    Tensor exps = new_rows(x, blocks_of(C), x.options().dtype(at::kByte));
+    Tensor codes = new_map(x.sizes(), x.options().dtype(at::kChar));
+    Tensor exps = new_map(map_shape(x, blocks_of(C)), x.options().dtype(at::kByte));
     check_status(tvdcn_compress_activation(map_dtype(x.scalar_type(), COMPRESS), x.size(0) * pixels_of(x), C, ptr(r),
                                            (int8_t *)ptr(codes), (uint8_t *)ptr(exps), stream_of(x)),
                  COMPRESS);
-    return {to_map(codes), to_map(exps)};
+    return {codes, exps};
 }
 Tensor expand_hip(const Tensor &codes, const Tensor &exponents, at::ScalarType dtype) {
     check_expand(codes, exponents, dtype);
     c10::DeviceGuard guard(codes.device());
-    const Tensor q = to_rows(codes), e = to_rows(exponents);
+    const Tensor q = rows_of(codes), e = rows_of(exponents);
     const int64_t C = codes.size(1);
-    Tensor y = new_rows(codes, C, codes.options().dtype(dtype));
+    Tensor y = new_map(codes.sizes(), codes.options().dtype(dtype));
     check_status(tvdcn_expand_activation(map_dtype(dtype, EXPAND), codes.size(0) * pixels_of(codes), C, (const int8_t *)ptr(q),
                                          (const uint8_t *)ptr(e), ptr(y), stream_of(codes)),
                  EXPAND);
-    return to_map(y);
+    return y;
 }
 
 Two compress_meta(const Tensor &x) {
     check_compress(x);
     const int64_t C = x.size(1);
-    return {to_map(new_rows(x, C, x.options().dtype(at::kChar))),
-            to_map(new_rows(x, blocks_of(C), x.options().dtype(at::kByte)))};
+    return {new_map(x.sizes(), x.options().dtype(at::kChar)), new_map(map_shape(x, blocks_of(C)), x.options().dtype(at::kByte))};
 }
 Tensor expand_meta(const Tensor &codes, const Tensor &exponents, at::ScalarType dtype) {
     check_expand(codes, exponents, dtype);
-    return to_map(new_rows(codes, codes.size(1), codes.options().dtype(dtype)));
+    return new_map(codes.sizes(), codes.options().dtype(dtype));
 }
 
 Two compress_cpu(const Tensor &x) {
@@ -220,67 +243,73 @@ void check_source(const Tensor &grad, MaybeTensor input, MaybeTensor codes, Mayb
     }
 }
 void check_norm_backward(const Tensor &grad, MaybeTensor input, MaybeTensor codes, MaybeTensor exponents,
-                         MaybeTensor weight, MaybeTensor bias, const Tensor &mean, const Tensor &rstd,
-                         int64_t activation) {
+                         MaybeTensor weight, MaybeTensor bias, const Tensor &stats, int64_t activation) {
     check_map(grad, NORM);
     check_activation(activation, NORM);
     check_source(grad, input, codes, exponents, grad.size(1), NORM);
     check_like(grad, weight, "weight", {grad.size(1)}, NORM);
     check_like(grad, bias, "bias", {grad.size(1)}, NORM);
-    TORCH_CHECK(mean.dim() == 2 && mean.size(0) == grad.size(0) && mean.size(1) > 0 && grad.size(1) % mean.size(1) == 0 &&
-                    mean.sizes() == rstd.sizes() && mean.scalar_type() == rstd.scalar_type() &&
-                    mean.scalar_type() == (grad.scalar_type() == at::kDouble ? at::kDouble : at::kFloat) &&
-                    mean.device() == grad.device() && rstd.device() == grad.device(),
-                NORM, " backward: mean and rstd are not those of the forward");
+    TORCH_CHECK(stats.dim() == 3 && stats.size(0) == 2 && stats.size(1) == grad.size(0) && stats.size(2) > 0 &&
+                    grad.size(1) % stats.size(2) == 0 &&
+                    stats.scalar_type() == (grad.scalar_type() == at::kDouble ? at::kDouble : at::kFloat) &&
+                    stats.device() == grad.device(),
+                NORM, " backward: the statistics are not those of the forward");
 }
 
-Three norm_forward_hip(const Tensor &x, int64_t groups, MaybeTensor weight, MaybeTensor bias, double eps, int64_t act) {
+// y and the statistics (2, batch, groups): means, reciprocal deviations
+Two norm_forward_hip(const Tensor &x, int64_t groups, MaybeTensor weight, MaybeTensor bias, double eps, int64_t act) {
     check_norm(x, groups, weight, bias, eps, act);
     c10::DeviceGuard guard(x.device());
-    const Tensor r = to_rows(x), w = flat(weight), b = flat(bias);
+    const Tensor r = rows_of(x), w = flat(weight), b = flat(bias);
     const tvdcn_norm_desc d{map_dtype(x.scalar_type(), NORM), (int32_t)act, x.size(0), pixels_of(x), x.size(1), groups, eps};
-    Tensor y = new_rows(x, x.size(1), x.options());
-    const auto f32 = x.options().dtype(at::kFloat);
-    Tensor mean = at::empty({x.size(0), groups}, f32), rstd = at::empty({x.size(0), groups}, f32);
-    if (x.numel() == 0) return {to_map(y), mean.zero_(), rstd.zero_()};
+    // (the second half starts on a multiple of 16 bytes)
+    const int64_t half = (x.size(0) * groups + 3) / 4 * 4;
+    Tensor y = new_map(x.sizes(), x.options());
+    Tensor stats = at::empty_strided({2, x.size(0), groups}, {half, groups, 1}, x.options().dtype(at::kFloat));
+    if (x.numel() == 0) return {y, stats.zero_()};
     const size_t n = tvdcn_group_norm_act_forward_workspace_size(&d);
-    const Tensor work = bytes(x, n);
-    check_status(tvdcn_group_norm_act_forward(&d, ptr(r), ptr(w), ptr(b), ptr(y), (float *)ptr(mean), (float *)ptr(rstd),
-                                              ptr(work), n, stream_of(x)),
-                 NORM);
-    return {to_map(y), mean, rstd};
+    const Tensor work = n ? bytes(x, n) : Tensor();
+    float *mean = (float *)ptr(stats);
+    check_status(tvdcn_group_norm_act_forward(&d, ptr(r), ptr(w), ptr(b), ptr(y), mean, mean + half, ptr(work), n, stream_of(x)), NORM);
+    return {y, stats};
 }
 Three norm_backward_hip(const Tensor &grad, MaybeTensor input, MaybeTensor codes, MaybeTensor exponents, MaybeTensor weight,
-                        MaybeTensor bias, const Tensor &mean, const Tensor &rstd, int64_t act, std::array<bool, 3> want) {
-    check_norm_backward(grad, input, codes, exponents, weight, bias, mean, rstd, act);
+                        MaybeTensor bias, const Tensor &stats_, int64_t act, std::array<bool, 3> want) {
+    check_norm_backward(grad, input, codes, exponents, weight, bias, stats_, act);
     c10::DeviceGuard guard(grad.device());
-    const Tensor g = to_rows(grad), r = to_rows(input), q = to_rows(codes), e = to_rows(exponents);
-    const Tensor w = flat(weight), b = flat(bias), mu = flat(maybe(mean)), rs = flat(maybe(rstd));
-    const int64_t C = grad.size(1);
-    const tvdcn_norm_desc d{map_dtype(grad.scalar_type(), NORM), (int32_t)act, grad.size(0), pixels_of(grad), C, mean.size(1), 0.0};
+    const Tensor g = rows_of(grad), r = rows_of(input), q = rows_of(codes), e = rows_of(exponents);
+    const Tensor w = flat(weight), b = flat(bias);
+    const int64_t C = grad.size(1), groups = stats_.size(2);
+    Tensor stats = stats_;
+    if (stats.numel() > 0 && (stats.stride(2) != 1 || (stats.size(1) > 1 && stats.stride(1) != groups) || stats.stride(0) % 4 || !is_aligned(stats))) {
+        stats = at::empty_strided(stats_.sizes(), {(grad.size(0) * groups + 3) / 4 * 4, groups, 1}, stats_.options());
+        stats.copy_(stats_);
+    }
+    const float *mean = (const float *)ptr(stats);
+    const tvdcn_norm_desc d{map_dtype(grad.scalar_type(), NORM), (int32_t)act, grad.size(0), pixels_of(grad), C, groups, 0.0};
     Tensor dx, dw, db;
-    if (want[0]) dx = new_rows(grad, C, grad.options());
+    if (want[0]) dx = new_map(grad.sizes(), grad.options());
     if (want[1]) dw = at::empty({C}, grad.options());
     if (want[2]) db = at::empty({C}, grad.options());
     const size_t n = tvdcn_group_norm_act_backward_workspace_size(&d);
-    const Tensor work = bytes(grad, n);
+    const Tensor work = n ? bytes(grad, n) : Tensor();
     check_status(tvdcn_group_norm_act_backward(&d, ptr(g), ptr(r), (const int8_t *)ptr(q), (const uint8_t *)ptr(e), ptr(w), ptr(b),
-                                               (const float *)ptr(mu), (const float *)ptr(rs), ptr(dx), ptr(dw), ptr(db),
+                                               mean, mean ? mean + stats.stride(0) : nullptr, ptr(dx), ptr(dw), ptr(db),
                                                ptr(work), n, stream_of(grad)),
                  "group_norm_act backward");
-    return {dx.defined() ? to_map(dx) : dx, dw, db};
+    return {dx, dw, db};
 }
 
-Three norm_forward_meta(const Tensor &x, int64_t groups, MaybeTensor weight, MaybeTensor bias, double eps, int64_t act) {
+Two norm_forward_meta(const Tensor &x, int64_t groups, MaybeTensor weight, MaybeTensor bias, double eps, int64_t act) {
     check_norm(x, groups, weight, bias, eps, act);
     const auto o = x.options().dtype(x.scalar_type() == at::kDouble ? at::kDouble : at::kFloat);
-    return {to_map(new_rows(x, x.size(1), x.options())), at::empty({x.size(0), groups}, o), at::empty({x.size(0), groups}, o)};
+    return {new_map(x.sizes(), x.options()), at::empty({2, x.size(0), groups}, o)};
 }
 Three norm_backward_meta(const Tensor &grad, MaybeTensor input, MaybeTensor codes, MaybeTensor exponents, MaybeTensor weight,
-                         MaybeTensor bias, const Tensor &mean, const Tensor &rstd, int64_t act, std::array<bool, 3> want) {
-    check_norm_backward(grad, input, codes, exponents, weight, bias, mean, rstd, act);
+                         MaybeTensor bias, const Tensor &stats, int64_t act, std::array<bool, 3> want) {
+    check_norm_backward(grad, input, codes, exponents, weight, bias, stats, act);
     const int64_t C = grad.size(1);
-    return {want[0] ? to_map(new_rows(grad, C, grad.options())) : Tensor(), want[1] ? at::empty({C}, grad.options()) : Tensor(),
+    return {want[0] ? new_map(grad.sizes(), grad.options()) : Tensor(), want[1] ? at::empty({C}, grad.options()) : Tensor(),
             want[2] ? at::empty({C}, grad.options()) : Tensor()};
 }
 
@@ -315,36 +344,31 @@ NormRows norm_rows(const Tensor &map, int64_t groups, MaybeTensor weight, MaybeT
     return {map.to(t).reshape({map.size(0), -1, groups, Cg}), param(weight, 1.0), param(bias, 0.0)};
 }
 
-Three norm_forward_cpu(const Tensor &x, int64_t groups, MaybeTensor weight, MaybeTensor bias, double eps, int64_t act) {
+Two norm_forward_cpu(const Tensor &x, int64_t groups, MaybeTensor weight, MaybeTensor bias, double eps, int64_t act) {
     check_norm(x, groups, weight, bias, eps, act);
-    const auto t = wide_type(x);
-    if (x.numel() == 0) {
-        const Tensor zero = at::zeros({x.size(0), groups}, x.options().dtype(t));
-        return {to_map(new_rows(x, x.size(1), x.options())), zero, zero.clone()};
-    }
+    if (x.numel() == 0) return {new_map(x.sizes(), x.options()), at::zeros({2, x.size(0), groups}, x.options().dtype(wide_type(x)))};
     const Tensor rows = to_rows(x);
     const NormRows n = norm_rows(rows, groups, weight, bias);
     const Tensor mean = n.x.mean(at::IntArrayRef({1, 3}), true), d = n.x - mean;
     const Tensor rstd = at::rsqrt(d.square().mean(at::IntArrayRef({1, 3}), true) + eps);
     const Tensor y = act_value(d * rstd * n.w + n.b, act).to(x.scalar_type()).reshape(rows.sizes());
-    return {to_map(y), mean.reshape({x.size(0), groups}), rstd.reshape({x.size(0), groups})};
+    return {to_map(y), at::stack({mean.reshape({x.size(0), groups}), rstd.reshape({x.size(0), groups})})};
 }
 Three norm_backward_cpu(const Tensor &grad, MaybeTensor input, MaybeTensor codes, MaybeTensor exponents, MaybeTensor weight,
-                        MaybeTensor bias, const Tensor &mean, const Tensor &rstd, int64_t act, std::array<bool, 3> want) {
-    check_norm_backward(grad, input, codes, exponents, weight, bias, mean, rstd, act);
-    const int64_t C = grad.size(1), groups = mean.size(1);
+                        MaybeTensor bias, const Tensor &stats, int64_t act, std::array<bool, 3> want) {
+    check_norm_backward(grad, input, codes, exponents, weight, bias, stats, act);
+    const int64_t C = grad.size(1), groups = stats.size(2);
     const auto t = grad.scalar_type();
     if (grad.numel() == 0)
-        return {want[0] ? to_map(new_rows(grad, C, grad.options())) : Tensor(), want[1] ? at::zeros({C}, grad.options()) : Tensor(),
+        return {want[0] ? new_map(grad.sizes(), grad.options()) : Tensor(), want[1] ? at::zeros({C}, grad.options()) : Tensor(),
                 want[2] ? at::zeros({C}, grad.options()) : Tensor()};
     const Tensor rows = to_rows(grad);
     const Tensor src = has(input) ? to_rows(*input) : expand_rows(*codes, *exponents, t).to(at::kFloat);
     const NormRows n = norm_rows(src, groups, weight, bias);
-    const Tensor rs = rstd.reshape({-1, 1, groups, 1}), h = (n.x - mean.reshape({-1, 1, groups, 1})) * rs;
+    const Tensor rs = stats[1].reshape({-1, 1, groups, 1}), h = (n.x - stats[0].reshape({-1, 1, groups, 1})) * rs;
     const Tensor dz = rows.to(wide_type(grad)).reshape(n.x.sizes()) * act_slope(h * n.w + n.b, act), dn = dz * n.w;
     Tensor dx, dw, db;
-    if (want[0])
-        dx = to_map((rs * (dn - dn.mean(at::IntArrayRef({1, 3}), true) - h * (dn * h).mean(at::IntArrayRef({1, 3}), true))).to(t).reshape(rows.sizes()));
+    if (want[0]) dx = to_map((rs * (dn - dn.mean(at::IntArrayRef({1, 3}), true) - h * (dn * h).mean(at::IntArrayRef({1, 3}), true))).to(t).reshape(rows.sizes()));
     if (want[1]) dw = (dz * h).sum(at::IntArrayRef({0, 1})).reshape({C}).to(t);
     if (want[2]) db = dz.sum(at::IntArrayRef({0, 1})).reshape({C}).to(t);
     return {dx, dw, db};
@@ -383,49 +407,49 @@ Two point_forward_hip(const Tensor &x, const Tensor &weight, MaybeTensor bias, M
                       bool save_pre) {
     check_pointwise(x, weight, bias, residual, act);
     c10::DeviceGuard guard(x.device());
-    const Tensor r = to_rows(x), w = flat(maybe(weight)), b = flat(bias), res = to_rows(residual);
+    const Tensor r = rows_of(x), w = flat(maybe(weight)), b = flat(bias), res = rows_of(residual);
     const int64_t N = weight.size(0);
     const tvdcn_pointwise_desc d{map_dtype(x.scalar_type(), POINT), (int32_t)act, x.size(0) * pixels_of(x), x.size(1), N};
-    Tensor y = new_rows(x, N, x.options()), pre;
-    pre = save_pre ? at::empty_like(y) : at::empty({0}, x.options());
+    Tensor y = new_map(map_shape(x, N), x.options());
+    Tensor pre = save_pre ? new_map(y.sizes(), x.options()) : Tensor();
     const size_t n = tvdcn_pointwise_conv_forward_workspace_size(&d);
     const Tensor work = n ? bytes(x, n) : Tensor();
-    check_status(tvdcn_pointwise_conv_forward(&d, ptr(r), ptr(w), ptr(b), ptr(res), ptr(y), save_pre ? ptr(pre) : nullptr,
+    check_status(tvdcn_pointwise_conv_forward(&d, ptr(r), ptr(w), ptr(b), ptr(res), ptr(y), ptr(pre),
                                               ptr(work), n, stream_of(x)),
                  POINT);
-    return {to_map(y), save_pre ? to_map(pre) : pre};
+    return {y, pre};
 }
 Three point_backward_hip(const Tensor &grad, MaybeTensor input, MaybeTensor codes, MaybeTensor exponents, const Tensor &weight,
                          MaybeTensor pre, int64_t act, std::array<bool, 3> want) {
     check_pointwise_backward(grad, input, codes, exponents, weight, pre, act);
     c10::DeviceGuard guard(grad.device());
-    const Tensor g = to_rows(grad), r = to_rows(input), q = to_rows(codes), e = to_rows(exponents), p = to_rows(pre);
+    const Tensor g = rows_of(grad), r = rows_of(input), q = rows_of(codes), e = rows_of(exponents), p = rows_of(pre);
     const Tensor w = flat(maybe(weight));
     const int64_t N = weight.size(0), K = weight.size(1);
     const tvdcn_pointwise_desc d{map_dtype(grad.scalar_type(), POINT), (int32_t)act, grad.size(0) * pixels_of(grad), K, N};
     Tensor dx, dw, db;
-    if (want[0]) dx = new_rows(grad, K, grad.options());
+    if (want[0]) dx = new_map(map_shape(grad, K), grad.options());
     if (want[1]) dw = at::empty({N, K}, grad.options());
     if (want[2]) db = at::empty({N}, grad.options());
     const size_t n = tvdcn_pointwise_conv_backward_workspace_size(&d, has(codes));
-    const Tensor work = bytes(grad, n);
+    const Tensor work = n ? bytes(grad, n) : Tensor();
     check_status(tvdcn_pointwise_conv_backward(&d, ptr(g), ptr(r), (const int8_t *)ptr(q), (const uint8_t *)ptr(e), ptr(w), ptr(p),
                                                ptr(dx), ptr(dw), ptr(db), ptr(work), n, stream_of(grad)),
                  "pointwise_conv backward");
-    return {dx.defined() ? to_map(dx) : dx, dw, db};
+    return {dx, dw, db};
 }
 
 Two point_forward_meta(const Tensor &x, const Tensor &weight, MaybeTensor bias, MaybeTensor residual, int64_t act,
                        bool save_pre) {
     check_pointwise(x, weight, bias, residual, act);
-    return {to_map(new_rows(x, weight.size(0), x.options())),
-            save_pre ? to_map(new_rows(x, weight.size(0), x.options())) : at::empty({0}, x.options())};
+    const auto shape = map_shape(x, weight.size(0));
+    return {new_map(shape, x.options()), save_pre ? new_map(shape, x.options()) : Tensor()};
 }
 Three point_backward_meta(const Tensor &grad, MaybeTensor input, MaybeTensor codes, MaybeTensor exponents,
                           const Tensor &weight, MaybeTensor pre, int64_t act, std::array<bool, 3> want) {
     check_pointwise_backward(grad, input, codes, exponents, weight, pre, act);
     const auto o = grad.options();
-    return {want[0] ? to_map(new_rows(grad, weight.size(1), o)) : Tensor(), want[1] ? at::empty(weight.sizes(), o) : Tensor(),
+    return {want[0] ? new_map(map_shape(grad, weight.size(1)), o) : Tensor(), want[1] ? at::empty(weight.sizes(), o) : Tensor(),
             want[2] ? at::empty({weight.size(0)}, o) : Tensor()};
 }
 
@@ -440,7 +464,7 @@ Two point_forward_cpu(const Tensor &x, const Tensor &weight, MaybeTensor bias, M
     Tensor v = act_value(z, act);
     if (has(residual)) v = v + to_rows(*residual).to(t).reshape(v.sizes());
     return {to_map(v.to(x.scalar_type()).reshape(y.sizes())),
-            save_pre ? to_map(z.to(x.scalar_type()).reshape(y.sizes())) : at::empty({0}, x.options())};
+            save_pre ? to_map(z.to(x.scalar_type()).reshape(y.sizes())) : Tensor()};
 }
 Three point_backward_cpu(const Tensor &grad, MaybeTensor input, MaybeTensor codes, MaybeTensor exponents, const Tensor &weight,
                          MaybeTensor pre, int64_t act, std::array<bool, 3> want) {
@@ -462,9 +486,9 @@ Three point_backward_cpu(const Tensor &grad, MaybeTensor input, MaybeTensor code
 // ---------------------------------------------------------------------------
 // dispatch, autograd, autocast
 // ---------------------------------------------------------------------------
-using NormFwd = Three(const Tensor &, int64_t, MaybeTensor, MaybeTensor, double, int64_t);
+using NormFwd = Two(const Tensor &, int64_t, MaybeTensor, MaybeTensor, double, int64_t);
 using NormBwd = Three(const Tensor &, MaybeTensor, MaybeTensor, MaybeTensor, MaybeTensor, MaybeTensor, const Tensor &,
-                      const Tensor &, int64_t, std::array<bool, 3>);
+                      int64_t, std::array<bool, 3>);
 using PointFwd = Two(const Tensor &, const Tensor &, MaybeTensor, MaybeTensor, int64_t, bool);
 using PointBwd = Three(const Tensor &, MaybeTensor, MaybeTensor, MaybeTensor, const Tensor &, MaybeTensor, int64_t,
                        std::array<bool, 3>);
@@ -530,13 +554,13 @@ class NormFunction : public torch::autograd::Function<NormFunction> {
     static Tensor forward(AutogradContext *ctx, const Tensor &x, int64_t groups, MaybeTensor weight, MaybeTensor bias,
                           double eps, int64_t act, bool keep_int8) {
         at::AutoDispatchBelowADInplaceOrView guard;
-        Three r = norm_fwd().call(x, groups, weight, bias, eps, act);
+        Two r = norm_fwd().call(x, groups, weight, bias, eps, act);
         Tensor input = x, codes, exps;
         if (keep_int8) {
             std::tie(codes, exps) = compress_op().call(x);
             input = Tensor();
         }
-        ctx->save_for_backward({input, codes, exps, get(weight), get(bias), std::get<1>(r), std::get<2>(r)});
+        ctx->save_for_backward({input, codes, exps, get(weight), get(bias), std::get<1>(r)});
         ctx->saved_data["act"] = act;
         ctx->saved_data["weight"] = (int64_t)(has(weight) ? 1 : -1);
         ctx->saved_data["bias"] = (int64_t)(has(bias) ? 1 + has(weight) : -1);
@@ -548,7 +572,7 @@ class NormFunction : public torch::autograd::Function<NormFunction> {
         Three r;
         {
             at::AutoDispatchBelowADInplaceOrView guard;
-            r = norm_bwd().call(g[0], maybe(s[0]), maybe(s[1]), maybe(s[2]), maybe(s[3]), maybe(s[4]), s[5], s[6],
+            r = norm_bwd().call(g[0], maybe(s[0]), maybe(s[1]), maybe(s[2]), maybe(s[3]), maybe(s[4]), s[5],
                                 ctx->saved_data["act"].toInt(), want);
         }
         const variable_list d = with_node(r, {g[0], s[0], s[3], s[4]}, NORM);
@@ -653,9 +677,9 @@ TORCH_LIBRARY_FRAGMENT(tvdcn, m) {
     m.def("group_norm_act(Tensor input, int num_groups, Tensor? weight=None, Tensor? bias=None, float eps=1e-05, "
           "int activation=0, bool keep_int8=False) -> Tensor");
     m.def("_group_norm_act_forward(Tensor input, int num_groups, Tensor? weight, Tensor? bias, float eps, "
-          "int activation) -> (Tensor, Tensor, Tensor)");
+          "int activation) -> (Tensor, Tensor)");
     m.def("_group_norm_act_backward(Tensor grad, Tensor? input, Tensor? codes, Tensor? exponents, Tensor? weight, "
-          "Tensor? bias, Tensor mean, Tensor rstd, int activation, bool[3] output_mask) -> (Tensor, Tensor, Tensor)");
+          "Tensor? bias, Tensor stats, int activation, bool[3] output_mask) -> (Tensor, Tensor, Tensor)");
     m.def("pointwise_conv(Tensor input, Tensor weight, Tensor? bias=None, Tensor? residual=None, int activation=0, "
           "bool keep_int8=False) -> Tensor");
     m.def("_pointwise_conv_forward(Tensor input, Tensor weight, Tensor? bias, Tensor? residual, int activation, "
