@@ -56,9 +56,7 @@ template <typename T, int VEC, bool KEPT> struct Source {
     __device__ __forceinline__ void get(int64_t row, int c, float *f) const {
         if constexpr (KEPT) {
             const Pack<int8_t, VEC> q = *reinterpret_cast<const Pack<int8_t, VEC> *>(codes + row * C + c);
-            const float scale = kept_scale<T>(exps[row * blocks + c / kKeptBlock]);
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) f[v] = kept_value<T>(q.v[v], scale);
+            kept_values<T, VEC>(q.v, exps[row * blocks + c / kKeptBlock], f);
         } else {
             const Pack<T, VEC> p = *reinterpret_cast<const Pack<T, VEC> *>(x + row * C + c);
 #pragma unroll

@@ -66,13 +66,13 @@ __global__ void __launch_bounds__(TB) expand_kernel(const int8_t *__restrict__ c
         Pack<D, VEC> p{};
         if (c < C) {
             const Pack<int8_t, VEC> q = *reinterpret_cast<const Pack<int8_t, VEC> *>(codes + row * C + c);
-            const float scale = kept_scale<T>(exps[row * blocks + c / kKeptBlock]);
+            float f[VEC];
+            kept_values<T, VEC>(q.v, exps[row * blocks + c / kKeptBlock], f);
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
-                float f = kept_value<T>(q.v[v], scale);
                 // (the one value beyond bfloat16 that a float32 block can stand for is the clamp itself)
-                if (sizeof(D) < sizeof(T) && f == f) f = fminf(fmaxf(f, -most<D>()), most<D>());
-                p.v[v] = (D)f;
+                if (sizeof(D) < sizeof(T) && f[v] == f[v]) f[v] = fminf(fmaxf(f[v], -most<D>()), most<D>());
+                p.v[v] = (D)f[v];
             }
         }
         *reinterpret_cast<Pack<D, VEC> *>(y + row * pitch + c) = p;

@@ -152,14 +152,20 @@ template <> __device__ __forceinline__ float most<float>() { return 3.402823466e
 template <> __device__ __forceinline__ float most<f16>() { return 65504.f; }
 template <> __device__ __forceinline__ float most<bf16>() { return 3.389531390e38f; }
 
-// What code q of exponent byte e stands for: q * 2^(e - bias) clamped to T's finite values (128 q' 2^k may pass them by
-// its rounding), NaN for a block that held a value that is not finite. The scaling is exact.
+// What code q of exponent byte e stands for: q * 2^(e - bias) clamped to T's finite values, NaN for a block that held a value
+// that is not finite. The scaling is exact; only 64 and more steps of the largest exponent of all pass the finite values.
 template <typename T> __device__ __forceinline__ float kept_scale(uint8_t e) {
     return e == kKeptNaN ? __builtin_nanf("") : __uint_as_float((uint32_t)e << 23);
 }
-template <typename T> __device__ __forceinline__ float kept_value(int8_t q, float scale) {
-    const float v = (float)q * scale;
-    return v != v ? v : fminf(fmaxf(v, -most<T>()), most<T>());
+template <typename T> __device__ __forceinline__ float most_scale() { return 5.316911983e36f; }   // 2^122
+template <> __device__ __forceinline__ float most_scale<f16>() { return 1024.f; }
+template <typename T, int N> __device__ __forceinline__ void kept_values(const int8_t *q, uint8_t e, float *f) {
+    const float scale = kept_scale<T>(e);
+#pragma unroll
+    for (int v = 0; v < N; ++v) f[v] = (float)q[v] * scale;
+    if (scale >= most_scale<T>())
+#pragma unroll
+        for (int v = 0; v < N; ++v) f[v] = fminf(fmaxf(f[v], -most<T>()), most<T>());
 }
 
 }  // namespace tvdcn_hip

@@ -357,6 +357,69 @@ template <bool TM, bool PERM> struct SubTile {
     }
 };
 
+// The results of a tile of 256 rows: acc[i][j] are the fragments of columns i and rows j, `first` + 32 j this lane's rows, col0 its
+// wave's first column, q its quarter of a fragment's columns.
+template <typename T, bool CT, int FC>
+__device__ __forceinline__ void store_results(const Product &p, const fvec4 (&acc)[FC][8], int split, int first, int col0, int q) {
+            // Results: a lane's columns are the same in all its rows. What is read on the way comes ahead of its use: the bias once,
+            // the residual a row ahead of the stores.
+            constexpr int RUN = CT ? 4 : 8, RUNS = 4 * FC / RUN;
+            typedef Pack<T, RUN> Run;
+            const int colbase = col0 + q * RUN;
+            auto col_of = [&](int r) { return colbase + r * 4 * RUN; };
+            Run bias[RUNS] = {}, ahead_r[RUNS] = {};
+            auto residual = [&](int row) {
+#pragma unroll
+                for (int r = 0; r < RUNS; ++r)
+                    if (row < p.rows && col_of(r) < p.cols)
+                        ahead_r[r] = *reinterpret_cast<const Run *>((const T *)p.residual + (int64_t)row * p.cols + col_of(r));
+            };
+            if (p.bias)
+#pragma unroll
+                for (int r = 0; r < RUNS; ++r)
+                    if (col_of(r) < p.cols) bias[r] = *reinterpret_cast<const Run *>((const T *)p.bias + col_of(r));
+            if (p.residual) residual(first);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int row = first + j * 32;
+                Run res[RUNS];
+#pragma unroll
+                for (int r = 0; r < RUNS; ++r) res[r] = ahead_r[r];
+                if (p.residual && j < 7) residual(row + 32);
+#pragma unroll
+                for (int r = 0; r < RUNS; ++r) {
+                    const int col = col_of(r);
+                    float v[RUN];
+#pragma unroll
+                    for (int e = 0; e < RUN; ++e) v[e] = CT ? acc[r][j][e] : acc[r * 2 + e / 4][j][e % 4];
+                    if (row >= p.rows || col >= p.cols) continue;
+                    const int64_t at_o = (int64_t)row * p.cols + col;
+                    if (p.sums) {
+                        float *o = (float *)p.out + (int64_t)split * p.rows * p.cols + at_o;
+#pragma unroll
+                        for (int e = 0; e < RUN; e += 4) *reinterpret_cast<fvec4 *>(o + e) = fvec4{v[e], v[e + 1], v[e + 2], v[e + 3]};
+                        continue;
+                    }
+                    Run o;
+                    if (p.bias)
+#pragma unroll
+                        for (int e = 0; e < RUN; ++e) v[e] += (float)bias[r].v[e];
+                    if (p.pre) {
+#pragma unroll
+                        for (int e = 0; e < RUN; ++e) o.v[e] = (T)v[e];
+                        *reinterpret_cast<Run *>((T *)p.pre + at_o) = o;
+                    }
+                    act_values<is_f32<T>(), RUN>(v, p.act);
+                    if (p.residual)
+#pragma unroll
+                        for (int e = 0; e < RUN; ++e) v[e] += (float)res[r].v[e];
+#pragma unroll
+                    for (int e = 0; e < RUN; ++e) o.v[e] = (T)v[e];
+                    *reinterpret_cast<Run *>((T *)p.out + at_o) = o;
+                }
+            }
+}
+
 // A workgroup's tiles: the XCD's run of neighbouring ones (columns first), its workgroups in turn
 struct WideTiles {
     int first, step, count;
@@ -370,7 +433,7 @@ struct WideTiles {
 };
 // Tiles go through eight columns of them at a time, rows behind: a run of 32 (an XCD's workgroups) is then about as wide as it
 // is high, and shares most of what it reads.
-template <int BC> struct WideTile {
+template <int BC, int STEP = 64> struct WideTile {
     int split, row0, col0, nk;
     int64_t kbeg;
     __device__ __forceinline__ WideTile(const Product &p, int tile) {
@@ -383,41 +446,41 @@ template <int BC> struct WideTile {
         const int64_t kall = p.R.lim > p.C.lim ? p.R.lim : p.C.lim;
         kbeg = split * p.share;
         const int64_t kend = kbeg + p.share < kall ? kbeg + p.share : kall;
-        nk = (int)((kend - kbeg + 63) / 64);
+        nk = (int)((kend - kbeg + STEP - 1) / STEP);
     }
 };
 
 // Where a workgroup's loads of one operand are: the stage's base, and how many bytes from a sub-tile's first element on are
 // its own (rows, or columns of the last t, behind the edge are then read as zeros)
-template <bool TM, int B> struct WideSource {
+template <bool TM, int B, int STEP = 64> struct WideSource {
     uint64_t base, step;     // of a stage; from sub-tile to sub-tile
     int inside;              // output indexes from the tile's first one on
     uint32_t rows;           // t-major: the bytes of the stage's t before the last one
     uint32_t pitch;          // bytes
     uint32_t off;            // the lane's offset, past the end where its reduction indexes are
     int stages, tail;        // from this one to the operand's end, and the length of the last of them
+    __device__ __forceinline__ int left() const { return stages > 1 ? STEP : tail; }
     __device__ __forceinline__ void trim(uint32_t lane_off, int lane_at) {
-        const int left = stages > 1 ? 64 : tail;
-        if (TM) rows = (uint32_t)(left - 1) * pitch, off = lane_off;
-        else off = lane_at < left ? lane_off : 0x80000000u;
+        if (TM) rows = (uint32_t)(left() - 1) * pitch, off = lane_off;
+        else off = lane_at < left() ? lane_off : 0x80000000u;
     }
     __device__ __forceinline__ void enter(const Operand &o, int piece, int first, int64_t k0, uint32_t lane_off, int lane_at) {
         base = (uint64_t)o.p + 2 * (uint64_t)(o.plane * piece + (TM ? k0 * o.ld + first : first * o.ld + k0));
         inside = __builtin_amdgcn_readfirstlane((int)(o.width - first < B ? o.width - first : B));
         pitch = 2u * (uint32_t)o.ld;
         step = TM ? 128 : 64 * (uint64_t)pitch;
-        const int64_t t = o.lim - k0, n = (t + 63) >> 6;
+        const int64_t t = o.lim - k0, n = (t + STEP - 1) / STEP;
         stages = __builtin_amdgcn_readfirstlane((int)(n < (1 << 30) ? n : 1 << 30));
-        tail = (((int)t - 1) & 63) + 1;
+        tail = (((int)t - 1) & (STEP - 1)) + 1;
         trim(lane_off, lane_at);
     }
     __device__ __forceinline__ void advance(uint32_t lane_off, int lane_at) {
-        base += TM ? 64 * (uint64_t)pitch : 128;
+        base += TM ? STEP * (uint64_t)pitch : 2 * STEP;
         --stages;
         trim(lane_off, lane_at);
     }
-    __device__ __forceinline__ u32x4 descriptor(int q) const {
-        const uint64_t b = base + q * step;
+    __device__ __forceinline__ u32x4 descriptor(int q, uint64_t beyond = 0) const {
+        const uint64_t b = base + q * step + beyond;
         const int n = min(max(inside - 64 * q, 0), 64);
         const uint32_t bytes = TM ? (n ? rows + 2u * n : 0u) : (uint32_t)n * pitch;
         // (uniform, which the compiler does not always see)
@@ -426,7 +489,8 @@ template <bool TM, int B> struct WideSource {
     }
 };
 
-template <typename E, typename T, bool RT, bool CT, int FC> __global__ void __launch_bounds__(512, 2) wide_product_kernel(Product p) {
+template <typename E, typename T, bool RT, bool CT, int FC>
+__global__ void __launch_bounds__(512, 2) wide_product_kernel(Product p) {
     constexpr int BC = 64 * FC, COLS = 32768, STAGE = COLS + BC * 128;   // bytes; the columns' sub-tiles follow the rows'
     extern __shared__ __align__(1024) char smem[];
     typedef SubTile<RT, false> SR;
@@ -544,63 +608,198 @@ template <typename E, typename T, bool RT, bool CT, int FC> __global__ void __la
             phase(std::integral_constant<int, 3>());
         }
         if (!wr) asm volatile("s_barrier" ::: "memory");   // level again
-        // Results: a lane's columns are the same in all its rows. What is read on the way comes ahead of its use: the bias once,
-        // the residual a row ahead of the stores.
-        constexpr int RUN = CT ? 4 : 8, RUNS = 4 * FC / RUN;
-        typedef Pack<T, RUN> Run;
-        const int q = lane >> 4, colbase = tile.col0 + wc * 16 * FC + q * RUN, first = tile.row0 + wr * 16 + (lane & 15);
-        auto col_of = [&](int r) { return colbase + r * 4 * RUN; };
-        Run bias[RUNS] = {}, ahead_r[RUNS] = {};
-        auto residual = [&](int row) {
+        store_results<T, CT, FC>(p, acc, tile.split, tile.row0 + wr * 16 + (lane & 15), tile.col0 + wc * 16 * FC, lane >> 4);
+        // the loads' counts above are of loads alone
+        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    }
+}
+
+// float32: the three pieces of both operands (or of the rows' alone: PC = 1 piece of the columns', values that bfloat16 holds) in
+// one stage of 32 along the reduction, multiplied there in all their pairs: half the loads and LDS reads of going through the
+// pieces' products one after another. Tiles of 256 x 128, waves and phases as above: a phase has 24 MFMAs (12).
+//
+// A block of 64 output indexes x 32 x one piece is 4 KB, four loads. Three loads per wave are the columns of a stage (PC = 1: one),
+// three rows 0..127, three rows 128..255: issued in phase 1 of stage i for stage i + 2, in phase 3 for it, and in phase 0 of stage
+// i + 1 for stage i + 2. At the end of phase 3's memory half 6 + PC are younger than what the next stage starts with, at the end
+// of phase 1's 6 + 2 PC younger than its rows 128..255.
+template <bool TM, bool PERM> struct Block32 {
+    static __device__ __forceinline__ int swz(int n) {
+        if (TM) return (((n >> 1) & 1) | ((n >> 3) & 1) << 1) << 1;   // LDS rows of 64 indexes, two to a pass of 256 bytes
+        return (PERM ? n >> 3 : n >> 2) & 3;                          // LDS rows of 32 along t, four to a pass
+    }
+    // load `part` of a block: the lane's offset, and its first reduction index
+    static __device__ __forceinline__ uint32_t offset(const Operand &o, int part, int lane, int &at) {
+        const int row = TM ? part * 8 + lane / 8 : part * 16 + lane / 4;
+        const int chunk = TM ? (lane & 7) ^ swz(row) : (lane & 3) ^ swz(row);
+        at = TM ? 0 : chunk * 8;
+        return (uint32_t)(row * (int)o.ld + chunk * 8) * 2u;
+    }
+    static __device__ __forceinline__ bf16x8 frag(const char *block, int first, int lane) {
+        const int q = lane >> 4, r = lane & 15;
+        if constexpr (TM) {
+            union {
+                s16x4 h[2];
+                bf16x8 f;
+            } u;
 #pragma unroll
-            for (int r = 0; r < RUNS; ++r)
-                if (row < p.rows && col_of(r) < p.cols)
-                    ahead_r[r] = *reinterpret_cast<const Run *>((const T *)p.residual + (int64_t)row * p.cols + col_of(r));
-        };
-        if (p.bias)
-#pragma unroll
-            for (int r = 0; r < RUNS; ++r)
-                if (col_of(r) < p.cols) bias[r] = *reinterpret_cast<const Run *>((const T *)p.bias + col_of(r));
-        if (p.residual) residual(first);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int row = first + j * 32;
-            Run res[RUNS];
-#pragma unroll
-            for (int r = 0; r < RUNS; ++r) res[r] = ahead_r[r];
-            if (p.residual && j < 7) residual(row + 32);
-#pragma unroll
-            for (int r = 0; r < RUNS; ++r) {
-                const int col = col_of(r);
-                float v[RUN];
-#pragma unroll
-                for (int e = 0; e < RUN; ++e) v[e] = CT ? acc[r][j][e] : acc[r * 2 + e / 4][j][e % 4];
-                if (row >= p.rows || col >= p.cols) continue;
-                const int64_t at_o = (int64_t)row * p.cols + col;
-                if (p.sums) {
-                    float *o = (float *)p.out + (int64_t)tile.split * p.rows * p.cols + at_o;
-#pragma unroll
-                    for (int e = 0; e < RUN; e += 4) *reinterpret_cast<fvec4 *>(o + e) = fvec4{v[e], v[e + 1], v[e + 2], v[e + 3]};
-                    continue;
-                }
-                Run o;
-                if (p.bias)
-#pragma unroll
-                    for (int e = 0; e < RUN; ++e) v[e] += (float)bias[r].v[e];
-                if (p.pre) {
-#pragma unroll
-                    for (int e = 0; e < RUN; ++e) o.v[e] = (T)v[e];
-                    *reinterpret_cast<Run *>((T *)p.pre + at_o) = o;
-                }
-                act_values<is_f32<T>(), RUN>(v, p.act);
-                if (p.residual)
-#pragma unroll
-                    for (int e = 0; e < RUN; ++e) v[e] += (float)res[r].v[e];
-#pragma unroll
-                for (int e = 0; e < RUN; ++e) o.v[e] = (T)v[e];
-                *reinterpret_cast<Run *>((T *)p.out + at_o) = o;
+            for (int h = 0; h < 2; ++h) {
+                const int t = q * 8 + h * 4 + r / 4, c = first + (r & 3) * 4;
+                const char *p = block + t * 128 + (((c >> 3) ^ swz(t)) << 4) + (c & 7) * 2;
+                typedef __attribute__((address_space(3))) s16x4 *lds_t;
+                u.h[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)p);
             }
+            return u.f;
+        } else {
+            const int n = PERM ? (first & ~31) + (r >> 2) * 8 + (first & 16) / 4 + (r & 3) : first + r;
+            return *reinterpret_cast<const bf16x8 *>(block + n * 64 + ((q ^ swz(n)) << 4));
         }
+    }
+};
+
+template <bool RT, bool CT, int PC> __global__ void __launch_bounds__(512, 2) pieces_product_kernel(Product p) {
+    constexpr int BC = 128, COLS = 4 * 3 * 4096, STAGE = COLS + 2 * PC * 4096;
+    extern __shared__ __align__(1024) char smem[];
+    typedef Block32<RT, false> SR;
+    typedef Block32<CT, !CT> SC;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wr = wave >> 2, wc = wave & 3;
+    const WideTiles tiles(p);
+    if (tiles.count == 0) return;
+    typedef __attribute__((address_space(3))) char *lds_t;
+    const uint32_t lds = (uint32_t)(uintptr_t)(lds_t)smem;
+
+    // load l of the wave: part (3 wave + l) % 4 of block (3 wave + l) / 4 of two rows' quarters (block: 3 quarter + piece), and the
+    // same of the columns' halves
+    uint32_t off_r[3], off_c[PC];
+    int at_r[3], at_c[PC];
+#pragma unroll
+    for (int l = 0; l < 3; ++l) off_r[l] = SR::offset(p.R, (wave * 3 + l) & 3, lane, at_r[l]);
+#pragma unroll
+    for (int l = 0; l < PC; ++l) off_c[l] = SC::offset(p.C, (wave * PC + l) & 3, lane, at_c[l]);
+
+    int tile_n = 0, step = 0, buf = 0;
+    WideTile<BC, 32> ahead(p, tiles.first);
+    WideSource<RT, 256, 32> rows;
+    WideSource<CT, BC, 32> cols;
+    auto enter = [&]() {
+        const int64_t k0 = ahead.kbeg + (int64_t)step * 32;
+        rows.enter(p.R, 0, ahead.row0, k0, 0, 0);
+        cols.enter(p.C, 0, ahead.col0, k0, 0, 0);
+        if (tile_n >= tiles.count) rows.inside = cols.inside = 0;   // past the last tile: loads that fetch nothing
+    };
+    auto next = [&]() {
+        buf ^= 1;
+        if (++step < ahead.nk) {
+            rows.advance(0, 0);
+            cols.advance(0, 0);
+            return;
+        }
+        step = 0;
+        if (++tile_n < tiles.count) ahead = WideTile<BC, 32>(p, tiles.first + tile_n * tiles.step);
+        enter();
+    };
+    u32x4 d[3];
+    uint32_t off[3], to = 0;
+    const uint64_t plane_r = 2 * (uint64_t)p.R.plane, plane_c = 2 * (uint64_t)p.C.plane;
+    auto aim_rows = [&](int q) {
+#pragma unroll
+        for (int l = 0; l < 3; ++l) {
+            const int block = (wave * 3 + l) >> 2;
+            d[l] = rows.descriptor(q + block / 3, block % 3 * plane_r);
+            off[l] = RT || at_r[l] < rows.left() ? off_r[l] : 0x80000000u;
+        }
+        to = lds + buf * STAGE + q * 12288 + wave * 3072;
+    };
+    auto aim_cols = [&]() {
+#pragma unroll
+        for (int l = 0; l < PC; ++l) {
+            const int block = (wave * PC + l) >> 2;
+            d[l] = cols.descriptor(block / PC, block % PC * plane_c);
+            off[l] = CT || at_c[l] < cols.left() ? off_c[l] : 0x80000000u;
+        }
+        to = lds + buf * STAGE + COLS + wave * PC * 1024;
+    };
+    auto load = [&](auto count) {
+#pragma unroll
+        for (int l = 0; l < decltype(count)::value; ++l) load_to_lds(d[l], off[l], to + l * 1024);
+    };
+    typedef std::integral_constant<int, 3> Rows;
+    typedef std::integral_constant<int, PC> Cols;
+
+    enter();
+    aim_cols(), load(Cols());
+    aim_rows(0), load(Rows());
+    aim_rows(2), load(Rows());
+    next();
+    aim_cols(), load(Cols());
+    aim_rows(0), load(Rows());
+    aim_rows(2);
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(6 + PC) : "memory");
+
+    int at = 0;
+    for (int n = 0; n < tiles.count; ++n) {
+        const WideTile<BC, 32> tile(p, tiles.first + n * tiles.step);
+        fvec4 acc[2][8];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc[i][j] = fvec4{0.f, 0.f, 0.f, 0.f};
+        if (wr) asm volatile("s_barrier" ::: "memory");   // one half behind
+        for (int it = 0; it < tile.nk; ++it) {
+            const char *tr = smem + at * STAGE, *tc = tr + COLS + wc / 2 * PC * 4096;
+            at ^= 1;
+            bf16x8 a[PC][2];
+            auto phase = [&](auto number) {
+                constexpr int ph = decltype(number)::value;
+                bf16x8 b[3][2];
+                if constexpr (ph == 0)
+#pragma unroll
+                    for (int k = 0; k < PC; ++k)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) a[k][i] = SC::frag(tc + k * 4096, wc % 2 * 32 + i * 16, lane);
+#pragma unroll
+                for (int k = 0; k < 3; ++k)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) b[k][j] = SR::frag(tr + (ph * 3 + k) * 4096, j * 32 + wr * 16, lane);
+                if constexpr (ph == 0 || ph == 3) load(Rows());
+                if constexpr (ph == 1) load(Cols());
+                if constexpr (ph == 1)
+                    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(6 + 2 * PC) : "memory");
+                else if constexpr (ph == 3)
+                    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(6 + PC) : "memory");
+                else
+                    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                __builtin_amdgcn_s_setprio(1);
+                if constexpr (ph == 0) next();
+                // the smallest products first: pieces of the rows x of the columns
+#pragma unroll
+                for (int sum = 2; sum >= 0; --sum)
+#pragma unroll
+                    for (int k = sum; k >= 0; --k)
+                        if (sum - k < PC)
+#pragma unroll
+                            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                                for (int j = 0; j < 2; ++j)
+                                    acc[i][ph * 2 + j] = mfma(a[(sum - k) % PC][i], b[k][j], acc[i][ph * 2 + j]);
+                if constexpr (ph == 0) aim_cols();
+                if constexpr (ph == 2) aim_rows(0);
+                if constexpr (ph == 3) aim_rows(2);
+#pragma unroll
+                for (int m = 0; m < (PC == 3 ? 24 : 12); ++m) {   // scalar work between the MFMAs
+                    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x4, 3, 0);
+                }
+                __builtin_amdgcn_s_setprio(0);
+                asm volatile("s_barrier" ::: "memory");
+            };
+            phase(std::integral_constant<int, 0>());
+            phase(std::integral_constant<int, 1>());
+            phase(std::integral_constant<int, 2>());
+            phase(std::integral_constant<int, 3>());
+        }
+        if (!wr) asm volatile("s_barrier" ::: "memory");   // level again
+        store_results<float, CT, 2>(p, acc, tile.split, tile.row0 + wr * 16 + (lane & 15), tile.col0 + wc * 32, lane >> 4);
         // the loads' counts above are of loads alone
         asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
     }
@@ -804,31 +1003,55 @@ template <typename E, typename T, bool RT, bool CT, int FC> hipError_t launch_wi
     return hipGetLastError();
 }
 
+template <bool RT, bool CT, int PC> hipError_t launch_pieces(Product &p, hipStream_t s) {
+    static std::atomic<unsigned long long> done{0};
+    const auto kernel = pieces_product_kernel<RT, CT, PC>;
+    if (hipError_t e = raise_lds_limit((const void *)kernel, done)) return e;
+    p.tiles_r = (int)ceil_div(p.rows, 256);
+    p.tiles_c = (int)ceil_div(p.cols, 128);
+    const int64_t tiles = (int64_t)p.tiles_r * p.tiles_c * p.splits;
+    kernel<<<(unsigned)(tiles < 256 ? tiles : 256), 512, 2 * (12 + 2 * PC) * 4096, s>>>(p);
+    return hipGetLastError();
+}
+
 // Which tiles an output takes: 256 x 256 or 256 x 128 (of whole eights of columns), one workgroup per CU; 128 x 128 or 64 x 64,
 // two per CU. The least of what they take, in microseconds: launch, first loads and results, and so much per step of 64 along
 // the reduction and round of workgroups. Measured in bfloat16, 16 steps: 2048 x 1024 takes 33.6 / 23.7 / 21.1 / 15.6 us in the
 // four; 24 steps, 32768 x 256: 47.8 / 35.0 / 43.3 / 79.7; 32 steps, 65536 x 512: 130 / 166 / 253 / -.
-enum Tiles { WIDE, HALF, BIG, SMALL };
+// float32 (all its pieces' products): 32768 x 256 from 256 takes 33.7 us by the pieces' own kernel, 41.3 / 43.9 / 68.4 in 256 x
+// 128, 128 x 128 and 64 x 64; 8192 x 256 26.5, 35.4 / 29.0 / 21.8.
+enum Tiles { PIECES, WIDE, HALF, BIG, SMALL };
 double tiles_cost(Tiles t, int64_t rows, int64_t cols, int64_t splits, double steps) {
     auto count = [&](int64_t r, int64_t c) { return ceil_div(rows, r) * ceil_div(cols, c) * splits; };
     switch (t) {
+        case PIECES: return 10 + 0.87 * steps * (double)ceil_div(count(256, 128), 256);
         case WIDE: return 10 + 1.75 * steps * (double)ceil_div(count(256, 256), 256);
         case HALF: return 7 + 1.2 * steps * (double)ceil_div(count(256, 128), 256);
         case BIG: return 6 + steps * (count(128, 128) <= 256 ? 0.95 : 1.7 * (double)ceil_div(count(128, 128), 512));
         default: return 4 + steps * (count(64, 64) <= 256 ? 0.55 : 0.75 * (double)ceil_div(count(64, 64), 512));
     }
 }
-Tiles choose_tiles(int64_t rows, int64_t cols, double steps) {
+bool tiles_fit(Tiles t, bool wide, int64_t cols) {   // wide: float32
+    return t >= BIG || (cols % 8 == 0 && (t == PIECES) == wide);
+}
+Tiles choose_tiles(bool wide, int64_t rows, int64_t cols, double steps) {
     Tiles best = SMALL;
-    for (Tiles t : {BIG, HALF, WIDE})
-        if ((t == BIG || cols % 8 == 0) && tiles_cost(t, rows, cols, 1, steps) < tiles_cost(best, rows, cols, 1, steps)) best = t;
+    for (Tiles t : {BIG, HALF, WIDE, PIECES})
+        if (tiles_fit(t, wide, cols) && tiles_cost(t, rows, cols, 1, steps) < tiles_cost(best, rows, cols, 1, steps)) best = t;
     return best;
 }
 
 template <typename E, typename T, bool RT, bool CT> hipError_t launch_product(Product p, Tiles tiles, hipStream_t s) {
+    if constexpr (is_f32<T>()) {
+        if (tiles == PIECES) {
+            if (p.npair == 6) return launch_pieces<RT, CT, 3>(p, s);
+            if constexpr (RT) return launch_pieces<RT, CT, 1>(p, s);   // the weight gradient of a kept input
+        }
+    } else {
+        if (tiles == WIDE) return launch_wide<E, T, RT, CT, 4>(p, s);
+        if (tiles == HALF) return launch_wide<E, T, RT, CT, 2>(p, s);
+    }
     switch (tiles) {
-        case WIDE: return launch_wide<E, T, RT, CT, 4>(p, s);
-        case HALF: return launch_wide<E, T, RT, CT, 2>(p, s);
         case BIG: return launch_tiles<E, T, RT, CT, 2, 2, 4, 4, 64, 2, 2>(p, s);
         default: return launch_tiles<E, T, RT, CT, 2, 2, 2, 2, 64, 3, 2>(p, s);
     }
@@ -849,7 +1072,7 @@ template <typename E, typename T, bool CT> hipError_t launch_rows(Product p, int
         p.out = out + first * p.cols;
         p.pre = pre ? pre + first * p.cols : nullptr;
         p.residual = res ? res + first * p.cols : nullptr;
-        if (hipError_t e = launch_product<E, T, false, CT>(p, choose_tiles(p.rows, p.cols, steps), s)) return e;
+        if (hipError_t e = launch_product<E, T, false, CT>(p, choose_tiles(is_f32<T>(), p.rows, p.cols, steps), s)) return e;
     }
     return hipSuccess;
 }
@@ -916,8 +1139,9 @@ Plan make_plan(const PointwiseArgs &a) {
     double least = 0;
     int64_t splits = 0;
     for (const auto &[t, r, c, slots] : {std::tuple<Tiles, int, int, int>{SMALL, 64, 64, 512}, {BIG, 128, 128, 256},
-                                         {BIG, 128, 128, 512}, {HALF, 256, 128, 256}, {WIDE, 256, 256, 256}}) {
-        if (t <= HALF && a.in % 8 != 0) continue;
+                                         {BIG, 128, 128, 512}, {HALF, 256, 128, 256}, {WIDE, 256, 256, 256},
+                                         {PIECES, 256, 128, 256}}) {
+        if (!tiles_fit(t, wide, a.in)) continue;
         const int64_t n = std::min(std::max<int64_t>(1, slots / (ceil_div(a.out, r) * ceil_div(a.in, c))), most_splits);
         const double steps = (double)ceil_div(ceil_div(a.rows, n), SHARE) * k.np * (k.npx == 3 ? 2 : 1);
         const double cost = tiles_cost(t, a.out, a.in, n, steps) + (n > 1 ? (double)(n * a.out) * a.in * 2e-6 : 0.0);
