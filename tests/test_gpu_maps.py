@@ -112,7 +112,8 @@ def test_pointwise(shape, out, dtype):
 # outputs that fill the chip with the largest tiles, their last ones in part: rows, columns and reduction of all remainders
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,channels,out", [(20011, 72, 520), (33000, 264, 256), (9000, 1032, 2056), (70001, 8, 264),
-                                               (16384, 200, 1024), (40000, 520, 24)])
+                                               (16384, 200, 1024), (40000, 520, 24), (30001, 513, 264),
+                                               (30001, 264, 515)])
 def test_pointwise_of_many_pixels(rows, channels, out, dtype):
     x = make((rows, channels), dtype, 1)
     w = make((out, channels), dtype, 2, spread=channels ** -0.5)
@@ -135,11 +136,15 @@ def test_pointwise_kept_in_8_bits(shape, out, dtype):
 
 
 def test_pointwise_float32_is_float32_accurate():
-    """The pieces and their six products: independent roundings leave about sqrt(6 K / 32) last bits, 6e-7 at K = 600."""
-    x, w = make((1, 600, 400), torch.float32, 1), make((192, 600), torch.float32, 2)
-    dy = make((1, 192, 400), torch.float32, 3)
-    for g, (r, _) in zip(run_pointwise(x, w, None, None, "none", dy), pointwise(x, w, None, None, "none", dy)):
-        assert (g.double() - r).norm() / r.norm() < 2e-6
+    """On the float32 MFMAs and in pieces: independent roundings leave about sqrt(K / 4) last bits, or sqrt(6 K / 32), 7e-7 at
+    K = 600, and as many of the 128 rows and 100 shares that the weight's gradient adds up."""
+    for n in (400, 60000):   # as it lies, and in pieces
+        x, w = make((1, 600, n), torch.float32, 1), make((192, 600), torch.float32, 2)
+        dy = make((1, 192, n), torch.float32, 3)
+        for keep in (False, True):
+            want = pointwise(x, w, None, None, "none", dy, keep)
+            for g, (r, _) in zip(run_pointwise(x, w, None, None, "none", dy, keep), want):
+                assert (g.double() - r).norm() / r.norm() < 2e-6
     big = torch.tensor([[3.4e38, 1e-3, 1.0, 0, 0, 0, 0, 0]], device="cuda")
     assert torch.equal(tvdcn.pointwise_conv(big, torch.eye(8, device="cuda")), big)
 

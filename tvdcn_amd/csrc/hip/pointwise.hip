@@ -13,9 +13,10 @@
 // fixed by the lane) so that the lanes of a read fall into different banks. Values beyond an operand's edge are read as
 // zeros by the buffer's own bounds check.
 //
-// float32 maps run as three bfloat16 pieces per value (exact) and the six products of pieces that reach
-// float32's precision, smallest first: 2^-24 relative to the operands' products, at a sixth of the 16-bit rate (2.6 times
-// the rate of the float32 MFMAs). An infinite operand may turn into a NaN where float32 would keep an infinity.
+// float32 maps are multiplied on the float32 MFMAs as they lie, or, where the products are large, as three bfloat16 pieces per
+// value (exact) by the six products of pieces that reach float32's precision: 2^-24 relative to the operands' products, at a sixth
+// of the 16-bit rate (2.6 times the rate of the float32 MFMAs). An infinite operand may turn into a NaN there where float32 would
+// keep an infinity.
 #include <algorithm>
 #include <atomic>
 #include <tuple>
@@ -55,8 +56,7 @@ struct Operand {
 
 struct Product {
     Operand R, C;
-    int npair;
-    int8_t pr[6], pc[6];      // pieces of each product
+    int pieces_c;             // float32 in pieces: of a value of C (of R: 3)
     int rows, cols;           // of the output
     int64_t share;            // reduction per workgroup (a multiple of SHARE, or all of it)
     int tiles_r, tiles_c, splits;
@@ -112,11 +112,11 @@ template <bool TM, bool PERM, int B, int F, int BK, int NW> struct Stager {
             }
         }
     }
-    __device__ __forceinline__ void load(const Operand &o, int piece, int64_t first, int64_t k0, int64_t kend, uint32_t lds,
+    __device__ __forceinline__ void load(const Operand &o, int64_t first, int64_t k0, int64_t kend, uint32_t lds,
                                          int wave) const {
         const int64_t lim = kend < o.lim ? kend : o.lim;
         const int left = (int)(lim - k0 < BK ? lim - k0 : BK);
-        const uint64_t base = (uint64_t)o.p + 2 * (uint64_t)(o.plane * piece + (TM ? k0 * o.ld + first : first * o.ld + k0));
+        const uint64_t base = (uint64_t)o.p + 2 * (uint64_t)(TM ? k0 * o.ld + first : first * o.ld + k0);
         const u32x4 rsrc = {(uint32_t)base, (uint32_t)(base >> 32) & 0xffffu, 0x7fffffffu, 0x00020000u};
 #pragma unroll
         for (int i = 0; i < LOADS; ++i)
@@ -192,21 +192,31 @@ __device__ __forceinline__ void emit(const Product &p, int split, int row, int c
         for (int v = 0; v < RUN; ++v) o.v[v] = (T)(act_value<is_f32<T>()>(z[v], p.act) + r[v]);
         *reinterpret_cast<P *>((T *)p.out + at) = o;
     } else {
+        // (loads that stay in the row, all on their way at once)
+        const int last = p.cols - 1 - col;
 #pragma unroll
-        for (int v = 0; v < RUN; ++v) {
-            if (col + v >= p.cols) break;
-            float zv = acc[v];
-            if (p.bias) zv += (float)((const T *)p.bias)[col + v];
-            if (p.pre) ((T *)p.pre)[at + v] = (T)zv;
-            float o = act_value<is_f32<T>()>(zv, p.act);
-            if (p.residual) o += (float)((const T *)p.residual)[at + v];
-            ((T *)p.out)[at + v] = (T)o;
-        }
+        for (int v = 0; v < RUN; ++v) z[v] = r[v] = 0.f;
+        if (p.bias)
+#pragma unroll
+            for (int v = 0; v < RUN; ++v) z[v] = (float)((const T *)p.bias)[col + (v < last ? v : last)];
+        if (p.residual)
+#pragma unroll
+            for (int v = 0; v < RUN; ++v) r[v] = (float)((const T *)p.residual)[at + (v < last ? v : last)];
+#pragma unroll
+        for (int v = 0; v < RUN; ++v) z[v] += acc[v];
+        if (p.pre)
+#pragma unroll
+            for (int v = 0; v < RUN; ++v)
+                if (v <= last) ((T *)p.pre)[at + v] = (T)z[v];
+        act_values<is_f32<T>(), RUN>(z, p.act);
+#pragma unroll
+        for (int v = 0; v < RUN; ++v)
+            if (v <= last) ((T *)p.out)[at + v] = (T)(z[v] + r[v]);
     }
 }
 
 // WR x WC waves, each FR x FC fragments of 16 x 16; STAGES tiles of BK along the reduction in LDS
-template <typename E, typename T, bool RT, bool CT, int WR, int WC, int FR, int FC, int BK, int STAGES, int BLOCKS>
+template <typename T, bool RT, bool CT, int WR, int WC, int FR, int FC, int BK, int STAGES, int BLOCKS>
 __global__ void __launch_bounds__(WR * WC * 64, BLOCKS * WR * WC / 4) product_kernel(Product p) {
     constexpr int NW = WR * WC, BR = WR * 16 * FR, BC = WC * 16 * FC, TILE = (BR + BC) * BK * 2;
     extern __shared__ __align__(1024) char smem[];
@@ -220,7 +230,7 @@ __global__ void __launch_bounds__(WR * WC * 64, BLOCKS * WR * WC / 4) product_ke
     const int row0 = in_split / p.tiles_c * BR, col0 = in_split % p.tiles_c * BC;
     const int64_t kall = p.R.lim > p.C.lim ? p.R.lim : p.C.lim;
     const int64_t kbeg = split * p.share, kend = kbeg + p.share < kall ? kbeg + p.share : kall;
-    const int nk = (int)((kend - kbeg + BK - 1) / BK), iters = nk * p.npair;
+    const int iters = (int)((kend - kbeg + BK - 1) / BK);
 
     typedef Stager<RT, false, BR, FR, BK, NW> SR;
     typedef Stager<CT, !CT, BC, FC, BK, NW> SC;
@@ -239,12 +249,12 @@ __global__ void __launch_bounds__(WR * WC * 64, BLOCKS * WR * WC / 4) product_ke
 #pragma unroll
         for (int j = 0; j < FR; ++j) acc[i][j] = fvec4{0.f, 0.f, 0.f, 0.f};
 
-    int pair = 0, step = 0, to = 0, at = 0;   // the next tile to stage and its buffer; the buffer to read
+    int step = 0, to = 0, at = 0;   // the next tile to stage and its buffer; the buffer to read
     auto stage = [&]() {
         const int64_t k0 = kbeg + (int64_t)step * BK;
-        sr.load(p.R, p.pr[pair], row0, k0, kend, lds + to * TILE, wave);
-        sc.load(p.C, p.pc[pair], col0, k0, kend, lds + to * TILE + BR * BK * 2, wave);
-        if (++step == nk) step = 0, ++pair;
+        sr.load(p.R, row0, k0, kend, lds + to * TILE, wave);
+        sc.load(p.C, col0, k0, kend, lds + to * TILE + BR * BK * 2, wave);
+        ++step;
         if (++to == STAGES) to = 0;
     };
     for (int it = 0; it < STAGES - 1 && it < iters; ++it) stage();
@@ -260,11 +270,11 @@ __global__ void __launch_bounds__(WR * WC * 64, BLOCKS * WR * WC / 4) product_ke
         if (++at == STAGES) at = 0;
 #pragma unroll
         for (int kk = 0; kk < BK / 32; ++kk) {
-            typename Frag<E>::type a[FC], b[FR];
+            typename Frag<T>::type a[FC], b[FR];
 #pragma unroll
-            for (int i = 0; i < FC; ++i) a[i] = SC::template frag<E>(tc, wc * 16 * FC, i, kk, lane);
+            for (int i = 0; i < FC; ++i) a[i] = SC::template frag<T>(tc, wc * 16 * FC, i, kk, lane);
 #pragma unroll
-            for (int j = 0; j < FR; ++j) b[j] = SR::template frag<E>(tr, wr * 16 * FR, j, kk, lane);
+            for (int j = 0; j < FR; ++j) b[j] = SR::template frag<T>(tr, wr * 16 * FR, j, kk, lane);
 #pragma unroll
             for (int i = 0; i < FC; ++i)
 #pragma unroll
@@ -464,8 +474,8 @@ template <bool TM, int B, int STEP = 64> struct WideSource {
         if (TM) rows = (uint32_t)(left() - 1) * pitch, off = lane_off;
         else off = lane_at < left() ? lane_off : 0x80000000u;
     }
-    __device__ __forceinline__ void enter(const Operand &o, int piece, int first, int64_t k0, uint32_t lane_off, int lane_at) {
-        base = (uint64_t)o.p + 2 * (uint64_t)(o.plane * piece + (TM ? k0 * o.ld + first : first * o.ld + k0));
+    __device__ __forceinline__ void enter(const Operand &o, int first, int64_t k0, uint32_t lane_off, int lane_at) {
+        base = (uint64_t)o.p + 2 * (uint64_t)(TM ? k0 * o.ld + first : first * o.ld + k0);
         inside = __builtin_amdgcn_readfirstlane((int)(o.width - first < B ? o.width - first : B));
         pitch = 2u * (uint32_t)o.ld;
         step = TM ? 128 : 64 * (uint64_t)pitch;
@@ -489,7 +499,7 @@ template <bool TM, int B, int STEP = 64> struct WideSource {
     }
 };
 
-template <typename E, typename T, bool RT, bool CT, int FC>
+template <typename T, bool RT, bool CT, int FC>
 __global__ void __launch_bounds__(512, 2) wide_product_kernel(Product p) {
     constexpr int BC = 64 * FC, COLS = 32768, STAGE = COLS + BC * 128;   // bytes; the columns' sub-tiles follow the rows'
     extern __shared__ __align__(1024) char smem[];
@@ -506,14 +516,14 @@ __global__ void __launch_bounds__(512, 2) wide_product_kernel(Product p) {
     const uint32_t off_r = SR::offset(p.R, wave, lane, at_r), off_c = SC::offset(p.C, wave, lane, at_c);
 
     // the stage to load next
-    int tile_n = 0, pair = 0, step = 0, buf = 0;
+    int tile_n = 0, step = 0, buf = 0;
     WideTile<BC> ahead(p, tiles.first);
     WideSource<RT, 256> rows;
     WideSource<CT, BC> cols;
     auto enter = [&]() {
         const int64_t k0 = ahead.kbeg + (int64_t)step * 64;
-        rows.enter(p.R, p.pr[pair], ahead.row0, k0, off_r, at_r);
-        cols.enter(p.C, p.pc[pair], ahead.col0, k0, off_c, at_c);
+        rows.enter(p.R, ahead.row0, k0, off_r, at_r);
+        cols.enter(p.C, ahead.col0, k0, off_c, at_c);
         if (tile_n >= tiles.count) rows.inside = cols.inside = 0;   // past the last tile: loads that fetch nothing
     };
     auto next = [&]() {
@@ -524,10 +534,7 @@ __global__ void __launch_bounds__(512, 2) wide_product_kernel(Product p) {
             return;
         }
         step = 0;
-        if (++pair == p.npair) {
-            pair = 0;
-            if (++tile_n < tiles.count) ahead = WideTile<BC>(p, tiles.first + tile_n * tiles.step);
-        }
+        if (++tile_n < tiles.count) ahead = WideTile<BC>(p, tiles.first + tile_n * tiles.step);
         enter();
     };
     // two sub-tiles' loads, their descriptors made ahead (beside the MFMAs)
@@ -552,28 +559,27 @@ __global__ void __launch_bounds__(512, 2) wide_product_kernel(Product p) {
     int at = 0;
     for (int n = 0; n < tiles.count; ++n) {
         const WideTile<BC> tile(p, tiles.first + n * tiles.step);
-        const int iters = tile.nk * p.npair;
         fvec4 acc[FC][8];
 #pragma unroll
         for (int i = 0; i < FC; ++i)
 #pragma unroll
             for (int j = 0; j < 8; ++j) acc[i][j] = fvec4{0.f, 0.f, 0.f, 0.f};
         if (wr) asm volatile("s_barrier" ::: "memory");   // one half behind
-        for (int it = 0; it < iters; ++it) {
+        for (int it = 0; it < tile.nk; ++it) {
             const char *tr = smem + at * STAGE, *tc = tr + COLS + wc * FC / 4 * 8192;
             at ^= 1;
-            typename Frag<E>::type a[2][FC];
+            typename Frag<T>::type a[2][FC];
             auto phase = [&](auto number) {
                 constexpr int ph = decltype(number)::value;
-                typename Frag<E>::type b[2][2];
+                typename Frag<T>::type b[2][2];
 #pragma unroll
                 for (int kk = 0; kk < 2; ++kk) {
                     if constexpr (ph == 0) {
 #pragma unroll
-                        for (int i = 0; i < FC; ++i) a[kk][i] = SC::template frag<E>(tc, wc * FC % 4 * 16 + i * 16, kk, lane);
+                        for (int i = 0; i < FC; ++i) a[kk][i] = SC::template frag<T>(tc, wc * FC % 4 * 16 + i * 16, kk, lane);
                     }
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) b[kk][j] = SR::template frag<E>(tr + ph * 8192, j * 32 + wr * 16, kk, lane);
+                    for (int j = 0; j < 2; ++j) b[kk][j] = SR::template frag<T>(tr + ph * 8192, j * 32 + wr * 16, kk, lane);
                 }
                 if constexpr (FC == 4 || ph != 2) load();
                 if constexpr (ph == 1)
@@ -683,8 +689,8 @@ template <bool RT, bool CT, int PC> __global__ void __launch_bounds__(512, 2) pi
     WideSource<CT, BC, 32> cols;
     auto enter = [&]() {
         const int64_t k0 = ahead.kbeg + (int64_t)step * 32;
-        rows.enter(p.R, 0, ahead.row0, k0, 0, 0);
-        cols.enter(p.C, 0, ahead.col0, k0, 0, 0);
+        rows.enter(p.R, ahead.row0, k0, 0, 0);
+        cols.enter(p.C, ahead.col0, k0, 0, 0);
         if (tile_n >= tiles.count) rows.inside = cols.inside = 0;   // past the last tile: loads that fetch nothing
     };
     auto next = [&]() {
@@ -805,6 +811,137 @@ template <bool RT, bool CT, int PC> __global__ void __launch_bounds__(512, 2) pi
     }
 }
 
+// float32 as it lies, on the float32 MFMAs (16x16x4): no pieces, no copies of the operands, any pitch. Waves 2 x 2 of 2 x 2 fragments,
+// tiles of 64 x 64 (128 x 128 ones are 2% faster to 8% slower); a step is 16 along the reduction, staged through registers (16-byte loads where the rows allow them), double-
+// buffered in LDS. A lane's four values along the reduction serve four MFMAs: quarter q of a wave holds t = 4 q + m in MFMA m, of
+// both operands. t-contiguous tiles lie in rows of 16 (a wave reads 1 KB in a row), t-major ones in rows of B + 4, so that the four
+// quarters' rows, four apart, fall into different banks. Bound by the MFMAs (157 TFLOP/s)
+// and the steps' barriers: 87 TFLOP/s at 32768 x 256 from 256, 105 at 4096 x 2048 from 2048.
+template <bool TM, int B> struct FloatStage {
+    static constexpr int N = B / 64, LD = TM ? B + 4 : 16, BYTES = (TM ? 16 : B) * LD * 4;   // accesses of 16 bytes per thread
+    fvec4 v[N];
+    const float *p[N];   // where the next step's lie
+    int64_t pace;
+    int at[N], more;     // the access's first t of a step; t-major, its columns up to the edge
+    // (outputs beyond the edge are not stored: what they are made of is any value that may be read)
+    __device__ __forceinline__ void init(const Operand &o, int64_t first, int64_t k0, int t) {
+        more = (int)(o.width - first < B ? o.width - first : B);
+        pace = TM ? 16 * o.ld : 16;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int id = t + i * 256, n = TM ? id % (B / 4) * 4 : id / 4;
+            at[i] = TM ? id / (B / 4) : id % 4 * 4;
+            p[i] = (const float *)o.p + (TM ? (k0 + at[i]) * o.ld + first + (n < more ? n : 0) : (first + (n < more ? n : 0)) * o.ld + k0 + at[i]);
+            if (TM) at[i] |= (n < more ? n : 0) << 8;
+        }
+    }
+    // a step of which `left` along t remain
+    __device__ __forceinline__ void load(bool vec, int left) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int k = TM ? at[i] & 255 : at[i];
+            if (TM) {
+                const int cols = more - (at[i] >> 8);   // (at least one)
+                if (k >= left) {
+                    v[i] = fvec4{0.f, 0.f, 0.f, 0.f};
+                } else if (vec) {
+                    v[i] = *reinterpret_cast<const fvec4 *>(p[i]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[i][e] = p[i][e < cols ? e : 0];
+                }
+            } else if (vec && left >= 16) {
+                v[i] = *reinterpret_cast<const fvec4 *>(p[i]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[i][e] = p[i][k + e < left ? e : -k];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (k + e >= left) v[i][e] = 0.f;
+            }
+            p[i] += pace;
+        }
+    }
+    __device__ __forceinline__ void store(float *tile, int t) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int id = t + i * 256;
+            *reinterpret_cast<fvec4 *>(TM ? tile + id / (B / 4) * LD + id % (B / 4) * 4 : tile + id * 4) = v[i];
+        }
+    }
+    static __device__ __forceinline__ fvec4 frag(const float *tile, int first, int lane) {
+        const int q = lane >> 4, n = first + (lane & 15);
+        if constexpr (TM) {
+            fvec4 f;
+#pragma unroll
+            for (int m = 0; m < 4; ++m) f[m] = tile[(q * 4 + m) * LD + n];
+            return f;
+        } else {
+            return *reinterpret_cast<const fvec4 *>(tile + n * LD + q * 4);
+        }
+    }
+};
+
+template <bool RT, bool CT> __global__ void __launch_bounds__(256) float_product_kernel(Product p, bool vec_r, bool vec_c) {
+    constexpr int F = 2, B = 32 * F;
+    typedef FloatStage<RT, B> SR;
+    typedef FloatStage<CT, B> SC;
+    __shared__ __align__(16) char smem[2 * (SR::BYTES + SC::BYTES)];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, wr = wave >> 1, wc = wave & 1;
+    const int total = p.tiles_r * p.tiles_c * p.splits, id = blockIdx.x;
+    const int per = total / 8, extra = total % 8, xcd = id % 8;
+    const int tile = xcd * per + min(xcd, extra) + id / 8;
+    const int split = tile / (p.tiles_r * p.tiles_c), in_split = tile - split * (p.tiles_r * p.tiles_c);
+    const int row0 = in_split / p.tiles_c * B, col0 = in_split % p.tiles_c * B;
+    const int64_t kbeg = split * p.share, kend = kbeg + p.share < p.R.lim ? kbeg + p.share : p.R.lim;
+    fvec4 acc[F][F];
+#pragma unroll
+    for (int i = 0; i < F; ++i)
+#pragma unroll
+        for (int j = 0; j < F; ++j) acc[i][j] = fvec4{0.f, 0.f, 0.f, 0.f};
+    SR sr;
+    SC sc;
+    sr.init(p.R, row0, kbeg, t);
+    sc.init(p.C, col0, kbeg, t);
+    auto left = [&](int64_t k0) { return (int)(kend - k0 < 16 ? kend - k0 : 16); };
+    sr.load(vec_r, left(kbeg));
+    sc.load(vec_c, left(kbeg));
+    int buf = 0;
+    for (int64_t k0 = kbeg; k0 < kend; k0 += 16, buf ^= 1) {
+        float *tr = (float *)(smem + buf * (SR::BYTES + SC::BYTES)), *tc = (float *)((char *)tr + SR::BYTES);
+        sr.store(tr, t);
+        sc.store(tc, t);
+        __syncthreads();   // (a wave that stores into the other buffer has passed this: every read of that one is over)
+        if (k0 + 16 < kend) {
+            sr.load(vec_r, left(k0 + 16));
+            sc.load(vec_c, left(k0 + 16));
+        }
+        fvec4 a[F], b[F];
+#pragma unroll
+        for (int i = 0; i < F; ++i) a[i] = SC::frag(tc, wc * 16 * F + i * 16, lane);
+#pragma unroll
+        for (int j = 0; j < F; ++j) b[j] = SR::frag(tr, wr * 16 * F + j * 16, lane);
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int i = 0; i < F; ++i)
+#pragma unroll
+                for (int j = 0; j < F; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i][m], b[j][m], acc[i][j], 0, 0, 0);
+    }
+#pragma unroll
+    for (int j = 0; j < F; ++j) {
+        const int row = row0 + wr * 16 * F + j * 16 + (lane & 15);
+        if (row >= p.rows) continue;
+#pragma unroll
+        for (int i = 0; i < F; ++i) {
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e];
+            emit<float, 4>(p, split, row, col0 + wc * 16 * F + i * 16 + (lane >> 4) * 4, v);
+        }
+    }
+}
+
 // ---- operands laid out for the product: rows of a multiple of 8 elements, zeros behind the channels ----
 
 // float32 as three bfloat16 pieces, each the rest rounded to the nearest: hi + mid + lo = x exactly (hi leaves at most 16
@@ -833,45 +970,57 @@ template <typename E, int NP> __device__ __forceinline__ void split_pack(float x
 }
 
 // eight elements of a row, zeros behind its end
-template <typename T> __device__ __forceinline__ void load8(const T *row, int c, int C, bool vec, float *f) {
-    if (vec) {
+template <typename T, bool VEC> __device__ __forceinline__ void load8(const T *row, int c, int C, float *f) {
+    if constexpr (VEC) {   // (rows in whole eights)
         const Pack<T, 8> p = *reinterpret_cast<const Pack<T, 8> *>(row + c);
 #pragma unroll
         for (int v = 0; v < 8; ++v) f[v] = (float)p.v[v];
     } else {
 #pragma unroll
-        for (int v = 0; v < 8; ++v) f[v] = c + v < C ? (float)row[c + v] : 0.f;
+        for (int v = 0; v < 8; ++v) f[v] = (float)row[c + v < C ? c + v : 0];
+#pragma unroll
+        for (int v = 0; v < 8; ++v)
+            if (c + v >= C) f[v] = 0.f;
     }
 }
 
+// A row-major matrix and its copy with rows of lanes_row eights, in NP pieces, a plane apart
+struct LayOut {
+    const void *from;
+    void *to;
+    int64_t rows;
+    int C, lanes_row;
+    int64_t lanes() const { return rows * lanes_row; }
+};
+
+// both operands of a product (the second may have no rows) in one launch
 template <typename T, typename E, int NP>
-__global__ void __launch_bounds__(TB) lay_out_kernel(const T *__restrict__ x, E *__restrict__ y, int64_t rows, int C,
-                                                     int lanes_row, int64_t plane) {
-    const bool vec = C % 8 == 0;
-    const int64_t lanes = rows * lanes_row;
-    for (int64_t i = (int64_t)blockIdx.x * TB + threadIdx.x; i < lanes; i += (int64_t)gridDim.x * TB) {
-        const int64_t row = i / lanes_row;
-        const int c = (int)(i - row * lanes_row) * 8;
+__global__ void __launch_bounds__(TB) lay_out_kernel(LayOut first, LayOut second, int64_t lanes_first, int64_t lanes) {
+    for (int64_t n = (int64_t)blockIdx.x * TB + threadIdx.x; n < lanes; n += (int64_t)gridDim.x * TB) {
+        const LayOut &m = n < lanes_first ? first : second;
+        const int64_t i = n < lanes_first ? n : n - lanes_first, row = i / m.lanes_row;
+        const int c = (int)(i - row * m.lanes_row) * 8;
         float f[8];
-        load8(x + row * C, c, C, vec, f);
+        if (m.C % 8 == 0) load8<T, true>((const T *)m.from + row * m.C, c, m.C, f);
+        else load8<T, false>((const T *)m.from + row * m.C, c, m.C, f);
         Pack<E, 8> o[NP];
 #pragma unroll
         for (int v = 0; v < 8; ++v) split_pack<E, NP>(f[v], v, o);
 #pragma unroll
-        for (int n = 0; n < NP; ++n) *reinterpret_cast<Pack<E, 8> *>(y + n * plane + i * 8) = o[n];
+        for (int k = 0; k < NP; ++k) *reinterpret_cast<Pack<E, 8> *>((E *)m.to + (k * m.rows * m.lanes_row + i) * 8) = o[k];
     }
 }
 
 // dz = dy act'(z) laid out as an operand (where dz is given), and its column sums over a chunk of rows. A workgroup has
 // `cols` lanes of 8 channels and TB / cols rows side by side.
-template <typename T, typename E, int NP>
+template <typename T, typename E, int NP, bool VEC>
 __global__ void __launch_bounds__(TB) slope_kernel(const T *__restrict__ dy, const T *__restrict__ pre, E *__restrict__ dz,
                                                    float *__restrict__ part, int64_t rows, int C, int lanes_row, int cols,
                                                    int64_t chunk, int64_t plane, int act) {
     __shared__ float red[TB * 8];
     const int t = threadIdx.x, lanes_r = TB / cols, col = t % cols, rl = t / cols;
     const int j = blockIdx.y * cols + col, c = j * 8;
-    const bool active = rl < lanes_r && j < lanes_row, vec = C % 8 == 0;
+    const bool active = rl < lanes_r && j < lanes_row;
     const int64_t first = blockIdx.x * chunk, last = first + chunk < rows ? first + chunk : rows;
     float s[8];
 #pragma unroll
@@ -883,8 +1032,8 @@ __global__ void __launch_bounds__(TB) slope_kernel(const T *__restrict__ dy, con
 #pragma unroll
             for (int u = 0; u < UNROLL; ++u) {
                 const int64_t ru = r0 + (int64_t)u * lanes_r, r = ru < last ? ru : first;
-                load8(dy + r * C, c, C, vec, d[u]);
-                if (act != TVDCN_ACT_NONE) load8(pre + r * C, c, C, vec, z[u]);
+                load8<T, VEC>(dy + r * C, c, C, d[u]);
+                if (act != TVDCN_ACT_NONE) load8<T, VEC>(pre + r * C, c, C, z[u]);
             }
 #pragma unroll
             for (int u = 0; u < UNROLL; ++u) {
@@ -971,20 +1120,11 @@ unsigned strided_grid(int64_t lanes) {
     return (unsigned)(b < 16384 ? b : 16384);
 }
 
-// The pieces' products: all of one piece, or float32's six in rising order of size (three where the columns' operand has
-// one piece)
-void set_pairs(Product &p, int nr, int nc) {
-    static const int8_t six[6][2] = {{2, 0}, {0, 2}, {1, 1}, {1, 0}, {0, 1}, {0, 0}};
-    p.npair = 0;
-    for (const auto &s : six)
-        if (s[0] < nr && s[1] < nc) p.pr[p.npair] = s[0], p.pc[p.npair] = s[1], ++p.npair;
-}
-
-template <typename E, typename T, bool RT, bool CT, int WR, int WC, int FR, int FC, int BK, int STAGES, int BLOCKS>
+template <typename T, bool RT, bool CT, int WR, int WC, int FR, int FC, int BK, int STAGES, int BLOCKS>
 hipError_t launch_tiles(Product &p, hipStream_t s) {
     constexpr int BR = WR * 16 * FR, BC = WC * 16 * FC, LDS = STAGES * (BR + BC) * BK * 2;
     static std::atomic<unsigned long long> done{0};
-    const auto kernel = product_kernel<E, T, RT, CT, WR, WC, FR, FC, BK, STAGES, BLOCKS>;
+    const auto kernel = product_kernel<T, RT, CT, WR, WC, FR, FC, BK, STAGES, BLOCKS>;
     if (hipError_t e = raise_lds_limit((const void *)kernel, done)) return e;
     p.tiles_r = (int)ceil_div(p.rows, BR);
     p.tiles_c = (int)ceil_div(p.cols, BC);
@@ -992,139 +1132,153 @@ hipError_t launch_tiles(Product &p, hipStream_t s) {
     return hipGetLastError();
 }
 
-template <typename E, typename T, bool RT, bool CT, int FC> hipError_t launch_wide(Product &p, hipStream_t s) {
-    static std::atomic<unsigned long long> done{0};
-    const auto kernel = wide_product_kernel<E, T, RT, CT, FC>;
+// the persistent kernels: a workgroup per CU
+template <typename K> hipError_t launch_persistent(K kernel, std::atomic<unsigned long long> &done, Product &p, int cols, int lds, hipStream_t s) {
     if (hipError_t e = raise_lds_limit((const void *)kernel, done)) return e;
     p.tiles_r = (int)ceil_div(p.rows, 256);
-    p.tiles_c = (int)ceil_div(p.cols, 64 * FC);
+    p.tiles_c = (int)ceil_div(p.cols, cols);
     const int64_t tiles = (int64_t)p.tiles_r * p.tiles_c * p.splits;
-    kernel<<<(unsigned)(tiles < 256 ? tiles : 256), 512, 2 * (32768 + 64 * FC * 128), s>>>(p);
+    kernel<<<(unsigned)(tiles < 256 ? tiles : 256), 512, lds, s>>>(p);
     return hipGetLastError();
 }
-
+template <typename T, bool RT, bool CT, int FC> hipError_t launch_wide(Product &p, hipStream_t s) {
+    static std::atomic<unsigned long long> done{0};
+    return launch_persistent(wide_product_kernel<T, RT, CT, FC>, done, p, 64 * FC, 2 * (32768 + 64 * FC * 128), s);
+}
 template <bool RT, bool CT, int PC> hipError_t launch_pieces(Product &p, hipStream_t s) {
     static std::atomic<unsigned long long> done{0};
-    const auto kernel = pieces_product_kernel<RT, CT, PC>;
-    if (hipError_t e = raise_lds_limit((const void *)kernel, done)) return e;
-    p.tiles_r = (int)ceil_div(p.rows, 256);
-    p.tiles_c = (int)ceil_div(p.cols, 128);
-    const int64_t tiles = (int64_t)p.tiles_r * p.tiles_c * p.splits;
-    kernel<<<(unsigned)(tiles < 256 ? tiles : 256), 512, 2 * (12 + 2 * PC) * 4096, s>>>(p);
+    return launch_persistent(pieces_product_kernel<RT, CT, PC>, done, p, 128, 2 * (12 + 2 * PC) * 4096, s);
+}
+template <bool RT, bool CT> hipError_t launch_float(Product &p, hipStream_t s) {
+    p.tiles_r = (int)ceil_div(p.rows, 64);
+    p.tiles_c = (int)ceil_div(p.cols, 64);
+    float_product_kernel<RT, CT><<<(unsigned)(p.tiles_r * p.tiles_c * p.splits), 256, 0, s>>>(p, p.R.ld % 4 == 0, p.C.ld % 4 == 0);
     return hipGetLastError();
 }
 
-// Which tiles an output takes: 256 x 256 or 256 x 128 (of whole eights of columns), one workgroup per CU; 128 x 128 or 64 x 64,
-// two per CU. The least of what they take, in microseconds: launch, first loads and results, and so much per step of 64 along
-// the reduction and round of workgroups. Measured in bfloat16, 16 steps: 2048 x 1024 takes 33.6 / 23.7 / 21.1 / 15.6 us in the
-// four; 24 steps, 32768 x 256: 47.8 / 35.0 / 43.3 / 79.7; 32 steps, 65536 x 512: 130 / 166 / 253 / -.
-// float32 (all its pieces' products): 32768 x 256 from 256 takes 33.7 us by the pieces' own kernel, 41.3 / 43.9 / 68.4 in 256 x
-// 128, 128 x 128 and 64 x 64; 8192 x 256 26.5, 35.4 / 29.0 / 21.8.
-enum Tiles { PIECES, WIDE, HALF, BIG, SMALL };
+// Which tiles an output takes. 16 bits: 256 x 256 or 256 x 128 (of whole eights of columns), one workgroup per CU; 128 x 128 or 64 x
+// 64, two per CU. float32: in pieces, 256 x 128, or as it lies, 64 x 64. The least of what they take, in microseconds: launch,
+// first loads and results, and so much per step of 64 along the reduction and round of workgroups. Measured in bfloat16, 16 steps:
+// 2048 x 1024 takes 33.6 / 23.7 / 21.1 / 15.6 us in the four; 24 steps, 32768 x 256: 47.8 / 35.0 / 43.3 / 79.7; 32 steps, 65536 x
+// 512: 130 / 166 / 253 / -. float32, 4 steps, 32768 x 256: 33.7 / 49.3; 8192 x 256: 26.3 / 16.9; 32 steps, 4096 x 2048: 166 / 339.
+enum Tiles { WIDE, HALF, BIG, SMALL, PIECES, FLOAT };
 double tiles_cost(Tiles t, int64_t rows, int64_t cols, int64_t splits, double steps) {
     auto count = [&](int64_t r, int64_t c) { return ceil_div(rows, r) * ceil_div(cols, c) * splits; };
     switch (t) {
-        case PIECES: return 10 + 0.87 * steps * (double)ceil_div(count(256, 128), 256);
         case WIDE: return 10 + 1.75 * steps * (double)ceil_div(count(256, 256), 256);
         case HALF: return 7 + 1.2 * steps * (double)ceil_div(count(256, 128), 256);
         case BIG: return 6 + steps * (count(128, 128) <= 256 ? 0.95 : 1.7 * (double)ceil_div(count(128, 128), 512));
-        default: return 4 + steps * (count(64, 64) <= 256 ? 0.55 : 0.75 * (double)ceil_div(count(64, 64), 512));
+        case SMALL: return 4 + steps * (count(64, 64) <= 256 ? 0.55 : 0.75 * (double)ceil_div(count(64, 64), 512));
+        case PIECES: return 10 + 5.2 * steps * (double)ceil_div(count(256, 128), 256);
+        default: return 6 + steps * std::max(2.2, 1.28 * (double)count(64, 64) / 256);
     }
 }
-bool tiles_fit(Tiles t, bool wide, int64_t cols) {   // wide: float32
-    return t >= BIG || (cols % 8 == 0 && (t == PIECES) == wide);
-}
-Tiles choose_tiles(bool wide, int64_t rows, int64_t cols, double steps) {
+Tiles choose_tiles(int64_t rows, int64_t cols, double steps) {   // 16 bits
     Tiles best = SMALL;
-    for (Tiles t : {BIG, HALF, WIDE, PIECES})
-        if (tiles_fit(t, wide, cols) && tiles_cost(t, rows, cols, 1, steps) < tiles_cost(best, rows, cols, 1, steps)) best = t;
+    for (Tiles t : {BIG, HALF, WIDE})
+        if ((t == BIG || cols % 8 == 0) && tiles_cost(t, rows, cols, 1, steps) < tiles_cost(best, rows, cols, 1, steps)) best = t;
     return best;
 }
 
-template <typename E, typename T, bool RT, bool CT> hipError_t launch_product(Product p, Tiles tiles, hipStream_t s) {
+template <typename T, bool RT, bool CT> hipError_t launch_product(Product p, Tiles tiles, hipStream_t s) {
     if constexpr (is_f32<T>()) {
-        if (tiles == PIECES) {
-            if (p.npair == 6) return launch_pieces<RT, CT, 3>(p, s);
-            if constexpr (RT) return launch_pieces<RT, CT, 1>(p, s);   // the weight gradient of a kept input
-        }
+        if (tiles == FLOAT) return launch_float<RT, CT>(p, s);
+        if constexpr (RT)   // (the weight gradient, perhaps of a kept input)
+            if (p.pieces_c == 1) return launch_pieces<RT, CT, 1>(p, s);
+        return launch_pieces<RT, CT, 3>(p, s);
     } else {
-        if (tiles == WIDE) return launch_wide<E, T, RT, CT, 4>(p, s);
-        if (tiles == HALF) return launch_wide<E, T, RT, CT, 2>(p, s);
-    }
-    switch (tiles) {
-        case BIG: return launch_tiles<E, T, RT, CT, 2, 2, 4, 4, 64, 2, 2>(p, s);
-        default: return launch_tiles<E, T, RT, CT, 2, 2, 2, 2, 64, 3, 2>(p, s);
+        switch (tiles) {
+            case WIDE: return launch_wide<T, RT, CT, 4>(p, s);
+            case HALF: return launch_wide<T, RT, CT, 2>(p, s);
+            case BIG: return launch_tiles<T, RT, CT, 2, 2, 4, 4, 64, 2, 2>(p, s);
+            default: return launch_tiles<T, RT, CT, 2, 2, 2, 2, 64, 3, 2>(p, s);
+        }
     }
 }
 
 // y or dx: rows in runs whose workgroups HIP takes in one launch
-template <typename E, typename T, bool CT> hipError_t launch_rows(Product p, int64_t rows, hipStream_t s) {
+template <typename T, bool CT> hipError_t launch_rows(Product p, bool pieces, int64_t rows, hipStream_t s) {
     const int64_t run = (int64_t)(1 << 22) / ceil_div(p.cols, 64) * 64;
     const char *r = (const char *)p.R.p;
-    const int64_t ld = p.R.ld;
-    const double steps = (double)ceil_div(p.share, 64) * p.npair;
+    const int64_t bytes = p.R.ld * (is_f32<T>() && !pieces ? 4 : 2);
     T *out = (T *)p.out, *pre = (T *)p.pre;
     const T *res = (const T *)p.residual;
     for (int64_t first = 0; first < rows; first += run) {
         p.rows = (int)(rows - first < run ? rows - first : run);
-        p.R.p = r + first * ld * 2;
+        p.R.p = r + first * bytes;
         p.R.width = p.rows;
         p.out = out + first * p.cols;
         p.pre = pre ? pre + first * p.cols : nullptr;
         p.residual = res ? res + first * p.cols : nullptr;
-        if (hipError_t e = launch_product<E, T, false, CT>(p, choose_tiles(is_f32<T>(), p.rows, p.cols, steps), s)) return e;
+        const Tiles tiles = is_f32<T>() ? (pieces ? PIECES : FLOAT) : choose_tiles(p.rows, p.cols, (double)ceil_div(p.share, 64));
+        if (hipError_t e = launch_product<T, false, CT>(p, tiles, s)) return e;
     }
     return hipSuccess;
 }
 
-template <typename T, typename E, int NP>
-hipError_t lay_out(const void *x, void *y, int64_t rows, int C, hipStream_t s) {
-    const int lanes_row = (int)ceil_div(C, 8);
-    lay_out_kernel<T, E, NP><<<strided_grid(rows * lanes_row), TB, 0, s>>>((const T *)x, (E *)y, rows, C, lanes_row,
-                                                                        rows * lanes_row * 8);
+template <typename T, typename E, int NP> hipError_t lay_out(const LayOut &first, const LayOut &second, hipStream_t s) {
+    const int64_t lanes = first.lanes() + second.lanes();
+    lay_out_kernel<T, E, NP><<<strided_grid(lanes), TB, 0, s>>>(first, second, first.lanes(), lanes);
     return hipGetLastError();
 }
 
+// float32 in pieces or as it lies: the pieces' products run at about 190 TFLOP/s against 105, and cost the operands' copies
+// (10 bytes a value at 5 TB/s; in the backward dz in pieces too, 2 bytes a value more) and about 12 us of launches and first loads a
+// product. The pieces' kernel writes whole eights of columns.
+bool forward_in_pieces(const PointwiseArgs &a) {
+    const double saved = 2.0 * a.rows * a.in * a.out * 4.26e-9;
+    return f32(a) && a.out % 8 == 0 && saved > 12 + a.rows * 2e-6 * a.in;
+}
+bool backward_in_pieces(const PointwiseArgs &a) {
+    const double saved = 4.0 * a.rows * a.in * a.out * 4.26e-9;
+    return f32(a) && a.in % 8 == 0 && saved > 24 + a.rows * (2e-6 * a.in + 0.4e-6 * a.out);
+}
+
 struct Plan {
-    int64_t pi, po;                    // pitches of the channels
+    bool pieces;                       // (float32)
+    int64_t pi, po;                    // pitches of the channels of x and W, of dz
     bool x_laid, w_laid, dz_laid;      // the operand is a copy in the workspace
-    int np, npx;                       // pieces per value; of x in the backward
-    size_t x_at, w_at, dz_at, part_at, sums_at, forward, backward;
+    size_t x_at, w_at, dz_at, part_at, sums_at, bytes;
     int cols, chunks;                  // bias gradient: lanes of channels, chunks of rows
     int64_t chunk;
     Tiles tiles;                       // weight gradient: its tiles, and shares of the rows
     int splits;
     int64_t share;
+    size_t take(size_t n) {
+        const size_t at = bytes;
+        bytes += align256(n);
+        return at;
+    }
 };
 
-Plan make_plan(const PointwiseArgs &a) {
+Plan forward_plan(const PointwiseArgs &a) {
     Plan k{};
-    const bool wide = f32(a);
-    k.pi = round_up(a.in, 8);
-    k.po = round_up(a.out, 8);
-    k.np = wide ? 3 : 1;
-    const bool odd_in = a.in % 8 != 0, odd_out = a.out % 8 != 0;
-    k.w_laid = wide || odd_in;
-    k.x_laid = wide || odd_in;   // forward
-    size_t off = 0;
-    auto take = [&](size_t bytes) {
-        const size_t at = off;
-        off += align256(bytes);
-        return at;
-    };
-    k.w_at = k.w_laid ? take((size_t)a.out * k.pi * 2 * k.np) : 0;
-    k.x_at = k.x_laid ? take((size_t)a.rows * k.pi * 2 * k.np) : 0;
-    k.forward = off;
+    k.pieces = forward_in_pieces(a);
+    k.x_laid = k.w_laid = k.pieces || (!f32(a) && a.in % 8 != 0);
+    k.pi = k.x_laid ? round_up(a.in, 8) : a.in;
+    const size_t value = k.pieces ? 6 : 2;
+    if (k.w_laid) k.w_at = k.take((size_t)a.out * k.pi * value);
+    if (k.x_laid) k.x_at = k.take((size_t)a.rows * k.pi * value);
+    return k;
+}
 
-    off = 0;
-    const bool kept = a.codes != nullptr;
-    k.npx = wide && !kept ? 3 : 1;
-    k.dz_laid = wide || odd_out || a.act != TVDCN_ACT_NONE;
-    if (k.w_laid) k.w_at = take((size_t)a.out * k.pi * 2 * k.np);
-    if (k.x_laid || kept) k.x_at = take((size_t)a.rows * k.pi * 2 * k.npx);
-    k.dz_at = k.dz_laid ? take((size_t)a.rows * k.po * 2 * k.np) : 0;
+Plan backward_plan(const PointwiseArgs &a) {
+    Plan k{};
+    const bool wide = f32(a), kept = a.codes != nullptr;
+    k.pieces = backward_in_pieces(a);
+    const bool copies = k.pieces || (!wide && a.in % 8 != 0);
+    k.w_laid = copies;
+    k.x_laid = copies && !kept;
+    k.pi = copies || kept ? round_up(a.in, 8) : a.in;
+    k.dz_laid = k.pieces || a.act != TVDCN_ACT_NONE || (!wide && a.out % 8 != 0);
+    k.po = k.dz_laid ? round_up(a.out, 8) : a.out;
+    const size_t plain = wide ? 4 : 2, value = k.pieces ? 6 : plain;
+    if (k.w_laid) k.w_at = k.take((size_t)a.out * k.pi * value);
+    if (k.x_laid) k.x_at = k.take((size_t)a.rows * k.pi * value);
+    if (kept) k.x_at = k.take((size_t)a.rows * k.pi * (k.pieces ? 2 : plain));
+    if (k.dz_laid) k.dz_at = k.take((size_t)a.rows * k.po * value);
     // about 1024 workgroups, at most 256 chunks: the last step adds them up
-    const int lanes = (int)(k.po / 8);
+    const int lanes = (int)ceil_div(a.out, 8);
     k.cols = lanes < 32 ? lanes : 32;
     int64_t chunks = ceil_div(1024, ceil_div(lanes, k.cols));
     const int64_t most = ceil_div(a.rows, (TB / k.cols) * 4);
@@ -1132,43 +1286,45 @@ Plan make_plan(const PointwiseArgs &a) {
     chunks = chunks < 256 ? chunks : 256;
     k.chunk = ceil_div(a.rows, chunks < 1 ? 1 : chunks);
     k.chunks = (int)ceil_div(a.rows, k.chunk < 1 ? 1 : k.chunk);
-    k.part_at = take((size_t)k.chunks * a.out * 4);
-    // shares of the rows: as many as give every CU its workgroups, each share at least four steps. The shares' sums are
-    // written and read again: 8 bytes per output and share, at about 4 TB/s.
-    const int64_t most_splits = std::max<int64_t>(1, a.rows / (4 * SHARE));
+    k.part_at = k.take((size_t)k.chunks * a.out * 4);
+    // shares of the rows: as many as give every CU its workgroups, each share at least four steps (two of the slower float32 ones).
+    // The shares' sums are written and read again: 8 bytes per output and share, at about 4 TB/s.
+    const int64_t most_splits = std::max<int64_t>(1, a.rows / ((wide ? 2 : 4) * SHARE));
     double least = 0;
     int64_t splits = 0;
     for (const auto &[t, r, c, slots] : {std::tuple<Tiles, int, int, int>{SMALL, 64, 64, 512}, {BIG, 128, 128, 256},
                                          {BIG, 128, 128, 512}, {HALF, 256, 128, 256}, {WIDE, 256, 256, 256},
-                                         {PIECES, 256, 128, 256}}) {
-        if (!tiles_fit(t, wide, a.in)) continue;
+                                         {PIECES, 256, 128, 256}, {FLOAT, 64, 64, 256}, {FLOAT, 64, 64, 512},
+                                         {FLOAT, 64, 64, 1024}}) {
+        if (wide ? t != (k.pieces ? PIECES : FLOAT) : t >= PIECES || (t <= HALF && a.in % 8 != 0)) continue;
         const int64_t n = std::min(std::max<int64_t>(1, slots / (ceil_div(a.out, r) * ceil_div(a.in, c))), most_splits);
-        const double steps = (double)ceil_div(ceil_div(a.rows, n), SHARE) * k.np * (k.npx == 3 ? 2 : 1);
+        const double steps = (double)ceil_div(ceil_div(a.rows, n), SHARE);
         const double cost = tiles_cost(t, a.out, a.in, n, steps) + (n > 1 ? (double)(n * a.out) * a.in * 2e-6 : 0.0);
         if (splits == 0 || cost < least) least = cost, splits = n, k.tiles = t;
     }
     k.share = round_up(ceil_div(a.rows, splits), SHARE);
     k.splits = (int)ceil_div(a.rows, k.share < 1 ? 1 : k.share);
-    k.sums_at = k.splits > 1 ? take((size_t)k.splits * a.out * a.in * 4) : 0;
-    k.backward = off;
+    k.sums_at = k.splits > 1 ? k.take((size_t)k.splits * a.out * a.in * 4) : 0;
     return k;
 }
 
-template <typename T, typename E, int NP> hipError_t forward(const PointwiseArgs &a, hipStream_t s) {
-    const Plan k = make_plan(a);
-    const void *x = a.x, *w = a.weight;
-    if (k.w_laid) {
-        if (hipError_t e = lay_out<T, E, NP>(w, a.work + k.w_at, a.out, a.in, s)) return e;
-        w = a.work + k.w_at;
-    }
-    if (k.x_laid) {
-        if (hipError_t e = lay_out<T, E, NP>(x, a.work + k.x_at, a.rows, a.in, s)) return e;
-        x = a.work + k.x_at;
-    }
+// The operands that are copied: x (unless it is kept in 8 bits, or not asked for) and W
+template <typename T> hipError_t lay_out_operands(const PointwiseArgs &a, const Plan &k, bool x, bool w, hipStream_t s) {
+    const int lanes = (int)(k.pi / 8);
+    LayOut first{a.x, a.work + k.x_at, x && k.x_laid ? a.rows : 0, a.in, lanes};
+    LayOut second{a.weight, a.work + k.w_at, w && k.w_laid ? a.out : 0, a.in, lanes};
+    if (first.rows + second.rows == 0) return hipSuccess;
+    if constexpr (is_f32<T>()) return lay_out<T, bf16, 3>(first, second, s);
+    else return lay_out<T, T, 1>(first, second, s);
+}
+
+template <typename T> hipError_t forward(const PointwiseArgs &a, hipStream_t s) {
+    const Plan k = forward_plan(a);
+    if (hipError_t e = lay_out_operands<T>(a, k, true, true, s)) return e;
     Product p{};
-    p.R = {x, k.pi, a.rows * k.pi, k.pi, a.rows};
-    p.C = {w, k.pi, a.out * k.pi, k.pi, a.out};
-    set_pairs(p, NP, NP);
+    p.R = {k.x_laid ? a.work + k.x_at : a.x, k.pi, a.rows * k.pi, k.pi, a.rows};
+    p.C = {k.w_laid ? a.work + k.w_at : a.weight, k.pi, a.out * k.pi, k.pi, a.out};
+    p.pieces_c = 3;
     p.cols = a.out;
     p.splits = 1;
     p.share = k.pi;
@@ -1177,87 +1333,90 @@ template <typename T, typename E, int NP> hipError_t forward(const PointwiseArgs
     p.residual = a.residual;
     p.pre = a.pre;
     p.act = a.act;
-    return launch_rows<E, T, false>(p, a.rows, s);
+    return launch_rows<T, false>(p, k.pieces, a.rows, s);
 }
 
-template <typename T, typename E, int NP> hipError_t backward(const PointwiseArgs &a, hipStream_t s) {
-    const Plan k = make_plan(a);
-    const void *dz = a.dy, *w = a.weight, *x = a.x;
+// dz as an operand (to == null: not needed so) and the bias gradient's chunks (part == null: not needed)
+template <typename T, typename E, int NP> hipError_t slopes(const PointwiseArgs &a, const Plan &k, void *to, float *part, hipStream_t s) {
+    const int lanes = (int)ceil_div(a.out, 8);
+    const auto kernel = a.out % 8 == 0 ? slope_kernel<T, E, NP, true> : slope_kernel<T, E, NP, false>;
+    kernel<<<dim3(k.chunks, (unsigned)ceil_div(lanes, k.cols)), TB, 0, s>>>(
+        (const T *)a.dy, (const T *)a.pre, (E *)to, part, a.rows, a.out, lanes, k.cols, k.chunk, a.rows * k.po, a.act);
+    return hipGetLastError();
+}
+
+template <typename T> hipError_t backward(const PointwiseArgs &a, hipStream_t s) {
+    const Plan k = backward_plan(a);
+    const bool any = a.rows > 0, need_dx = any && a.dx, need_dw = any && a.dweight;
     float *part = a.dbias ? (float *)(a.work + k.part_at) : nullptr;
-    const bool need_dz = a.dx || a.dweight;
-    if (a.rows > 0 && (a.dbias || (need_dz && k.dz_laid))) {
-        const int lanes = (int)(k.po / 8);
-        E *to = need_dz && k.dz_laid ? (E *)(a.work + k.dz_at) : nullptr;
-        slope_kernel<T, E, NP><<<dim3(k.chunks, (unsigned)ceil_div(lanes, k.cols)), TB, 0, s>>>(
-            (const T *)a.dy, (const T *)a.pre, to, part, a.rows, a.out, lanes, k.cols, k.chunk, a.rows * k.po, a.act);
-        if (hipError_t e = hipGetLastError()) return e;
-        if (to) dz = to;
+    void *laid = (need_dx || need_dw) && k.dz_laid ? a.work + k.dz_at : nullptr;
+    const void *dz = laid ? laid : a.dy;
+    if (any && (part || laid)) {
+        hipError_t e;
+        if constexpr (is_f32<T>()) e = k.pieces ? slopes<T, bf16, 3>(a, k, laid, part, s) : slopes<T, float, 1>(a, k, laid, part, s);
+        else e = slopes<T, T, 1>(a, k, laid, part, s);
+        if (e) return e;
     }
-    if (a.dx && a.rows > 0) {
-        if (k.w_laid) {
-            if (hipError_t e = lay_out<T, E, NP>(w, a.work + k.w_at, a.out, a.in, s)) return e;
-            w = a.work + k.w_at;
-        }
+    if (hipError_t e = lay_out_operands<T>(a, k, need_dw, need_dx, s)) return e;
+    // (as they lie, float32 operands end at their own channels; copies are zeros up to their pitch)
+    const bool lies = f32(a) && !k.pieces;
+    if (need_dx) {
         Product p{};
-        p.R = {dz, k.po, a.rows * k.po, k.po, a.rows};
-        p.C = {w, k.pi, a.out * k.pi, a.out, k.pi};
-        set_pairs(p, NP, NP);
+        p.R = {dz, k.po, a.rows * k.po, lies ? a.out : k.po, a.rows};
+        p.C = {k.w_laid ? a.work + k.w_at : a.weight, k.w_laid ? k.pi : a.in, a.out * k.pi, a.out, k.w_laid ? k.pi : a.in};
+        p.pieces_c = 3;
         p.cols = a.in;
         p.splits = 1;
-        p.share = k.po;
+        p.share = lies ? a.out : k.po;
         p.out = a.dx;
-        if (hipError_t e = launch_rows<E, T, true>(p, a.rows, s)) return e;
+        if (hipError_t e = launch_rows<T, true>(p, k.pieces, a.rows, s)) return e;
     }
-    if (a.dweight && a.rows > 0) {
-        if (a.codes) {
-            if (hipError_t e = launch_expand(a.dtype, f32(a), a.rows, a.in, k.pi, a.codes, a.exps, a.work + k.x_at, s)) return e;
-            x = a.work + k.x_at;
-        } else if (k.x_laid) {
-            if (hipError_t e = lay_out<T, E, NP>(x, a.work + k.x_at, a.rows, a.in, s)) return e;
-            x = a.work + k.x_at;
-        }
+    if (need_dw) {
+        const void *x = a.codes || k.x_laid ? a.work + k.x_at : a.x;
+        if (a.codes)
+            if (hipError_t e = launch_expand(a.dtype, k.pieces, a.rows, a.in, k.pi, a.codes, a.exps, a.work + k.x_at, s)) return e;
         Product p{};
-        p.R = {dz, k.po, a.rows * k.po, a.rows, k.po};
-        p.C = {x, k.pi, a.rows * k.pi, a.rows, k.pi};
-        set_pairs(p, NP, k.npx);
+        p.R = {dz, k.po, a.rows * k.po, a.rows, lies ? a.out : k.po};
+        p.C = {x, k.pi, a.rows * k.pi, a.rows, lies ? a.in : k.pi};
+        p.pieces_c = a.codes ? 1 : 3;
         p.rows = a.out;
         p.cols = a.in;
         p.splits = k.splits;
         p.share = k.share;
         p.sums = k.splits > 1;
         p.out = p.sums ? (void *)(a.work + k.sums_at) : a.dweight;
-        if (hipError_t e = launch_product<E, T, true, true>(p, k.tiles, s)) return e;
+        if (hipError_t e = launch_product<T, true, true>(p, k.tiles, s)) return e;
     }
     // (no rows: zeros, the sum of nothing)
-    const bool sum_w = a.dweight && (k.splits > 1 || a.rows == 0);
+    const bool sum_w = a.dweight && (k.splits > 1 || !any);
     const int64_t n = (int64_t)a.out * a.in;
     const int w_blocks = sum_w ? (int)std::min<int64_t>(ceil_div(n, FIN), 4096) : 0, b_blocks = a.dbias ? (int)ceil_div(a.out, 16) : 0;
     if (w_blocks + b_blocks == 0) return hipSuccess;
     finish_kernel<T><<<(unsigned)(w_blocks + b_blocks), FIN, 0, s>>>((const float *)(a.work + k.sums_at), (T *)a.dweight, n,
-                                                                   a.rows ? k.splits : 0, w_blocks, part, (T *)a.dbias,
-                                                                   a.out, a.rows ? k.chunks : 0);
+                                                                   any ? k.splits : 0, w_blocks, part, (T *)a.dbias,
+                                                                   a.out, any ? k.chunks : 0);
     return hipGetLastError();
 }
 
 }  // namespace
 
-size_t pointwise_forward_bytes(const PointwiseArgs &a) { return make_plan(a).forward; }
-size_t pointwise_backward_bytes(const PointwiseArgs &a) { return make_plan(a).backward; }
+size_t pointwise_forward_bytes(const PointwiseArgs &a) { return forward_plan(a).bytes; }
+size_t pointwise_backward_bytes(const PointwiseArgs &a) { return backward_plan(a).bytes; }
 
 hipError_t launch_pointwise_forward(const PointwiseArgs &a, hipStream_t s) {
     if (a.rows == 0) return hipSuccess;
     switch (a.dtype) {
-        case TVDCN_DTYPE_FLOAT32: return forward<float, bf16, 3>(a, s);
-        case TVDCN_DTYPE_FLOAT16: return forward<f16, f16, 1>(a, s);
-        default: return forward<bf16, bf16, 1>(a, s);
+        case TVDCN_DTYPE_FLOAT32: return forward<float>(a, s);
+        case TVDCN_DTYPE_FLOAT16: return forward<f16>(a, s);
+        default: return forward<bf16>(a, s);
     }
 }
 
 hipError_t launch_pointwise_backward(const PointwiseArgs &a, hipStream_t s) {
     switch (a.dtype) {
-        case TVDCN_DTYPE_FLOAT32: return backward<float, bf16, 3>(a, s);
-        case TVDCN_DTYPE_FLOAT16: return backward<f16, f16, 1>(a, s);
-        default: return backward<bf16, bf16, 1>(a, s);
+        case TVDCN_DTYPE_FLOAT32: return backward<float>(a, s);
+        case TVDCN_DTYPE_FLOAT16: return backward<f16>(a, s);
+        default: return backward<bf16>(a, s);
     }
 }
 
