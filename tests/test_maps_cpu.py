@@ -293,7 +293,7 @@ def test_c_abi_refuses_descriptors(lib):
 
 def test_c_abi_refuses_pointers_and_workspaces(lib):
     p, odd, big = P(4096), P(4104), 1 << 40
-    d = ctypes.byref(norm_desc())
+    d = ctypes.byref(norm_desc(pixels=1 << 20))   # (groups that a workgroup holds need no workspace forward)
     f, b = lib.tvdcn_group_norm_act_forward, lib.tvdcn_group_norm_act_backward
     assert f(None, p, p, p, p, p, p, p, big, None) == INVALID
     assert f(d, None, p, p, p, p, p, p, big, None) == INVALID and f(d, p, p, p, None, p, p, p, big, None) == INVALID
@@ -307,7 +307,7 @@ def test_c_abi_refuses_pointers_and_workspaces(lib):
     assert b(d, p, None, p, None, p, p, p, p, p, p, p, p, big, None) == INVALID       # codes alone
     assert b(d, None, p, None, None, p, p, p, p, p, p, p, p, big, None) == INVALID
     assert b(d, p, p, None, None, p, p, p, p, None, None, None, p, big, None) == SUCCESS   # nothing asked for
-    d = ctypes.byref(point_desc(activation=2))
+    d = ctypes.byref(point_desc(dtype=2, activation=2, in_channels=9))   # (channels in eights, or float32: none)
     f, b = lib.tvdcn_pointwise_conv_forward, lib.tvdcn_pointwise_conv_backward
     assert f(d, None, p, p, p, p, p, p, big, None) == INVALID and f(d, p, p, p, p, None, p, p, big, None) == INVALID
     assert f(d, p, p, odd, p, p, p, p, big, None) == INVALID
@@ -319,7 +319,11 @@ def test_c_abi_refuses_pointers_and_workspaces(lib):
     assert b(d, p, p, p, p, p, p, p, p, p, p, big, None) == INVALID
     assert b(d, p, None, None, None, p, p, p, p, p, p, big, None) == INVALID
     assert b(d, p, p, None, None, None, p, p, p, p, p, big, None) == INVALID
-    # 16-bit maps of whole eights of channels are multiplied where they lie
+    assert lib.tvdcn_group_norm_act_forward_workspace_size(ctypes.byref(norm_desc())) == 0
+    # 16-bit maps of whole eights of channels are multiplied where they lie, and so are float32 ones of small products
+    assert lib.tvdcn_pointwise_conv_forward_workspace_size(ctypes.byref(point_desc(dtype=0, in_channels=9))) == 0
+    large = dict(rows=1 << 20, in_channels=512, out_channels=512)
+    assert lib.tvdcn_pointwise_conv_forward_workspace_size(ctypes.byref(point_desc(**large))) > 0
     assert lib.tvdcn_pointwise_conv_forward_workspace_size(ctypes.byref(point_desc(dtype=3))) == 0
     # rows of none: nothing to do, no pointers needed
     assert f(ctypes.byref(point_desc(rows=0)), None, None, None, None, None, None, None, 0, None) == SUCCESS
