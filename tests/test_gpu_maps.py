@@ -149,6 +149,19 @@ def test_pointwise_float32_is_float32_accurate():
     assert torch.equal(tvdcn.pointwise_conv(big, torch.eye(8, device="cuda")), big)
 
 
+@pytest.mark.parametrize("device", ["cpu", "cuda"])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_float16_arguments_beyond_its_range(act, device):
+    """z = +-100000 is no float16: the activation is z or 0 there and its slope 1 or 0."""
+    x = torch.full((3, 8), 250.0, dtype=torch.float16, device=device)
+    w = torch.full((8, 8), 50.0, dtype=torch.float16, device=device)
+    w[4:] = -50.0
+    r = torch.zeros(3, 8, dtype=torch.float16, device=device)
+    y, dx, dw = run_pointwise(x, w, None, r, act, torch.ones_like(r))
+    assert torch.isposinf(y[:, :4]).all() and not y[:, 4:].any()
+    assert (dx == 200.0).all() and (dw[:4] == 750.0).all() and not dw[4:].any()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_only_the_gradients_asked_for(dtype):
     x, w, b = make((2, 24, 9), dtype, 1), make((16, 24), dtype, 2), make((16,), dtype, 3)

@@ -5,6 +5,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../../include/tvdcn_hip.h"
 
 namespace tvdcn_hip {
@@ -151,6 +153,15 @@ template <typename T> __device__ __forceinline__ float most() { return 0.f; }
 template <> __device__ __forceinline__ float most<float>() { return 3.402823466e38f; }
 template <> __device__ __forceinline__ float most<f16>() { return 65504.f; }
 template <> __device__ __forceinline__ float most<bf16>() { return 3.389531390e38f; }
+
+// The activation's argument as it is kept for the backward: a finite one beyond float16 stays finite, at whose largest values the
+// slopes are what they are further out (0 or 1; at an infinity they would be NaN)
+template <typename T> __device__ __forceinline__ T kept_argument(float z) {
+    if constexpr (std::is_same<T, f16>::value) {
+        if (fabsf(z) < __builtin_inff()) z = fminf(fmaxf(z, -most<f16>()), most<f16>());
+    }
+    return (T)z;
+}
 
 // What code q of exponent byte e stands for: q * 2^(e - bias) clamped to T's finite values, NaN for a block that held a value
 // that is not finite. The scaling is exact; only 64 and more steps of the largest exponent of all pass the finite values.

@@ -185,7 +185,7 @@ __device__ __forceinline__ void emit(const Product &p, int split, int row, int c
         P o;
         if (p.pre) {
 #pragma unroll
-            for (int v = 0; v < RUN; ++v) o.v[v] = (T)z[v];
+            for (int v = 0; v < RUN; ++v) o.v[v] = kept_argument<T>(z[v]);
             *reinterpret_cast<P *>((T *)p.pre + at) = o;
         }
 #pragma unroll
@@ -207,7 +207,7 @@ __device__ __forceinline__ void emit(const Product &p, int split, int row, int c
         if (p.pre)
 #pragma unroll
             for (int v = 0; v < RUN; ++v)
-                if (v <= last) ((T *)p.pre)[at + v] = (T)z[v];
+                if (v <= last) ((T *)p.pre)[at + v] = kept_argument<T>(z[v]);
         act_values<is_f32<T>(), RUN>(z, p.act);
 #pragma unroll
         for (int v = 0; v < RUN; ++v)
@@ -416,7 +416,7 @@ __device__ __forceinline__ void store_results(const Product &p, const fvec4 (&ac
                         for (int e = 0; e < RUN; ++e) v[e] += (float)bias[r].v[e];
                     if (p.pre) {
 #pragma unroll
-                        for (int e = 0; e < RUN; ++e) o.v[e] = (T)v[e];
+                        for (int e = 0; e < RUN; ++e) o.v[e] = kept_argument<T>(v[e]);
                         *reinterpret_cast<Run *>((T *)p.pre + at_o) = o;
                     }
                     act_values<is_f32<T>(), RUN>(v, p.act);

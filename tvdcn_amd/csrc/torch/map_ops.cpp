@@ -453,6 +453,11 @@ Three point_backward_meta(const Tensor &grad, MaybeTensor input, MaybeTensor cod
             want[2] ? at::empty({weight.size(0)}, o) : Tensor()};
 }
 
+// the activation's argument in the map's type; a finite one beyond float16 stays finite
+Tensor kept_argument(const Tensor &z, at::ScalarType t) {
+    return t == at::kHalf ? at::where(z.isfinite(), z.clamp(-65504.0, 65504.0), z).to(t) : z.to(t);
+}
+
 Two point_forward_cpu(const Tensor &x, const Tensor &weight, MaybeTensor bias, MaybeTensor residual, int64_t act,
                       bool save_pre) {
     check_pointwise(x, weight, bias, residual, act);
@@ -464,7 +469,7 @@ Two point_forward_cpu(const Tensor &x, const Tensor &weight, MaybeTensor bias, M
     Tensor v = act_value(z, act);
     if (has(residual)) v = v + to_rows(*residual).to(t).reshape(v.sizes());
     return {to_map(v.to(x.scalar_type()).reshape(y.sizes())),
-            save_pre ? to_map(z.to(x.scalar_type()).reshape(y.sizes())) : Tensor()};
+            save_pre ? to_map(kept_argument(z, x.scalar_type()).reshape(y.sizes())) : Tensor()};
 }
 Three point_backward_cpu(const Tensor &grad, MaybeTensor input, MaybeTensor codes, MaybeTensor exponents, const Tensor &weight,
                          MaybeTensor pre, int64_t act, std::array<bool, 3> want) {
