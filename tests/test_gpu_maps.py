@@ -162,6 +162,31 @@ def test_float16_arguments_beyond_its_range(act, device):
     assert (dx == 200.0).all() and (dw[:4] == 750.0).all() and not dw[4:].any()
 
 
+@pytest.mark.parametrize("device", ["cpu", "cuda"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_gradients_that_a_shut_rectifier_drops(bad, dtype, device):
+    """An infinity or a NaN in the gradient where relu is zero counts for nothing, in either operator."""
+    torch.manual_seed(3)
+    x = torch.randn(2, 16, 40, device=device).to(dtype)
+    w = torch.randn(24, 16, device=device).to(dtype)
+    for op, params in ((lambda v, *p: tvdcn.pointwise_conv(v, *p, activation="relu"), (w,)),
+                       (lambda v, *p: tvdcn.pointwise_conv(v, *p, residual=torch.ones_like(y), activation="relu"), (w,)),
+                       (lambda v, *p: tvdcn.group_norm_act(v, 4, *p, activation="relu"), (torch.ones_like(w[0]),)),
+                       (lambda v, *p: tvdcn.group_norm_act(v.repeat(1, 1, 600), 4, *p, activation="relu"), (torch.ones_like(w[0]),))):
+        with torch.no_grad():
+            y = tvdcn.pointwise_conv(x, w) if params[0] is w else op(x, *params)
+        shut = y <= 0
+        assert shut.any() and not shut.all()
+        got = []
+        for fill in (0.0, bad):
+            leaves = [leaf(x)] + [leaf(p) for p in params]
+            dy = torch.ones_like(y).masked_fill(shut, fill)
+            got.append(torch.autograd.grad(op(*leaves), leaves, dy))
+        for a, b in zip(*got):
+            assert b.isfinite().all() and torch.equal(a, b)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_only_the_gradients_asked_for(dtype):
     x, w, b = make((2, 24, 9), dtype, 1), make((16, 24), dtype, 2), make((16,), dtype, 3)

@@ -120,7 +120,6 @@ template <bool PRECISE, int N> __device__ __forceinline__ void act_values(float 
 }
 template <bool PRECISE> __device__ __forceinline__ float act_slope(float z, int act) {
     switch (act) {
-        case TVDCN_ACT_RELU: return z > 0.f ? 1.f : 0.f;
         case TVDCN_ACT_SILU: {
             const float s = quotient<PRECISE>(1.f, 1.f + exp32<PRECISE>(-z));
             return s * (1.f + z * (1.f - s));
@@ -138,7 +137,7 @@ template <bool PRECISE, int N> __device__ __forceinline__ void act_slopes(float 
     if (act == TVDCN_ACT_NONE) return;
     if (act == TVDCN_ACT_RELU) {
 #pragma unroll
-        for (int v = 0; v < N; ++v) d[v] *= act_slope<PRECISE>(z[v], TVDCN_ACT_RELU);
+        for (int v = 0; v < N; ++v) d[v] = z[v] <= 0.f ? 0.f : d[v];   // (also of a gradient that is not finite)
     } else if (act == TVDCN_ACT_SILU) {
 #pragma unroll
         for (int v = 0; v < N; ++v) d[v] *= act_slope<PRECISE>(z[v], TVDCN_ACT_SILU);

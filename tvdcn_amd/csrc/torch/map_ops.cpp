@@ -321,15 +321,16 @@ Tensor act_value(const Tensor &z, int64_t act) {
     if (act == TVDCN_ACT_GELU) return z * at::erfc(z * -M_SQRT1_2) * 0.5;
     return z;
 }
-Tensor act_slope(const Tensor &z, int64_t act) {
-    if (act == TVDCN_ACT_RELU) return (z > 0).to(z.scalar_type());
+// d act'(z); zero where a rectifier is shut, also of a gradient that is not finite
+Tensor act_slopes(const Tensor &d, const Tensor &z, int64_t act) {
+    if (act == TVDCN_ACT_RELU) return d.masked_fill(z <= 0, 0.0);
     if (act == TVDCN_ACT_SILU) {
         const Tensor s = at::sigmoid(z);
-        return s * (1 + z * (1 - s));
+        return d * (s * (1 + z * (1 - s)));
     }
     if (act == TVDCN_ACT_GELU)
-        return at::erfc(z * -M_SQRT1_2) * 0.5 + z * at::exp(z.square() * -0.5) * (0.5 * M_2_SQRTPI * M_SQRT1_2);
-    return at::ones_like(z);
+        return d * (at::erfc(z * -M_SQRT1_2) * 0.5 + z * at::exp(z.square() * -0.5) * (0.5 * M_2_SQRTPI * M_SQRT1_2));
+    return d;
 }
 
 struct NormRows {   // [batch, pixels, groups, channels per group] and parameters that broadcast over it
@@ -366,7 +367,7 @@ Three norm_backward_cpu(const Tensor &grad, MaybeTensor input, MaybeTensor codes
     const Tensor src = has(input) ? to_rows(*input) : expand_rows(*codes, *exponents, t).to(at::kFloat);
     const NormRows n = norm_rows(src, groups, weight, bias);
     const Tensor rs = stats[1].reshape({-1, 1, groups, 1}), h = (n.x - stats[0].reshape({-1, 1, groups, 1})) * rs;
-    const Tensor dz = rows.to(wide_type(grad)).reshape(n.x.sizes()) * act_slope(h * n.w + n.b, act), dn = dz * n.w;
+    const Tensor dz = act_slopes(rows.to(wide_type(grad)).reshape(n.x.sizes()), h * n.w + n.b, act), dn = dz * n.w;
     Tensor dx, dw, db;
     if (want[0]) dx = to_map((rs * (dn - dn.mean(at::IntArrayRef({1, 3}), true) - h * (dn * h).mean(at::IntArrayRef({1, 3}), true))).to(t).reshape(rows.sizes()));
     if (want[1]) dw = (dz * h).sum(at::IntArrayRef({0, 1})).reshape({C}).to(t);
@@ -477,7 +478,7 @@ Three point_backward_cpu(const Tensor &grad, MaybeTensor input, MaybeTensor code
     const auto t = wide_type(grad), out = grad.scalar_type();
     const int64_t N = weight.size(0), K = weight.size(1);
     Tensor dz = to_rows(grad).to(t).reshape({-1, N});
-    if (act != TVDCN_ACT_NONE) dz = dz * act_slope(to_rows(*pre).to(t).reshape({-1, N}), act);
+    if (act != TVDCN_ACT_NONE) dz = act_slopes(dz, to_rows(*pre).to(t).reshape({-1, N}), act);
     Tensor dx, dw, db;
     if (want[0]) dx = to_map(dz.mm(weight.to(t)).to(out).reshape(new_rows(grad, K, grad.options()).sizes()));
     if (want[1]) {
