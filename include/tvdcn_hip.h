@@ -260,8 +260,8 @@ tvdcn_status tvdcn_group_norm_act_backward(const tvdcn_norm_desc *desc, const vo
  * the activation is not TVDCN_ACT_NONE (TVDCN_ACT_RELU: a tensor that is positive where z is, as y
  * is without a residual) and the input as such or as its 8-bit map (input NULL, codes and exponents
  * not; kept_int8 = 1 in the workspace query). grad_input, grad_weight and grad_bias may be NULL
- * (not computed); the residual's gradient is grad_out itself. float32 products take three bfloat16
- * pieces per value: an infinite operand may give a NaN.
+ * (not computed); the residual's gradient is grad_out itself. Large float32 products (whole eights
+ * of channels) take three bfloat16 pieces per value: an infinite operand may give a NaN there.
  */
 typedef struct {
     int32_t dtype;       /* tvdcn_dtype */

@@ -8,15 +8,15 @@
 // the MFMA's row side: a lane then holds neighbouring output channels of one pixel and stores them together, with bias,
 // activation and residual applied on the way.
 //
-// Tiles of 64 along t are staged by direct-to-LDS loads, double-buffered: the next tile's loads are in flight while the
-// current one is multiplied. LDS chunks of 16 bytes are swizzled (on the global side of the load, since the LDS side is
+// Tiles of 64 along t are staged by direct-to-LDS loads into two or three buffers: the next tiles' loads are in flight while
+// the current one is multiplied. LDS chunks of 16 bytes are swizzled (on the global side of the load, since the LDS side is
 // fixed by the lane) so that the lanes of a read fall into different banks. Values beyond an operand's edge are read as
 // zeros by the buffer's own bounds check.
 //
-// float32 maps are multiplied on the float32 MFMAs as they lie, or, where the products are large, as three bfloat16 pieces per
-// value (exact) by the six products of pieces that reach float32's precision: 2^-24 relative to the operands' products, at a sixth
-// of the 16-bit rate (2.6 times the rate of the float32 MFMAs). An infinite operand may turn into a NaN there where float32 would
-// keep an infinity.
+// float32 maps are multiplied on the float32 MFMAs as they lie, or, where the products are large, as three bfloat16 pieces
+// per value (exact) by the six products of pieces that reach float32's precision: 2^-24 relative to the operands' products, at
+// a sixth of the 16-bit rate (2.6 times the rate of the float32 MFMAs). An infinite operand may turn into a NaN there where
+// float32 would keep an infinity.
 #include <algorithm>
 #include <atomic>
 #include <tuple>
@@ -36,6 +36,7 @@ typedef f16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int TB = 256;
 constexpr int SHARE = 64;   // rows of the weight gradient's shares come in multiples of this
+constexpr int BK = 64;      // of the reduction in a tile of product_kernel
 
 __device__ __forceinline__ fvec4 mfma(const bf16x8 &a, const bf16x8 &b, const fvec4 &c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -77,10 +78,10 @@ __device__ __forceinline__ void load_to_lds(const u32x4 &rsrc, uint32_t offset, 
 
 template <int N> constexpr int log2_of() { return N <= 1 ? 0 : 1 + log2_of<N / 2>(); }
 
-// Stages tiles of an operand: B rows (columns of the output, or rows) x BK. The NW waves issue B BK / 512 loads of 1 KB.
+// Stages tiles of an operand: B rows (columns of the output, or rows) x BK = 64. The NW waves issue B BK / 512 loads of 1 KB.
 //  t-contiguous: LDS row of BK elements per output index; chunk j of row n at j ^ swz(n)
 //  t-major:      LDS row of B elements per t; chunk j of row t at j ^ 2 swz(t)
-template <bool TM, bool PERM, int B, int F, int BK, int NW> struct Stager {
+template <bool TM, bool PERM, int B, int F, int NW> struct Stager {
     static constexpr int LOADS = B * BK / 512 / NW, CH = (TM ? B : BK) / 8;   // chunks of an LDS row
     static_assert(LOADS * 512 * NW == B * BK, "");
     uint32_t off[LOADS];
@@ -88,10 +89,9 @@ template <bool TM, bool PERM, int B, int F, int BK, int NW> struct Stager {
     int at[LOADS];           // first reduction index of the lane's chunk
 
     // Which chunk positions a row is turned by. t-contiguous: the 16 rows of one fragment read fall into different chunks
-    // of an LDS pass of 256 bytes (256 / (2 BK) rows); t-major: so do the eight rows of half a transposed read.
+    // of an LDS pass of 256 bytes (two rows); t-major: so do the eight rows of half a transposed read.
     static __device__ __forceinline__ int swz(int n) {
         if (TM) return (n & 3) | ((n >> 3) & 1) << 2;
-        if (BK == 32) return (PERM ? n >> log2_of<4 * F>() : n >> 2) & 3;
         if (PERM) return ((n >> 1) & 1) | ((n >> log2_of<4 * F>()) & 3) << 1;
         return (n >> 1) & 7;
     }
@@ -216,7 +216,7 @@ __device__ __forceinline__ void emit(const Product &p, int split, int row, int c
 }
 
 // WR x WC waves, each FR x FC fragments of 16 x 16; STAGES tiles of BK along the reduction in LDS
-template <typename T, bool RT, bool CT, int WR, int WC, int FR, int FC, int BK, int STAGES, int BLOCKS>
+template <typename T, bool RT, bool CT, int WR, int WC, int FR, int FC, int STAGES, int BLOCKS>
 __global__ void __launch_bounds__(WR * WC * 64, BLOCKS * WR * WC / 4) product_kernel(Product p) {
     constexpr int NW = WR * WC, BR = WR * 16 * FR, BC = WC * 16 * FC, TILE = (BR + BC) * BK * 2;
     extern __shared__ __align__(1024) char smem[];
@@ -232,8 +232,8 @@ __global__ void __launch_bounds__(WR * WC * 64, BLOCKS * WR * WC / 4) product_ke
     const int64_t kbeg = split * p.share, kend = kbeg + p.share < kall ? kbeg + p.share : kall;
     const int iters = (int)((kend - kbeg + BK - 1) / BK);
 
-    typedef Stager<RT, false, BR, FR, BK, NW> SR;
-    typedef Stager<CT, !CT, BC, FC, BK, NW> SC;
+    typedef Stager<RT, false, BR, FR, NW> SR;
+    typedef Stager<CT, !CT, BC, FC, NW> SC;
     constexpr int LOADS = SR::LOADS + SC::LOADS;
     SR sr;
     SC sc;
@@ -714,7 +714,7 @@ template <bool RT, bool CT, int PC> __global__ void __launch_bounds__(512, 2) pi
             d[l] = rows.descriptor(q + block / 3, block % 3 * plane_r);
             off[l] = RT || at_r[l] < rows.left() ? off_r[l] : 0x80000000u;
         }
-        to = lds + buf * STAGE + q * 12288 + wave * 3072;
+        to = lds + buf * STAGE + q * 12288 + wave * (3 * 1024);
     };
     auto aim_cols = [&]() {
 #pragma unroll
@@ -811,12 +811,13 @@ template <bool RT, bool CT, int PC> __global__ void __launch_bounds__(512, 2) pi
     }
 }
 
-// float32 as it lies, on the float32 MFMAs (16x16x4): no pieces, no copies of the operands, any pitch. Waves 2 x 2 of 2 x 2 fragments,
-// tiles of 64 x 64 (128 x 128 ones are 2% faster to 8% slower); a step is 16 along the reduction, staged through registers (16-byte loads where the rows allow them), double-
-// buffered in LDS. A lane's four values along the reduction serve four MFMAs: quarter q of a wave holds t = 4 q + m in MFMA m, of
-// both operands. t-contiguous tiles lie in rows of 16 (a wave reads 1 KB in a row), t-major ones in rows of B + 4, so that the four
-// quarters' rows, four apart, fall into different banks. Bound by the MFMAs (157 TFLOP/s)
-// and the steps' barriers: 87 TFLOP/s at 32768 x 256 from 256, 105 at 4096 x 2048 from 2048.
+// float32 as it lies, on the float32 MFMAs (16x16x4): no pieces, no copies of the operands, any pitch. Waves 2 x 2 of 2 x 2
+// fragments, tiles of 64 x 64 (128 x 128 ones are 2% faster to 8% slower); a step is 16 along the reduction, staged through
+// registers (16-byte loads where the rows allow them), double-buffered in LDS. A lane's four values along the reduction serve
+// four MFMAs: quarter q of a wave holds t = 4 q + m in MFMA m, of both operands. t-contiguous tiles lie in rows of 16 (a wave
+// reads 1 KB in a row), t-major ones in rows of B + 4, so that the four quarters' rows, four apart, fall into different banks.
+// Bound by the MFMAs (157 TFLOP/s) and the steps' barriers: 87 TFLOP/s at 32768 x 256 from 256 with silu and residual, 105 at
+// 4096 x 2048 from 2048.
 template <bool TM, int B> struct FloatStage {
     static constexpr int N = B / 64, LD = TM ? B + 4 : 16, BYTES = (TM ? 16 : B) * LD * 4;   // accesses of 16 bytes per thread
     fvec4 v[N];
@@ -1120,11 +1121,11 @@ unsigned strided_grid(int64_t lanes) {
     return (unsigned)(b < 16384 ? b : 16384);
 }
 
-template <typename T, bool RT, bool CT, int WR, int WC, int FR, int FC, int BK, int STAGES, int BLOCKS>
+template <typename T, bool RT, bool CT, int WR, int WC, int FR, int FC, int STAGES, int BLOCKS>
 hipError_t launch_tiles(Product &p, hipStream_t s) {
     constexpr int BR = WR * 16 * FR, BC = WC * 16 * FC, LDS = STAGES * (BR + BC) * BK * 2;
     static std::atomic<unsigned long long> done{0};
-    const auto kernel = product_kernel<T, RT, CT, WR, WC, FR, FC, BK, STAGES, BLOCKS>;
+    const auto kernel = product_kernel<T, RT, CT, WR, WC, FR, FC, STAGES, BLOCKS>;
     if (hipError_t e = raise_lds_limit((const void *)kernel, done)) return e;
     p.tiles_r = (int)ceil_div(p.rows, BR);
     p.tiles_c = (int)ceil_div(p.cols, BC);
@@ -1190,8 +1191,8 @@ template <typename T, bool RT, bool CT> hipError_t launch_product(Product p, Til
         switch (tiles) {
             case WIDE: return launch_wide<T, RT, CT, 4>(p, s);
             case HALF: return launch_wide<T, RT, CT, 2>(p, s);
-            case BIG: return launch_tiles<T, RT, CT, 2, 2, 4, 4, 64, 2, 2>(p, s);
-            default: return launch_tiles<T, RT, CT, 2, 2, 2, 2, 64, 3, 2>(p, s);
+            case BIG: return launch_tiles<T, RT, CT, 2, 2, 4, 4, 2, 2>(p, s);
+            default: return launch_tiles<T, RT, CT, 2, 2, 2, 2, 3, 2>(p, s);
         }
     }
 }

@@ -30,9 +30,10 @@ def pointwise_conv(input: Tensor, weight: Tensor, bias: Optional[Tensor] = None,
         keep_int8 (bool): the input is kept for the weight's gradient in 8 bits (see :func:`compress_activation`),
             which is taken with the values kept. The output and the other gradients do not change.
 
-    float16 and bfloat16 are multiplied as they are and summed in float32, float32 as three bfloat16 pieces per value
-    (an infinite value may give a NaN there); the result is rounded once. The backward reads the activation's argument,
-    kept in the input's type, and rounds its gradient to that type before the products. float64 runs on the CPU only.
+    Values are multiplied as they are and summed in float32 (large float32 products as three bfloat16 pieces per value,
+    to the same precision; an infinite value may give a NaN there); the result is rounded once. The backward reads the
+    activation's argument, kept in the input's type, and rounds its gradient to that type before the products. float64
+    runs on the CPU only.
 
     Returns:
         Tensor[batch, out_channels, \*size]: channels-last.
@@ -41,7 +42,7 @@ def pointwise_conv(input: Tensor, weight: Tensor, bias: Optional[Tensor] = None,
         _log_api_usage_once(pointwise_conv)
     _assert_has_ops()
     if weight.dim() > 2:
-        if weight[0, 0].numel() != 1:
+        if weight.numel() != weight.size(0) * weight.size(1):
             raise RuntimeError("pointwise_conv: expected a weight of shape (out_channels, in_channels) and axes of size "
                                "one, got {}".format(list(weight.shape)))
         weight = weight.flatten(1)
