@@ -47,20 +47,36 @@ Cut make_cut(int64_t batch, int64_t pixels, int channels, int vec) {
     return k;
 }
 
-// A lane's VEC channels of a pixel, from the map or its 8-bit form
+// A lane's VEC channels of a pixel, from the map or its 8-bit form: as they lie (so that several are on their way before the
+// first is looked at), and as values
 template <typename T, int VEC, bool KEPT> struct Source {
     const T *x;
     const int8_t *codes;
     const uint8_t *exps;
     int C, blocks;
-    __device__ __forceinline__ void get(int64_t row, int c, float *f) const {
+    struct Raw {
+        Pack<std::conditional_t<KEPT, int8_t, T>, VEC> p;
+        uint8_t e;
+    };
+    // where channel c of a row lies, and its exponent
+    __device__ __forceinline__ int64_t at(int64_t row, int c) const { return row * C + c; }
+    __device__ __forceinline__ int64_t block(int64_t row, int c) const { return KEPT ? row * blocks + c / kKeptBlock : 0; }
+    __device__ __forceinline__ Raw load(int64_t at, int64_t block) const {
+        Raw r;
         if constexpr (KEPT) {
-            const Pack<int8_t, VEC> q = *reinterpret_cast<const Pack<int8_t, VEC> *>(codes + row * C + c);
-            kept_values<T, VEC>(q.v, exps[row * blocks + c / kKeptBlock], f);
+            r.p = *reinterpret_cast<const decltype(r.p) *>(codes + at);
+            r.e = exps[block];
         } else {
-            const Pack<T, VEC> p = *reinterpret_cast<const Pack<T, VEC> *>(x + row * C + c);
+            r.p = *reinterpret_cast<const decltype(r.p) *>(x + at);
+        }
+        return r;
+    }
+    static __device__ __forceinline__ void values(const Raw &r, float *f) {
+        if constexpr (KEPT) {
+            kept_values<T, VEC>(r.p.v, r.e, f);
+        } else {
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) f[v] = (float)p.v[v];
+            for (int v = 0; v < VEC; ++v) f[v] = (float)r.p.v[v];
         }
     }
 };
@@ -75,6 +91,24 @@ template <typename T, int VEC> __device__ __forceinline__ void params(const void
 #pragma unroll
     for (int v = 0; v < VEC; ++v) f[v] = (float)p.v[v];
 }
+
+// The groups of VEC channels from c on
+template <int VEC> struct Groups {
+    int g[VEC];
+    __device__ __forceinline__ Groups(int c, int Cg) {
+        int group = c / Cg, left = (group + 1) * Cg - c;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            g[v] = group;
+            if (--left == 0) ++group, left = Cg;
+        }
+    }
+    // their values of one image
+    template <typename V> __device__ __forceinline__ void get(const V *__restrict__ from, V *to) const {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) to[v] = from[g[v]];
+    }
+};
 
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
@@ -116,6 +150,7 @@ __global__ void __launch_bounds__(TB) norm_stats_kernel(const T *__restrict__ x,
     const int t = threadIdx.x, col = t % k.cols, rl = t / k.cols, tile = blockIdx.y;
     const int c0 = (tile * k.cols + col) * VEC;
     const bool active = rl < k.lanes_r && c0 < C;
+    const Groups<VEC> of(active ? c0 : 0, Cg);
     for (int64_t unit = blockIdx.x; unit < k.units; unit += gridDim.x) {
         const int64_t b = unit / k.chunks, chunk = unit - b * k.chunks;
         const int64_t first = chunk * k.rows, last = first + k.rows < P ? first + k.rows : P;
@@ -124,7 +159,7 @@ __global__ void __launch_bounds__(TB) norm_stats_kernel(const T *__restrict__ x,
         for (int v = 0; v < VEC; ++v) s[v] = q[v] = shift[v] = 0.f;
         if (active) {
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) shift[v] = (float)x[b * P * C + (c0 + v) / Cg * Cg];
+            for (int v = 0; v < VEC; ++v) shift[v] = (float)x[b * P * C + of.g[v] * Cg];
             const T *xb = x + b * P * C + c0;
             for (int64_t r = first + rl; r < last; r += (int64_t)k.lanes_r * UNROLL) {
                 Pack<T, VEC> p[UNROLL];
@@ -200,16 +235,15 @@ __global__ void __launch_bounds__(TB) norm_apply_kernel(const T *__restrict__ x,
     float wv[VEC], bv[VEC];
     params<T, VEC>(w, c0, wv, 1.f);
     params<T, VEC>(bias, c0, bv, 0.f);
+    const Groups<VEC> of(c0, Cg);
     for (int64_t unit = blockIdx.x; unit < k.units; unit += gridDim.x) {
         const int64_t b = unit / k.chunks, chunk = unit - b * k.chunks;
         const int64_t first = chunk * k.rows, last = first + k.rows < P ? first + k.rows : P;
         float mu[VEC], sc[VEC];
+        of.get(mean + b * G, mu);
+        of.get(rstd + b * G, sc);
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            const int64_t i = b * G + (c0 + v) / Cg;
-            mu[v] = mean[i];
-            sc[v] = rstd[i] * wv[v];
-        }
+        for (int v = 0; v < VEC; ++v) sc[v] *= wv[v];
         const int64_t base = b * P * C + c0;
         for (int64_t r = first + rl; r < last; r += (int64_t)k.lanes_r * UNROLL) {
             Pack<T, VEC> p[UNROLL];
@@ -247,11 +281,13 @@ __global__ void __launch_bounds__(TB) norm_sums_kernel(Source<T, VEC, KEPT> src,
     const int t = threadIdx.x, col = t % k.cols, rl = t / k.cols, tile = blockIdx.y;
     const int c0 = (tile * k.cols + col) * VEC;
     const bool active = rl < k.lanes_r && c0 < C;
+    const int step = k.lanes_r * C, step_e = k.lanes_r * src.blocks;   // (under 2^21)
     float wv[VEC], bv[VEC];
     if (active) {
         params<T, VEC>(w, c0, wv, 1.f);
         params<T, VEC>(bias, c0, bv, 0.f);
     }
+    const Groups<VEC> of(active ? c0 : 0, Cg);
     for (int64_t unit = blockIdx.x; unit < k.units; unit += gridDim.x) {
         const int64_t b = unit / k.chunks, chunk = unit - b * k.chunks;
         const int64_t first = chunk * k.rows, last = first + k.rows < P ? first + k.rows : P;
@@ -259,38 +295,35 @@ __global__ void __launch_bounds__(TB) norm_sums_kernel(Source<T, VEC, KEPT> src,
 #pragma unroll
         for (int v = 0; v < VEC; ++v) s[v] = q[v] = 0.f;
         if (active) {
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                const int64_t i = b * G + (c0 + v) / Cg;
-                mu[v] = mean[i];
-                rs[v] = rstd[i];
-            }
-            const T *dyb = dy + b * P * C + c0;
-            for (int64_t r = first + rl; r < last; r += (int64_t)k.lanes_r * UNROLL) {
+            of.get(mean + b * G, mu);
+            of.get(rstd + b * G, rs);
+            int64_t at = src.at(b * P + first + rl, c0), block = src.block(b * P + first + rl, c0);
+            for (int64_t r = first + rl; r < last; r += (int64_t)k.lanes_r * UNROLL, at += UNROLL * step, block += UNROLL * step_e) {
                 Pack<T, VEC> d[UNROLL];
-                float f[UNROLL][VEC];
+                typename Source<T, VEC, KEPT>::Raw raw[UNROLL];
 #pragma unroll
-                for (int u = 0; u < UNROLL; ++u) {
-                    int64_t ru = r + (int64_t)u * k.lanes_r;
-                    ru = ru < last ? ru : first;
-                    d[u] = *reinterpret_cast<const Pack<T, VEC> *>(dyb + ru * C);
-                    src.get(b * P + ru, c0, f[u]);
+                for (int u = 0; u < UNROLL; ++u) {   // (past the chunk's end: the first of them again)
+                    const bool in = r + u * k.lanes_r < last;
+                    const int64_t at_u = at + (in ? u * step : 0);
+                    d[u] = *reinterpret_cast<const Pack<T, VEC> *>(dy + at_u);
+                    raw[u] = src.load(at_u, block + (in ? u * step_e : 0));
                 }
 #pragma unroll
                 for (int u = 0; u < UNROLL; ++u) {
-                    if (r + (int64_t)u * k.lanes_r >= last) break;
-                    float z[VEC], dz[VEC];
+                    if (r + u * k.lanes_r >= last) break;
+                    float f[VEC], z[VEC], dz[VEC];
+                    src.values(raw[u], f);
 #pragma unroll
                     for (int v = 0; v < VEC; ++v) {
-                        f[u][v] = (f[u][v] - mu[v]) * rs[v];
-                        z[v] = fmaf(f[u][v], wv[v], bv[v]);
+                        f[v] = (f[v] - mu[v]) * rs[v];
+                        z[v] = fmaf(f[v], wv[v], bv[v]);
                         dz[v] = (float)d[u].v[v];
                     }
                     act_slopes<is_f32<T>(), VEC>(dz, z, act);
 #pragma unroll
                     for (int v = 0; v < VEC; ++v) {
                         s[v] += dz[v];
-                        q[v] = fmaf(dz[v], f[u][v], q[v]);
+                        q[v] = fmaf(dz[v], f[v], q[v]);
                     }
                 }
             }
@@ -377,47 +410,45 @@ __global__ void __launch_bounds__(TB) norm_dx_kernel(Source<T, VEC, KEPT> src, c
     const int t = threadIdx.x, col = t % k.cols, rl = t / k.cols;
     const int c0 = (blockIdx.y * k.cols + col) * VEC;
     if (rl >= k.lanes_r || c0 >= C) return;
+    const int step = k.lanes_r * C, step_e = k.lanes_r * src.blocks;
     float wv[VEC], bv[VEC];
     params<T, VEC>(w, c0, wv, 1.f);
     params<T, VEC>(bias, c0, bv, 0.f);
+    const Groups<VEC> of(c0, Cg);
     for (int64_t unit = blockIdx.x; unit < k.units; unit += gridDim.x) {
         const int64_t b = unit / k.chunks, chunk = unit - b * k.chunks;
         const int64_t first = chunk * k.rows, last = first + k.rows < P ? first + k.rows : P;
-        float mu[VEC], rs[VEC], a1[VEC], a2[VEC];
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            const int64_t i = b * G + (c0 + v) / Cg;
-            mu[v] = mean[i];
-            rs[v] = rstd[i];
-            a1[v] = avg[i].x;
-            a2[v] = avg[i].y;
-        }
-        const int64_t base = b * P * C + c0;
-        for (int64_t r = first + rl; r < last; r += (int64_t)k.lanes_r * UNROLL) {
+        float mu[VEC], rs[VEC];
+        float2 av[VEC];
+        of.get(mean + b * G, mu);
+        of.get(rstd + b * G, rs);
+        of.get(avg + b * G, av);
+        int64_t at = src.at(b * P + first + rl, c0), block = src.block(b * P + first + rl, c0);
+        for (int64_t r = first + rl; r < last; r += (int64_t)k.lanes_r * UNROLL, at += UNROLL * step, block += UNROLL * step_e) {
             Pack<T, VEC> d[UNROLL];
-            float f[UNROLL][VEC];
+            typename Source<T, VEC, KEPT>::Raw raw[UNROLL];
 #pragma unroll
             for (int u = 0; u < UNROLL; ++u) {
-                int64_t ru = r + (int64_t)u * k.lanes_r;
-                ru = ru < last ? ru : first;
-                d[u] = *reinterpret_cast<const Pack<T, VEC> *>(dy + base + ru * C);
-                src.get(b * P + ru, c0, f[u]);
+                const bool in = r + u * k.lanes_r < last;
+                const int64_t at_u = at + (in ? u * step : 0);
+                d[u] = *reinterpret_cast<const Pack<T, VEC> *>(dy + at_u);
+                raw[u] = src.load(at_u, block + (in ? u * step_e : 0));
             }
 #pragma unroll
             for (int u = 0; u < UNROLL; ++u) {
-                const int64_t ru = r + (int64_t)u * k.lanes_r;
-                if (ru >= last) break;
-                float z[VEC], dz[VEC];
+                if (r + u * k.lanes_r >= last) break;
+                float f[VEC], z[VEC], dz[VEC];
+                src.values(raw[u], f);
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) {
-                    f[u][v] = (f[u][v] - mu[v]) * rs[v];
-                    z[v] = fmaf(f[u][v], wv[v], bv[v]);
+                    f[v] = (f[v] - mu[v]) * rs[v];
+                    z[v] = fmaf(f[v], wv[v], bv[v]);
                     dz[v] = (float)d[u].v[v];
                 }
                 act_slopes<is_f32<T>(), VEC>(dz, z, act);
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) d[u].v[v] = (T)(rs[v] * (dz[v] * wv[v] - a1[v] - f[u][v] * a2[v]));
-                *reinterpret_cast<Pack<T, VEC> *>(dx + base + ru * C) = d[u];
+                for (int v = 0; v < VEC; ++v) d[u].v[v] = (T)(rs[v] * (dz[v] * wv[v] - av[v].x - f[v] * av[v].y));
+                *reinterpret_cast<Pack<T, VEC> *>(dx + at + u * step) = d[u];
             }
         }
     }
@@ -543,23 +574,25 @@ __global__ void __launch_bounds__(block_of(TG))
     params<T, VEC>(bias, at.c0, bv, 0.f);
 #pragma unroll
     for (int v = 0; v < VEC; ++v) s[v] = q[v] = 0.f;
-    float f[NV][VEC], d[NV][VEC];   // x, then n; dy, then dz
+    float f[NV][VEC], d[NV][VEC];   // n, dz
+    typename Source<T, VEC, KEPT>::Raw raw[NV];
+    Pack<T, VEC> g[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int r = at.first + i * at.rows;
         if (r < P) {
-            src.get(at.b * P + r, at.c0, f[i]);
-            const Pack<T, VEC> g = *reinterpret_cast<const Pack<T, VEC> *>(dy + base + (int64_t)r * C);
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) d[i][v] = (float)g.v[v];
+            raw[i] = src.load(src.at(at.b * P + r, at.c0), src.block(at.b * P + r, at.c0));
+            g[i] = *reinterpret_cast<const Pack<T, VEC> *>(dy + base + (int64_t)r * C);
         }
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i)
         if (at.first + i * at.rows < P) {
             float z[VEC];
+            src.values(raw[i], f[i]);
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
+                d[i][v] = (float)g[i].v[v];
                 f[i][v] = (f[i][v] - mu) * rs;
                 z[v] = fmaf(f[i][v], wv[v], bv[v]);
             }

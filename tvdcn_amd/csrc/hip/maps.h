@@ -78,14 +78,19 @@ template <typename T, int N> struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N :
 
 // Activations. The argument is float32; ERF32: the error function to float32's last bits, otherwise to 1.5e-7
 // (Abramowitz and Stegun 7.1.26: erfc(u) = e^(-u^2) t (a1 + t (a2 + ...)), t = 1 / (1 + p u)), well under a half step
-// of the 16-bit types whose results it serves, at a third of the instructions.
+// of the 16-bit types whose results it serves, at a third of the instructions. (Here u = |z| / sqrt(2), and the result halved:
+// in the constants.)
 __device__ __forceinline__ float normal_cdf_poly(float z, float gauss) {   // gauss = e^(-z^2/2)
-    const float u = fabsf(z) * 0.70710678118654752f;
-    const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * u);
-    const float tail =
-        0.5f * gauss * t *
-        (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+    const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(z), 0.3275911f * 0.70710678118654752f, 1.f));
+    const float poly =
+        t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f), 0.5f * 1.421413741f), 0.5f * -0.284496736f),
+                 0.5f * 0.254829592f);
+    const float tail = gauss * poly;
     return z < 0.f ? tail : 1.f - tail;
+}
+// e^(-z^2/2)
+template <bool PRECISE> __device__ __forceinline__ float gauss_of(float z) {
+    return PRECISE ? expf(-0.5f * z * z) : __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);   // (log2(e) / 2)
 }
 template <bool ERF32> __device__ __forceinline__ float normal_cdf(float z, float gauss) {
     return ERF32 ? 0.5f * erfcf(-z * 0.70710678118654752f) : normal_cdf_poly(z, gauss);
@@ -100,7 +105,7 @@ template <bool PRECISE> __device__ __forceinline__ float act_value(float z, int 
     switch (act) {
         case TVDCN_ACT_RELU: return z < 0.f ? 0.f : z;   // (a NaN stays one)
         case TVDCN_ACT_SILU: return quotient<PRECISE>(z, 1.f + exp32<PRECISE>(-z));
-        case TVDCN_ACT_GELU: return z * normal_cdf<PRECISE>(z, exp32<PRECISE>(-0.5f * z * z));
+        case TVDCN_ACT_GELU: return z * normal_cdf<PRECISE>(z, gauss_of<PRECISE>(z));
         default: return z;
     }
 }
@@ -125,8 +130,8 @@ template <bool PRECISE> __device__ __forceinline__ float act_slope(float z, int 
             return s * (1.f + z * (1.f - s));
         }
         case TVDCN_ACT_GELU: {
-            const float gauss = exp32<PRECISE>(-0.5f * z * z);
-            return normal_cdf<PRECISE>(z, gauss) + z * gauss * 0.39894228040143268f;
+            const float gauss = gauss_of<PRECISE>(z);
+            return fmaf(z * gauss, 0.39894228040143268f, normal_cdf<PRECISE>(z, gauss));
         }
         default: return 1.f;
     }
