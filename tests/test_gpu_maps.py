@@ -135,6 +135,26 @@ def test_pointwise_kept_in_8_bits(shape, out, dtype):
             assert torch.equal(g, r)
 
 
+@pytest.mark.parametrize("rows,channels,out", [(32768, 256, 256), (32700, 260, 248), (32700, 248, 260), (65300, 100, 128)])
+def test_pointwise_float32_in_large_tiles(rows, channels, out):
+    """Rows, columns and reductions that end inside a tile or a stage, in one round of workgroups and more."""
+    f32 = torch.float32
+    x, w, b = make((rows, channels), f32, 1), make((out, channels), f32, 2, spread=channels ** -0.5), make((out,), f32, 3)
+    dy, r = make((rows, out), f32, 4), make((rows, out), f32, 5)
+    check(run_pointwise(x, w, b, r, "silu", dy), pointwise(x, w, b, r, "silu", dy))
+    check(run_pointwise(x, w, None, None, "none", dy), pointwise(x, w, None, None, "none", dy))
+
+
+@pytest.mark.parametrize("keep", [False, True])
+@pytest.mark.parametrize("rows,channels,out", [(20003, 1032, 1024), (17000, 2048, 513)])
+def test_pointwise_float32_in_pieces(rows, channels, out, keep):
+    """Products large enough for three bfloat16 pieces per value (one per value of an input kept in 8 bits)."""
+    f32 = torch.float32
+    x, w, b = make((rows, channels), f32, 1), make((out, channels), f32, 2, spread=channels ** -0.5), make((out,), f32, 3)
+    dy = make((rows, out), f32, 4)
+    check(run_pointwise(x, w, b, None, "gelu", dy, keep), pointwise(x, w, b, None, "gelu", dy, keep))
+
+
 def test_pointwise_float32_is_float32_accurate():
     """On the float32 MFMAs and in pieces: independent roundings leave about sqrt(K / 4) last bits, or sqrt(6 K / 32), 7e-7 at
     K = 600, and as many of the 128 rows and 100 shares that the weight's gradient adds up."""

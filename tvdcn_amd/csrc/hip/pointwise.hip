@@ -44,9 +44,15 @@ __device__ __forceinline__ fvec4 mfma(const bf16x8 &a, const bf16x8 &b, const fv
 __device__ __forceinline__ fvec4 mfma(const f16x8 &a, const f16x8 &b, const fvec4 &c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
+// MFMA m of a fragment: all of a 16-bit one, or of a float32 one the lanes' m-th values along t
+template <typename F> __device__ __forceinline__ fvec4 mfma_part(const F &a, const F &b, const fvec4 &c, int) { return mfma(a, b, c); }
+__device__ __forceinline__ fvec4 mfma_part(const fvec4 &a, const fvec4 &b, const fvec4 &c, int m) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(a[m], b[m], c, 0, 0, 0);
+}
 template <typename E> struct Frag;
 template <> struct Frag<bf16> { typedef bf16x8 type; };
 template <> struct Frag<f16> { typedef f16x8 type; };
+template <> struct Frag<float> { typedef fvec4 type; };   // along t
 
 // A matrix of 16-bit elements. t-contiguous: `width` rows of `lim` elements; t-major: `lim` rows of `width` elements.
 // Rows are `ld` apart, a multiple of 8; so are lim (t-contiguous) and width (t-major). Pieces are `plane` apart.
@@ -327,27 +333,42 @@ __global__ void __launch_bounds__(WR * WC * 64, BLOCKS * WR * WC / 4) product_ke
 //
 // Workgroups are persistent: a tile's stages follow the last one's, the first loads of the next tile are under way while the
 // results are stored.
-template <bool TM, bool PERM> struct SubTile {
+//
+// float32 on its own MFMAs (FC = 2) goes the same way in stages of 32, the same bytes: a lane's four values along the reduction
+// serve four MFMAs, quarter q of a wave holds t = 4 q + m in MFMA m, of both operands. 143 TFLOP/s along the reduction (the MFMAs'
+// own rate is 157); 32768 x 256 from 256 takes 49 us with launch, first loads and results, a plain library product 42.
+template <bool TM, bool PERM, int ES> struct SubTile {
     // the turn of an LDS row (128 bytes, 8 chunks): 16 rows of a fragment read, or the eight rows of half a transposed
-    // read, fall into different places of an LDS pass of 256 bytes
+    // read, fall into different places of an LDS pass of 256 bytes. float32, t-major: rows of 256 bytes, of which the four
+    // quarters of a wave read 64 bytes each of rows four apart
     static __device__ __forceinline__ int swz(int n) {
+        if (TM && ES == 4) return ((n >> 2) & 3) << 2;
         if (TM) return (((n >> 1) & 1) | ((n >> 3) & 1) << 1) << 1;
         if (PERM) return ((n >> 1) & 1) | ((n >> 3) & 3) << 1;
         return (n >> 1) & 7;
     }
     // the byte offset of a lane's 16 bytes from the sub-tile's first element; `at`: its first reduction index
     static __device__ __forceinline__ uint32_t offset(const Operand &o, int wave, int lane, int &at) {
-        const int row = wave * 8 + lane / 8, chunk = (lane & 7) ^ swz(row);
-        at = TM ? 0 : chunk * 8;
-        return (uint32_t)(row * (int)o.ld + chunk * 8) * 2u;
+        constexpr int CH = TM && ES == 4 ? 16 : 8, N = 16 / ES;   // chunks of an LDS row, elements of a chunk
+        const int row = wave * (64 / CH) + lane / CH, chunk = (lane & (CH - 1)) ^ swz(row);
+        at = TM ? 0 : chunk * N;
+        return (uint32_t)(row * (int)o.ld + chunk * N) * (uint32_t)ES;
     }
-    // 16 output indexes from `first`, reduction kk * 32 + (lane / 16) * 8 + 0..7. PERM: fragments 2i and 2i + 1 share 32, the
-    // MFMA's row r is (r / 4) 8 + r % 4 (+ 4): a lane then holds eight neighbouring indexes of theirs, four lanes 64 bytes of a
+    // 16 output indexes from `first`, reduction kk * 32 + (lane / 16) * 8 + 0..7 (float32: half of these). PERM: fragments 2i and
+    // 2i + 1 share 32, the MFMA's row r is (r / 4) 8 + r % 4 (+ 4): a lane then holds eight neighbouring indexes of theirs, four lanes 64 bytes of a
     // 16-bit row
     template <typename E>
     static __device__ __forceinline__ typename Frag<E>::type frag(const char *tile, int first, int kk, int lane) {
         const int q = lane >> 4, r = lane & 15;
-        if constexpr (TM) {
+        if constexpr (TM && ES == 4) {   // (t = kk * 16 + 4 q + 0..3)
+            fvec4 f;
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                const int t = kk * 16 + q * 4 + m, c = first + r;
+                f[m] = *reinterpret_cast<const float *>(tile + t * 256 + (((c >> 2) ^ swz(t)) << 4) + (c & 3) * 4);
+            }
+            return f;
+        } else if constexpr (TM) {
             union {
                 s16x4 h[2];
                 typename Frag<E>::type f;
@@ -462,7 +483,7 @@ template <int BC, int STEP = 64> struct WideTile {
 
 // Where a workgroup's loads of one operand are: the stage's base, and how many bytes from a sub-tile's first element on are
 // its own (rows, or columns of the last t, behind the edge are then read as zeros)
-template <bool TM, int B, int STEP = 64> struct WideSource {
+template <bool TM, int B, int STEP = 64, int ES = 2> struct WideSource {
     uint64_t base, step;     // of a stage; from sub-tile to sub-tile
     int inside;              // output indexes from the tile's first one on
     uint32_t rows;           // t-major: the bytes of the stage's t before the last one
@@ -475,24 +496,24 @@ template <bool TM, int B, int STEP = 64> struct WideSource {
         else off = lane_at < left() ? lane_off : 0x80000000u;
     }
     __device__ __forceinline__ void enter(const Operand &o, int first, int64_t k0, uint32_t lane_off, int lane_at) {
-        base = (uint64_t)o.p + 2 * (uint64_t)(TM ? k0 * o.ld + first : first * o.ld + k0);
+        base = (uint64_t)o.p + ES * (uint64_t)(TM ? k0 * o.ld + first : first * o.ld + k0);
         inside = __builtin_amdgcn_readfirstlane((int)(o.width - first < B ? o.width - first : B));
-        pitch = 2u * (uint32_t)o.ld;
-        step = TM ? 128 : 64 * (uint64_t)pitch;
+        pitch = (uint32_t)ES * (uint32_t)o.ld;
+        step = TM ? 64 * ES : 64 * (uint64_t)pitch;
         const int64_t t = o.lim - k0, n = (t + STEP - 1) / STEP;
         stages = __builtin_amdgcn_readfirstlane((int)(n < (1 << 30) ? n : 1 << 30));
         tail = (((int)t - 1) & (STEP - 1)) + 1;
         trim(lane_off, lane_at);
     }
     __device__ __forceinline__ void advance(uint32_t lane_off, int lane_at) {
-        base += TM ? STEP * (uint64_t)pitch : 2 * STEP;
+        base += TM ? STEP * (uint64_t)pitch : ES * STEP;
         --stages;
         trim(lane_off, lane_at);
     }
     __device__ __forceinline__ u32x4 descriptor(int q, uint64_t beyond = 0) const {
         const uint64_t b = base + q * step + beyond;
         const int n = min(max(inside - 64 * q, 0), 64);
-        const uint32_t bytes = TM ? (n ? rows + 2u * n : 0u) : (uint32_t)n * pitch;
+        const uint32_t bytes = TM ? (n ? rows + (uint32_t)ES * n : 0u) : (uint32_t)n * pitch;
         // (uniform, which the compiler does not always see)
         auto scalar = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
         return u32x4{scalar((uint32_t)b), scalar((uint32_t)(b >> 32)), scalar(bytes), 0x00020000u};
@@ -502,9 +523,11 @@ template <bool TM, int B, int STEP = 64> struct WideSource {
 template <typename T, bool RT, bool CT, int FC>
 __global__ void __launch_bounds__(512, 2) wide_product_kernel(Product p) {
     constexpr int BC = 64 * FC, COLS = 32768, STAGE = COLS + BC * 128;   // bytes; the columns' sub-tiles follow the rows'
+    constexpr int ES = sizeof(T), STEP = 128 / ES;                       // of the reduction in a stage
+    constexpr int PARTS = ES == 4 ? 4 : 1;                               // MFMAs of a fragment
     extern __shared__ __align__(1024) char smem[];
-    typedef SubTile<RT, false> SR;
-    typedef SubTile<CT, !CT> SC;
+    typedef SubTile<RT, false, ES> SR;
+    typedef SubTile<CT, !CT, ES> SC;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wr = wave >> 2, wc = wave & 3;
     const WideTiles tiles(p);
@@ -517,11 +540,11 @@ __global__ void __launch_bounds__(512, 2) wide_product_kernel(Product p) {
 
     // the stage to load next
     int tile_n = 0, step = 0, buf = 0;
-    WideTile<BC> ahead(p, tiles.first);
-    WideSource<RT, 256> rows;
-    WideSource<CT, BC> cols;
+    WideTile<BC, STEP> ahead(p, tiles.first);
+    WideSource<RT, 256, STEP, ES> rows;
+    WideSource<CT, BC, STEP, ES> cols;
     auto enter = [&]() {
-        const int64_t k0 = ahead.kbeg + (int64_t)step * 64;
+        const int64_t k0 = ahead.kbeg + (int64_t)step * STEP;
         rows.enter(p.R, ahead.row0, k0, off_r, at_r);
         cols.enter(p.C, ahead.col0, k0, off_c, at_c);
         if (tile_n >= tiles.count) rows.inside = cols.inside = 0;   // past the last tile: loads that fetch nothing
@@ -534,7 +557,7 @@ __global__ void __launch_bounds__(512, 2) wide_product_kernel(Product p) {
             return;
         }
         step = 0;
-        if (++tile_n < tiles.count) ahead = WideTile<BC>(p, tiles.first + tile_n * tiles.step);
+        if (++tile_n < tiles.count) ahead = WideTile<BC, STEP>(p, tiles.first + tile_n * tiles.step);
         enter();
     };
     // two sub-tiles' loads, their descriptors made ahead (beside the MFMAs)
@@ -558,7 +581,7 @@ __global__ void __launch_bounds__(512, 2) wide_product_kernel(Product p) {
 
     int at = 0;
     for (int n = 0; n < tiles.count; ++n) {
-        const WideTile<BC> tile(p, tiles.first + n * tiles.step);
+        const WideTile<BC, STEP> tile(p, tiles.first + n * tiles.step);
         fvec4 acc[FC][8];
 #pragma unroll
         for (int i = 0; i < FC; ++i)
@@ -593,15 +616,17 @@ __global__ void __launch_bounds__(512, 2) wide_product_kernel(Product p) {
 #pragma unroll
                 for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-                    for (int i = 0; i < FC; ++i)
+                    for (int m = 0; m < PARTS; ++m)
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) acc[i][ph * 2 + j] = mfma(a[kk][i], b[kk][j], acc[i][ph * 2 + j]);
+                        for (int i = 0; i < FC; ++i)
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) acc[i][ph * 2 + j] = mfma_part(a[kk][i], b[kk][j], acc[i][ph * 2 + j], m);
                 if constexpr (ph == 0) aim_cols(0);
                 if constexpr (ph == 1 && FC == 4) aim_cols(2);
                 if constexpr (ph == 2) aim_rows(0);
                 if constexpr (ph == 3) aim_rows(2);
 #pragma unroll
-                for (int m = 0; m < 4 * FC; ++m) {   // scalar work between the MFMAs
+                for (int m = 0; m < 4 * FC * PARTS; ++m) {   // scalar work between the MFMAs
                     __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
                     __builtin_amdgcn_sched_group_barrier(0x4, 3, 0);
                 }
@@ -1158,11 +1183,13 @@ template <bool RT, bool CT> hipError_t launch_float(Product &p, hipStream_t s) {
 }
 
 // Which tiles an output takes. 16 bits: 256 x 256 or 256 x 128 (of whole eights of columns), one workgroup per CU; 128 x 128 or 64 x
-// 64, two per CU. float32: in pieces, 256 x 128, or as it lies, 64 x 64. The least of what they take, in microseconds: launch,
-// first loads and results, and so much per step of 64 along the reduction and round of workgroups. Measured in bfloat16, 16 steps:
-// 2048 x 1024 takes 33.6 / 23.7 / 21.1 / 15.6 us in the four; 24 steps, 32768 x 256: 47.8 / 35.0 / 43.3 / 79.7; 32 steps, 65536 x
-// 512: 130 / 166 / 253 / -. float32, 4 steps, 32768 x 256: 33.7 / 49.3; 8192 x 256: 26.3 / 16.9; 32 steps, 4096 x 2048: 166 / 339.
-enum Tiles { WIDE, HALF, BIG, SMALL, PIECES, FLOAT };
+// 64, two per CU. float32: in pieces, 256 x 128, or as it lies, 64 x 64 or (rows of whole fours, whole eights of columns) 256 x 128.
+// The least of what they take, in microseconds: launch, first loads and results, and so much per step of 64 along the reduction and
+// round of workgroups. Measured in bfloat16, 16 steps: 2048 x 1024 takes 33.6 / 23.7 / 21.1 / 15.6 us in the four; 24 steps, 32768 x
+// 256: 47.8 / 35.0 / 43.3 / 79.7; 32 steps, 65536 x 512: 130 / 166 / 253 / -. float32, in pieces / 64 x 64 / 256 x 128: 4 steps, 32768
+// x 256: 33.7 / 60.7 / 49; 4 steps, 65536 x 256: - / 110 / 91; 2 steps, 32768 x 128: - / 20.9 / 28.4; 32 steps, 4096 x 2048: 166 /
+// 339 / -. (The weight gradient's shares gain nothing of the last: 57.9 us instead of 59.7 at 32768 rows of 256 and 256.)
+enum Tiles { WIDE, HALF, BIG, SMALL, PIECES, FLOAT, FLOAT_WIDE };
 double tiles_cost(Tiles t, int64_t rows, int64_t cols, int64_t splits, double steps) {
     auto count = [&](int64_t r, int64_t c) { return ceil_div(rows, r) * ceil_div(cols, c) * splits; };
     switch (t) {
@@ -1171,7 +1198,8 @@ double tiles_cost(Tiles t, int64_t rows, int64_t cols, int64_t splits, double st
         case BIG: return 6 + steps * (count(128, 128) <= 256 ? 0.95 : 1.7 * (double)ceil_div(count(128, 128), 512));
         case SMALL: return 4 + steps * (count(64, 64) <= 256 ? 0.55 : 0.75 * (double)ceil_div(count(64, 64), 512));
         case PIECES: return 10 + 5.2 * steps * (double)ceil_div(count(256, 128), 256);
-        default: return 6 + steps * std::max(2.2, 1.28 * (double)count(64, 64) / 256);
+        case FLOAT_WIDE: return 3 + (12 + 7.5 * steps) * (double)ceil_div(count(256, 128), 256);
+        default: return 6 + std::max(2.2 * steps, (1 + 1.28 * steps) * (double)count(64, 64) / 256);
     }
 }
 Tiles choose_tiles(int64_t rows, int64_t cols, double steps) {   // 16 bits
@@ -1181,11 +1209,18 @@ Tiles choose_tiles(int64_t rows, int64_t cols, double steps) {   // 16 bits
     return best;
 }
 
+Tiles choose_float(int64_t rows, int64_t cols, double steps, bool fours) {
+    return fours && cols % 8 == 0 && tiles_cost(FLOAT_WIDE, rows, cols, 1, steps) < tiles_cost(FLOAT, rows, cols, 1, steps) ? FLOAT_WIDE : FLOAT;
+}
+
 template <typename T, bool RT, bool CT> hipError_t launch_product(Product p, Tiles tiles, hipStream_t s) {
     if constexpr (is_f32<T>()) {
         if (tiles == FLOAT) return launch_float<RT, CT>(p, s);
-        if constexpr (RT)   // (the weight gradient, perhaps of a kept input)
+        if constexpr (!RT) {
+            if (tiles == FLOAT_WIDE) return launch_wide<float, RT, CT, 2>(p, s);
+        } else {   // (the weight gradient, perhaps of a kept input)
             if (p.pieces_c == 1) return launch_pieces<RT, CT, 1>(p, s);
+        }
         return launch_pieces<RT, CT, 3>(p, s);
     } else {
         switch (tiles) {
@@ -1211,7 +1246,11 @@ template <typename T, bool CT> hipError_t launch_rows(Product p, bool pieces, in
         p.out = out + first * p.cols;
         p.pre = pre ? pre + first * p.cols : nullptr;
         p.residual = res ? res + first * p.cols : nullptr;
-        const Tiles tiles = is_f32<T>() ? (pieces ? PIECES : FLOAT) : choose_tiles(p.rows, p.cols, (double)ceil_div(p.share, 64));
+        const double steps = (double)ceil_div(p.share, 64);
+        const bool fours = (p.R.ld | p.C.ld | p.R.lim | p.C.lim | p.C.width) % 4 == 0;
+        const Tiles tiles = !is_f32<T>() ? choose_tiles(p.rows, p.cols, steps)
+                            : pieces     ? PIECES
+                                         : choose_float(p.rows, p.cols, steps, fours);
         if (hipError_t e = launch_product<T, false, CT>(p, tiles, s)) return e;
     }
     return hipSuccess;
@@ -1223,15 +1262,17 @@ template <typename T, typename E, int NP> hipError_t lay_out(const LayOut &first
     return hipGetLastError();
 }
 
-// float32 in pieces or as it lies: the pieces' products run at about 190 TFLOP/s against 105, and cost the operands' copies
-// (10 bytes a value at 5 TB/s; in the backward dz in pieces too, 2 bytes a value more) and about 12 us of launches and first loads a
-// product. The pieces' kernel writes whole eights of columns.
+// float32 in pieces or as it lies: the pieces' products run at about 190 TFLOP/s against 128 (the weight gradient's, and all
+// where the 256 x 128 tiles do not serve: 105; 112 over both of a backward), and cost the operands' copies (10 bytes a value at
+// 5 TB/s; in the backward dz in pieces too, 2 bytes a value more) and launches and first loads. The pieces' kernel writes whole
+// eights of columns. 16384 x 512 to 512, in pieces / as it lies: forward 70 / 71 us, gradients of x 76 / 79, of W 88 / 105; 65536 x
+// 256 to 256: 91 as it lies, 103 / 86, 137 / 106 (each with the copies that the two share).
 bool forward_in_pieces(const PointwiseArgs &a) {
-    const double saved = 2.0 * a.rows * a.in * a.out * 4.26e-9;
-    return f32(a) && a.out % 8 == 0 && saved > 12 + a.rows * 2e-6 * a.in;
+    const double saved = 2.0 * a.rows * a.in * a.out * (a.in % 4 == 0 ? 2.55e-9 : 4.26e-9);
+    return f32(a) && a.out % 8 == 0 && saved > 5 + a.rows * 2e-6 * a.in;
 }
 bool backward_in_pieces(const PointwiseArgs &a) {
-    const double saved = 4.0 * a.rows * a.in * a.out * 4.26e-9;
+    const double saved = 4.0 * a.rows * a.in * a.out * (a.out % 4 == 0 ? 3.7e-9 : 4.26e-9);
     return f32(a) && a.in % 8 == 0 && saved > 24 + a.rows * (2e-6 * a.in + 0.4e-6 * a.out);
 }
 
