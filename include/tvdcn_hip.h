@@ -256,7 +256,8 @@ tvdcn_status tvdcn_group_norm_act_backward(const tvdcn_norm_desc *desc, const vo
 /*
  * The pointwise convolution: y = act(z) + residual, z = x weight^T + bias over the channels of
  * every row; weight (out_channels x in_channels), bias and residual (rows x out_channels) may be
- * NULL. pre (rows x out_channels, may be NULL) receives z. The backward takes z as pre wherever
+ * NULL. pre (rows x out_channels, may be NULL) receives z: in the map's type, but as float16 where a
+ * bfloat16 map has TVDCN_ACT_SILU or _GELU. The backward takes that as pre wherever
  * the activation is not TVDCN_ACT_NONE (TVDCN_ACT_RELU: a tensor that is positive where z is, as y
  * is without a residual) and the input as such or as its 8-bit map (input NULL, codes and exponents
  * not; kept_int8 = 1 in the workspace query). grad_input, grad_weight and grad_bias may be NULL

@@ -169,6 +169,19 @@ def test_pointwise_float32_is_float32_accurate():
     assert torch.equal(tvdcn.pointwise_conv(big, torch.eye(8, device="cuda")), big)
 
 
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("act", ["relu", "silu", "gelu"])
+def test_bfloat16_gradients_lose_two_roundings(act, residual):
+    """Two independent roundings of a step's size, of dz and of the result, leave sqrt(2) of one; the argument, kept with three
+    bits more, leaves 2^-6 of a third's square."""
+    x, w = make((4001, 136), torch.bfloat16, 1), make((520, 136), torch.bfloat16, 2, spread=136 ** -0.5)
+    dy, r = make((4001, 520), torch.bfloat16, 3), make((4001, 520), torch.bfloat16, 4) if residual else None
+    got = run_pointwise(x, w, None, r, act, dy)
+    for g, (want, _) in list(zip(got, pointwise(x, w, None, r, act, dy)))[1:]:
+        once = (want.bfloat16().double() - want).norm()
+        assert (g.double() - want).norm() < 1.45 * once
+
+
 @pytest.mark.parametrize("device", ["cpu", "cuda"])
 @pytest.mark.parametrize("act", ["silu", "gelu"])
 def test_float16_arguments_beyond_its_range(act, device):

@@ -158,13 +158,32 @@ template <> __device__ __forceinline__ float most<float>() { return 3.402823466e
 template <> __device__ __forceinline__ float most<f16>() { return 65504.f; }
 template <> __device__ __forceinline__ float most<bf16>() { return 3.389531390e38f; }
 
-// The activation's argument as it is kept for the backward: a finite one beyond float16 stays finite, at whose largest values the
-// slopes are what they are further out (0 or 1; at an infinity they would be NaN)
-template <typename T> __device__ __forceinline__ T kept_argument(float z) {
-    if constexpr (std::is_same<T, f16>::value) {
-        if (fabsf(z) < __builtin_inff()) z = fminf(fmaxf(z, -most<f16>()), most<f16>());
+// The activation's argument as it is kept for the backward: in the map's type, but for a silu or gelu of a bfloat16 map as float16
+// in the same 16 bits. Its slopes need the argument's last bits where it is of the order of 1, not its range: three bits more there
+// take the argument out of the gradients' error, which falls from 1.5 roundings of the map's type to 1.4. One beyond float16 is
+// read as its largest value, at which the slopes are what they are further out (0 or 1; at an infinity they would be NaN).
+template <typename T> struct Argument {   // silu and gelu
+    typedef T type;
+};
+template <> struct Argument<bf16> {
+    typedef f16 type;
+};
+template <typename T, int N> __device__ __forceinline__ void kept_arguments(const float *z, T *o, int act) {
+    if constexpr (is_f32<T>()) {
+#pragma unroll
+        for (int v = 0; v < N; ++v) o[v] = z[v];
+    } else if (std::is_same<T, bf16>::value && act != TVDCN_ACT_SILU && act != TVDCN_ACT_GELU) {
+#pragma unroll
+        for (int v = 0; v < N; ++v) o[v] = (T)z[v];
+    } else {
+#pragma unroll
+        for (int v = 0; v < N; ++v) o[v] = __builtin_bit_cast(T, (f16)z[v]);
     }
-    return (T)z;
+}
+template <typename Z, int N> __device__ __forceinline__ void argument_values(float *z) {
+    if constexpr (std::is_same<Z, f16>::value)
+#pragma unroll
+        for (int v = 0; v < N; ++v) z[v] = fabsf(z[v]) == __builtin_inff() ? copysignf(most<f16>(), z[v]) : z[v];
 }
 
 // What code q of exponent byte e stands for: q * 2^(e - bias) clamped to T's finite values, NaN for a block that held a value

@@ -190,8 +190,7 @@ __device__ __forceinline__ void emit(const Product &p, int split, int row, int c
         }
         P o;
         if (p.pre) {
-#pragma unroll
-            for (int v = 0; v < RUN; ++v) o.v[v] = kept_argument<T>(z[v]);
+            kept_arguments<T, RUN>(z, o.v, p.act);
             *reinterpret_cast<P *>((T *)p.pre + at) = o;
         }
 #pragma unroll
@@ -210,10 +209,13 @@ __device__ __forceinline__ void emit(const Product &p, int split, int row, int c
             for (int v = 0; v < RUN; ++v) r[v] = (float)((const T *)p.residual)[at + (v < last ? v : last)];
 #pragma unroll
         for (int v = 0; v < RUN; ++v) z[v] += acc[v];
-        if (p.pre)
+        if (p.pre) {
+            T o[RUN];
+            kept_arguments<T, RUN>(z, o, p.act);
 #pragma unroll
             for (int v = 0; v < RUN; ++v)
-                if (v <= last) ((T *)p.pre)[at + v] = kept_argument<T>(z[v]);
+                if (v <= last) ((T *)p.pre)[at + v] = o[v];
+        }
         act_values<is_f32<T>(), RUN>(z, p.act);
 #pragma unroll
         for (int v = 0; v < RUN; ++v)
@@ -436,8 +438,7 @@ __device__ __forceinline__ void store_results(const Product &p, const fvec4 (&ac
 #pragma unroll
                         for (int e = 0; e < RUN; ++e) v[e] += (float)bias[r].v[e];
                     if (p.pre) {
-#pragma unroll
-                        for (int e = 0; e < RUN; ++e) o.v[e] = kept_argument<T>(v[e]);
+                        kept_arguments<T, RUN>(v, o.v, p.act);
                         *reinterpret_cast<Run *>((T *)p.pre + at_o) = o;
                     }
                     act_values<is_f32<T>(), RUN>(v, p.act);
@@ -1039,8 +1040,8 @@ __global__ void __launch_bounds__(TB) lay_out_kernel(LayOut first, LayOut second
 
 // dz = dy act'(z) laid out as an operand (where dz is given), and its column sums over a chunk of rows. A workgroup has
 // `cols` lanes of 8 channels and TB / cols rows side by side.
-template <typename T, typename E, int NP, bool VEC>
-__global__ void __launch_bounds__(TB) slope_kernel(const T *__restrict__ dy, const T *__restrict__ pre, E *__restrict__ dz,
+template <typename T, typename Z, typename E, int NP, bool VEC>
+__global__ void __launch_bounds__(TB) slope_kernel(const T *__restrict__ dy, const Z *__restrict__ pre, E *__restrict__ dz,
                                                    float *__restrict__ part, int64_t rows, int C, int lanes_row, int cols,
                                                    int64_t chunk, int64_t plane, int act) {
     __shared__ float red[TB * 8];
@@ -1059,12 +1060,13 @@ __global__ void __launch_bounds__(TB) slope_kernel(const T *__restrict__ dy, con
             for (int u = 0; u < UNROLL; ++u) {
                 const int64_t ru = r0 + (int64_t)u * lanes_r, r = ru < last ? ru : first;
                 load8<T, VEC>(dy + r * C, c, C, d[u]);
-                if (act != TVDCN_ACT_NONE) load8<T, VEC>(pre + r * C, c, C, z[u]);
+                if (act != TVDCN_ACT_NONE) load8<Z, VEC>(pre + r * C, c, C, z[u]);
             }
 #pragma unroll
             for (int u = 0; u < UNROLL; ++u) {
                 const int64_t r = r0 + (int64_t)u * lanes_r;
                 if (r >= last) break;
+                argument_values<Z, 8>(z[u]);
                 act_slopes<is_f32<T>(), 8>(d[u], z[u], act);
 #pragma unroll
                 for (int v = 0; v < 8; ++v) s[v] += d[u][v];
@@ -1378,13 +1380,19 @@ template <typename T> hipError_t forward(const PointwiseArgs &a, hipStream_t s) 
     return launch_rows<T, false>(p, k.pieces, a.rows, s);
 }
 
-// dz as an operand (to == null: not needed so) and the bias gradient's chunks (part == null: not needed)
-template <typename T, typename E, int NP> hipError_t slopes(const PointwiseArgs &a, const Plan &k, void *to, float *part, hipStream_t s) {
+// dz as an operand (to == null: not needed so) and the bias gradient's chunks (part == null: not needed). Z: what pre holds.
+template <typename T, typename Z, typename E, int NP>
+hipError_t slopes_of(const PointwiseArgs &a, const Plan &k, void *to, float *part, hipStream_t s) {
     const int lanes = (int)ceil_div(a.out, 8);
-    const auto kernel = a.out % 8 == 0 ? slope_kernel<T, E, NP, true> : slope_kernel<T, E, NP, false>;
+    const auto kernel = a.out % 8 == 0 ? slope_kernel<T, Z, E, NP, true> : slope_kernel<T, Z, E, NP, false>;
     kernel<<<dim3(k.chunks, (unsigned)ceil_div(lanes, k.cols)), TB, 0, s>>>(
-        (const T *)a.dy, (const T *)a.pre, (E *)to, part, a.rows, a.out, lanes, k.cols, k.chunk, a.rows * k.po, a.act);
+        (const T *)a.dy, (const Z *)a.pre, (E *)to, part, a.rows, a.out, lanes, k.cols, k.chunk, a.rows * k.po, a.act);
     return hipGetLastError();
+}
+
+template <typename T, typename E, int NP> hipError_t slopes(const PointwiseArgs &a, const Plan &k, void *to, float *part, hipStream_t s) {
+    if (a.act == TVDCN_ACT_SILU || a.act == TVDCN_ACT_GELU) return slopes_of<T, typename Argument<T>::type, E, NP>(a, k, to, part, s);
+    return slopes_of<T, T, E, NP>(a, k, to, part, s);
 }
 
 template <typename T> hipError_t backward(const PointwiseArgs &a, hipStream_t s) {

@@ -394,6 +394,10 @@ void check_pointwise(const Tensor &x, const Tensor &weight, MaybeTensor bias, Ma
     check_like(x, bias, "bias", {weight.size(0)}, POINT);
     check_like(x, residual, "residual", map_shape(x, weight.size(0)), POINT);
 }
+// What the activation's argument is kept in: the map's type, but float16 for a silu or gelu of a bfloat16 map
+at::ScalarType argument_type(const Tensor &x, int64_t act) {
+    return x.scalar_type() == at::kBFloat16 && (act == TVDCN_ACT_SILU || act == TVDCN_ACT_GELU) ? at::kHalf : x.scalar_type();
+}
 void check_pointwise_backward(const Tensor &grad, MaybeTensor input, MaybeTensor codes, MaybeTensor exponents,
                               const Tensor &weight, MaybeTensor pre, int64_t activation) {
     check_map(grad, POINT);
@@ -401,7 +405,10 @@ void check_pointwise_backward(const Tensor &grad, MaybeTensor input, MaybeTensor
     check_activation(activation, POINT);
     check_source(grad, input, codes, exponents, weight.size(1), POINT);
     TORCH_CHECK(activation == TVDCN_ACT_NONE || has(pre), POINT, " backward: the activation's argument is missing");
-    check_like(grad, pre, "pre", grad.sizes(), POINT);
+    if (activation != TVDCN_ACT_NONE)
+        TORCH_CHECK(pre->sizes() == grad.sizes() && pre->scalar_type() == argument_type(grad, activation) &&
+                        pre->device() == grad.device(),
+                    POINT, " backward: the activation's argument is not that of the forward");
 }
 
 Two point_forward_hip(const Tensor &x, const Tensor &weight, MaybeTensor bias, MaybeTensor residual, int64_t act,
@@ -412,7 +419,7 @@ Two point_forward_hip(const Tensor &x, const Tensor &weight, MaybeTensor bias, M
     const int64_t N = weight.size(0);
     const tvdcn_pointwise_desc d{map_dtype(x.scalar_type(), POINT), (int32_t)act, x.size(0) * pixels_of(x), x.size(1), N};
     Tensor y = new_map(map_shape(x, N), x.options());
-    Tensor pre = save_pre ? new_map(y.sizes(), x.options()) : Tensor();
+    Tensor pre = save_pre ? new_map(y.sizes(), x.options().dtype(argument_type(x, act))) : Tensor();
     const size_t n = tvdcn_pointwise_conv_forward_workspace_size(&d);
     const Tensor work = n ? bytes(x, n) : Tensor();
     check_status(tvdcn_pointwise_conv_forward(&d, ptr(r), ptr(w), ptr(b), ptr(res), ptr(y), ptr(pre),
@@ -444,7 +451,7 @@ Two point_forward_meta(const Tensor &x, const Tensor &weight, MaybeTensor bias, 
                        bool save_pre) {
     check_pointwise(x, weight, bias, residual, act);
     const auto shape = map_shape(x, weight.size(0));
-    return {new_map(shape, x.options()), save_pre ? new_map(shape, x.options()) : Tensor()};
+    return {new_map(shape, x.options()), save_pre ? new_map(shape, x.options().dtype(argument_type(x, act))) : Tensor()};
 }
 Three point_backward_meta(const Tensor &grad, MaybeTensor input, MaybeTensor codes, MaybeTensor exponents,
                           const Tensor &weight, MaybeTensor pre, int64_t act, std::array<bool, 3> want) {
@@ -454,9 +461,9 @@ Three point_backward_meta(const Tensor &grad, MaybeTensor input, MaybeTensor cod
             want[2] ? at::empty({weight.size(0)}, o) : Tensor()};
 }
 
-// the activation's argument in the map's type; a finite one beyond float16 stays finite
-Tensor kept_argument(const Tensor &z, at::ScalarType t) {
-    return t == at::kHalf ? at::where(z.isfinite(), z.clamp(-65504.0, 65504.0), z).to(t) : z.to(t);
+// the activation's argument from what is kept: one beyond float16 is its largest value
+Tensor argument(const Tensor &pre, at::ScalarType t) {
+    return pre.scalar_type() == at::kHalf ? pre.to(t).clamp(-65504.0, 65504.0) : pre.to(t);
 }
 
 Two point_forward_cpu(const Tensor &x, const Tensor &weight, MaybeTensor bias, MaybeTensor residual, int64_t act,
@@ -470,7 +477,7 @@ Two point_forward_cpu(const Tensor &x, const Tensor &weight, MaybeTensor bias, M
     Tensor v = act_value(z, act);
     if (has(residual)) v = v + to_rows(*residual).to(t).reshape(v.sizes());
     return {to_map(v.to(x.scalar_type()).reshape(y.sizes())),
-            save_pre ? to_map(kept_argument(z, x.scalar_type()).reshape(y.sizes())) : Tensor()};
+            save_pre ? to_map(z.to(argument_type(x, act)).reshape(y.sizes())) : Tensor()};
 }
 Three point_backward_cpu(const Tensor &grad, MaybeTensor input, MaybeTensor codes, MaybeTensor exponents, const Tensor &weight,
                          MaybeTensor pre, int64_t act, std::array<bool, 3> want) {
@@ -478,7 +485,7 @@ Three point_backward_cpu(const Tensor &grad, MaybeTensor input, MaybeTensor code
     const auto t = wide_type(grad), out = grad.scalar_type();
     const int64_t N = weight.size(0), K = weight.size(1);
     Tensor dz = to_rows(grad).to(t).reshape({-1, N});
-    if (act != TVDCN_ACT_NONE) dz = act_slopes(dz, to_rows(*pre).to(t).reshape({-1, N}), act);
+    if (act != TVDCN_ACT_NONE) dz = act_slopes(dz, argument(to_rows(*pre), t).reshape({-1, N}), act);
     Tensor dx, dw, db;
     if (want[0]) dx = to_map(dz.mm(weight.to(t)).to(out).reshape(new_rows(grad, K, grad.options()).sizes()));
     if (want[1]) {

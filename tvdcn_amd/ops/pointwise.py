@@ -32,8 +32,8 @@ def pointwise_conv(input: Tensor, weight: Tensor, bias: Optional[Tensor] = None,
 
     Values are multiplied as they are and summed in float32 (large float32 products as three bfloat16 pieces per value,
     to the same precision; an infinite value may give a NaN there); the result is rounded once. The backward reads the
-    activation's argument, kept in the input's type, and rounds its gradient to that type before the products. float64
-    runs on the CPU only.
+    activation's argument, kept in the input's type (float16 for "silu" and "gelu" of bfloat16), and rounds its gradient
+    to the input's type before the products. float64 runs on the CPU only.
 
     Returns:
         Tensor[batch, out_channels, \*size]: channels-last.
