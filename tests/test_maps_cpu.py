@@ -154,6 +154,29 @@ def test_double_backward_is_refused():
             g.sum().backward()
 
 
+@pytest.mark.parametrize("grad_mode", [True, False])
+def test_forward_mode_derivatives_are_refused(grad_mode):
+    """A tangent of any input, with gradients recorded or not, through torch.func, and of the gradient in a backward."""
+    ad = torch.autograd.forward_ad
+    x, p, r = torch.randn(2, 6, 3), torch.randn(6), torch.randn(2, 4, 3)
+    w, b = torch.randn(4, 6), torch.randn(4)
+    match = "forward-mode derivatives .* not supported"
+    for f, args in ((lambda *a: tvdcn.group_norm_act(a[0], 2, *a[1:], activation="silu"), (x, p, p)),
+                    (lambda *a: tvdcn.pointwise_conv(*a, activation="gelu"), (x, w, b, r))):
+        for i, t in enumerate(args):
+            with ad.dual_level(), torch.set_grad_enabled(grad_mode):
+                dual = ad.make_dual(t, torch.ones_like(t))
+                with pytest.raises(RuntimeError, match=match):
+                    f(*args[:i], dual, *args[i + 1:])
+            with pytest.raises(RuntimeError, match=match), torch.set_grad_enabled(grad_mode):
+                torch.func.jvp(lambda v: f(*args[:i], v, *args[i + 1:]), (t,), (torch.ones_like(t),))
+        first = leaf(args[0])
+        y = f(first, *args[1:])
+        with ad.dual_level(), pytest.raises(RuntimeError, match=match):
+            torch.autograd.grad(y, first, ad.make_dual(torch.ones_like(y), torch.ones_like(y)))
+        assert f(*args).shape == y.shape
+
+
 def test_input_changed_before_the_backward_is_noticed():
     x, w = torch.randn(2, 6, 3), torch.randn(4, 6, requires_grad=True)
     y = tvdcn.pointwise_conv(x, w)

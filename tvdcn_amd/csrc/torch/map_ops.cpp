@@ -537,6 +537,12 @@ bool wanted(AutogradContext *ctx, const char *edge) {
     return i >= 0 && ctx->needs_input_grad(i);
 }
 
+// Forward-mode derivatives have no formula here: a tangent that an input brings is refused, not dropped
+void check_no_tangents(const char *name, std::initializer_list<Tensor> ts) {
+    for (const Tensor &t : ts)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), name, ": forward-mode derivatives (jvp) are not supported");
+}
+
 bool needs(const Tensor &t) { return t.defined() && t.requires_grad(); }
 bool needs(MaybeTensor t) { return has(t) && t->requires_grad(); }
 
@@ -580,6 +586,7 @@ class NormFunction : public torch::autograd::Function<NormFunction> {
         return std::get<0>(r);
     }
     static variable_list backward(AutogradContext *ctx, const variable_list &g) {
+        check_no_tangents(NORM, {g[0]});
         const auto s = ctx->get_saved_variables();
         const std::array<bool, 3> want{ctx->needs_input_grad(0), wanted(ctx, "weight"), wanted(ctx, "bias")};
         Three r;
@@ -615,6 +622,7 @@ class PointFunction : public torch::autograd::Function<PointFunction> {
         return y;
     }
     static variable_list backward(AutogradContext *ctx, const variable_list &g) {
+        check_no_tangents(POINT, {g[0]});
         const auto s = ctx->get_saved_variables();
         const std::array<bool, 3> want{ctx->needs_input_grad(0), ctx->needs_input_grad(1), wanted(ctx, "bias")};
         Three r;
@@ -637,6 +645,7 @@ bool any_grad(std::initializer_list<Tensor> ts) {
 
 Tensor norm_autograd(const Tensor &x, int64_t groups, MaybeTensor weight, MaybeTensor bias, double eps, int64_t act,
                      bool keep_int8) {
+    check_no_tangents(NORM, {x, get(weight), get(bias)});
     if (any_grad({x, get(weight), get(bias)})) {
         if (keep_int8)
             TORCH_CHECK(x.scalar_type() != at::kDouble, NORM, ": 8-bit maps of float64 are not supported");
@@ -650,6 +659,7 @@ Tensor norm_direct(const Tensor &x, int64_t groups, MaybeTensor weight, MaybeTen
 }
 Tensor point_autograd(const Tensor &x, const Tensor &weight, MaybeTensor bias, MaybeTensor residual, int64_t act,
                       bool keep_int8) {
+    check_no_tangents(POINT, {x, weight, get(bias), get(residual)});
     if (any_grad({x, weight, get(bias), get(residual)})) {
         if (keep_int8)
             TORCH_CHECK(x.scalar_type() != at::kDouble, POINT, ": 8-bit maps of float64 are not supported");
