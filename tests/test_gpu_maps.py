@@ -76,6 +76,33 @@ def test_norm_of_large_means_and_constant_groups(dtype):
     assert torch.equal(y, b.view(1, -1, 1, 1).expand_as(y))
 
 
+# groups that no workgroup holds: their statistics come from sums of many workgroups (channels in whole accesses, one by one, and
+# accesses that span groups)
+LARGE_GROUPS = [((2, 16, 150, 140), 2), ((1, 33, 70, 80), 3), ((1, 72, 9001), 6)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape,groups", LARGE_GROUPS)
+def test_norm_of_large_groups_with_unlike_first_values(shape, groups, dtype):
+    """The first value of every group, or its whole first pixel, far from the others, as a padded corner's is: the statistics keep
+    the bits that they have without it. (Largest values that float16 holds; outliers of 300 and more spreads.)"""
+    x, w, b, dy = norm_case(shape, dtype)
+    flat = x.movedim(1, -1).view(shape[0], -1, shape[1])   # (the same memory)
+    for shift, first, step in ((0.0, 300.0, 1), (0.0, 10000.0, shape[1] // groups), (1000.0, 0.0, 1), (40.0, -60000.0, 1)):
+        flat.copy_(norm_case(shape, dtype)[0].movedim(1, -1).view_as(flat).float().add_(shift))
+        flat[:, 0, ::step] = first
+        check(run_norm(x, groups, w, b, "none", dy), norm(x, groups, w, b, 1e-5, "none", dy), (shape, shift, first))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape,groups", LARGE_GROUPS)
+def test_norm_of_large_groups_with_large_means_or_constant(shape, groups, dtype):
+    x, w, b, dy = norm_case(shape, dtype, shift=40.0)
+    check(run_norm(x, groups, w, b, "silu", dy), norm(x, groups, w, b, 1e-5, "silu", dy), shape)
+    y = tvdcn.group_norm_act(torch.full_like(x, 3.3), groups, w, b)
+    assert torch.equal(y, b.view(-1, *[1] * (len(shape) - 2)).expand_as(y))
+
+
 def test_norm_values_that_are_not_finite_stay_in_their_group():
     x, w, b, dy = norm_case((2, 32, 9, 9), torch.float32)
     ref = tvdcn.group_norm_act(x, 4, w, b, 1e-5, "silu")

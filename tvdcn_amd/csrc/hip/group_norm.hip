@@ -7,8 +7,8 @@
 // statistics read x once, the second pass reads it again (from the 256 MB last-level cache where it fits) and writes y. A
 // workgroup takes a run of pixels of one image and all channels (in tiles of 256
 // lanes), so every access is a run of whole rows; a lane keeps its 16 bytes of channels over all its pixels, and with
-// them the parameters of those channels. Sums are float32, of deviations from the group's first value (large means
-// against small spreads do not cancel), combined in a fixed order.
+// them the parameters of those channels. Sums are float32, those of the statistics of deviations from running means (large means
+// against small spreads do not cancel, nor does a value unlike the rest), joined in a fixed order.
 
 #include "maps.h"
 
@@ -142,83 +142,122 @@ template <int VEC> __device__ __forceinline__ void sum_pixel_lanes(float2 *red, 
     __syncthreads();
 }
 
-// part[(unit * tiles + tile) * G + g] = the tile's sums of x - shift and its square, shift = the group's first value
+// part[(unit * tiles + tile) * G + g] = the mean of the tile's values of the group, and their squared deviations from it
+//
+// A lane carries a channel's mean m and sum of squared deviations M over its n pixels so far, and takes UNROLL more at a time:
+// with s and q the sums of d = x - m and of d^2 over the k new ones, m' = m + s / (n + k), M' = M + q - s^2 / (n + k). What is
+// subtracted is at most k / (n + k) of q, so nothing cancels, whatever the first values are (m starts as the first, and a value
+// unlike the rest costs no more bits than it adds to the spread). Means are then joined over lanes and channels, and M by their
+// deviations from the joint one: M = sum M_i + n_i (m_i - m)^2.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(TB) norm_stats_kernel(const T *__restrict__ x, float2 *__restrict__ part, int64_t P,
                                                         int C, int G, int Cg, Cut k) {
     __shared__ float2 red[TB * VEC];
-    const int t = threadIdx.x, col = t % k.cols, rl = t / k.cols, tile = blockIdx.y;
+    const int t = threadIdx.x, col = t % k.cols, rl = t / k.cols, tile = blockIdx.y, n = k.cols * VEC;
     const int c0 = (tile * k.cols + col) * VEC;
     const bool active = rl < k.lanes_r && c0 < C;
-    const Groups<VEC> of(active ? c0 : 0, Cg);
+    const int base = tile * n, end = min(base + n, C), g0 = base / Cg, g1 = (end - 1) / Cg;
+    int per = 64;
+    while (per > 1 && (g1 - g0 + 1) * per > TB) per /= 2;
     for (int64_t unit = blockIdx.x; unit < k.units; unit += gridDim.x) {
         const int64_t b = unit / k.chunks, chunk = unit - b * k.chunks;
         const int64_t first = chunk * k.rows, last = first + k.rows < P ? first + k.rows : P;
-        float s[VEC], q[VEC], shift[VEC];
+        float mean[VEC], sq[VEC], count = 0.f;
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) s[v] = q[v] = shift[v] = 0.f;
+        for (int v = 0; v < VEC; ++v) mean[v] = sq[v] = 0.f;
         if (active) {
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) shift[v] = (float)x[b * P * C + of.g[v] * Cg];
             const T *xb = x + b * P * C + c0;
+            const Pack<T, VEC> p0 = *reinterpret_cast<const Pack<T, VEC> *>(xb + (first + rl < last ? first + rl : first) * C);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) mean[v] = (float)p0.v[v];
             for (int64_t r = first + rl; r < last; r += (int64_t)k.lanes_r * UNROLL) {
                 Pack<T, VEC> p[UNROLL];
+                float s[VEC], q[VEC];
 #pragma unroll
                 for (int u = 0; u < UNROLL; ++u) {
                     const int64_t ru = r + (int64_t)u * k.lanes_r;
                     p[u] = *reinterpret_cast<const Pack<T, VEC> *>(xb + (ru < last ? ru : first) * C);
                 }
 #pragma unroll
+                for (int v = 0; v < VEC; ++v) s[v] = q[v] = 0.f;
+#pragma unroll
                 for (int u = 0; u < UNROLL; ++u) {
                     if (r + (int64_t)u * k.lanes_r >= last) break;
+                    count += 1.f;
 #pragma unroll
                     for (int v = 0; v < VEC; ++v) {
-                        const float d = (float)p[u].v[v] - shift[v];
+                        const float d = (float)p[u].v[v] - mean[v];
                         s[v] += d;
                         q[v] = fmaf(d, d, q[v]);
                     }
                 }
+                const float inv = __builtin_amdgcn_rcpf(count);   // (a last bit off moves m by as much of its step)
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) {
+                    const float step = s[v] * inv;
+                    mean[v] += step;
+                    sq[v] += fmaf(-s[v], step, q[v]);
+                }
             }
         }
-        sum_pixel_lanes<VEC>(red, s, q, t, k, active);
-        // a wave per group of the tile
-        const int base = tile * k.cols * VEC, end = min(base + k.cols * VEC, C);
-        for (int g = base / Cg + t / 64; g <= (end - 1) / Cg; g += TB / 64) {
-            const int lo = max(g * Cg, base), hi = min((g + 1) * Cg, end);
-            float a = 0.f, c = 0.f;
-            for (int i = lo + (t & 63); i < hi; i += 64) {
-                a += red[i - base].x;
-                c += red[i - base].y;
-            }
-            a = wave_sum(a);
-            c = wave_sum(c);
-            if ((t & 63) == 0) part[(unit * k.tiles + tile) * G + g] = make_float2(a, c);
+        if (rl < k.lanes_r)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) red[rl * n + col * VEC + v] = make_float2(mean[v], sq[v]);
+        __syncthreads();
+        // over a group's channels and pixel lanes (lane r holds pixels r, r + lanes_r, ... of the chunk): `per` lanes to a group, a
+        // wave at most, so that a workgroup's groups are summed side by side
+        const int64_t rows = last - first, whole = rows / k.lanes_r;
+        const int more = (int)(rows - whole * k.lanes_r), lanes = whole ? k.lanes_r : more;
+        for (int g = g0 + t / per; g <= g1; g += TB / per) {
+            const int lo = max(g * Cg, base) - base, w = min((g + 1) * Cg, end) - base - lo, l = t % per, dr = per / w;
+            const int di = per - dr * w;
+            auto each = [&](auto f) {
+                for (int r = l / w, i = l - r * w; r < lanes;) {
+                    f((float)(whole + (r < more)), red[r * n + lo + i]);
+                    r += dr, i += di;
+                    if (i >= w) i -= w, ++r;
+                }
+            };
+            auto sum = [&](float v) {
+                for (int m = 1; m < per; m <<= 1) v += __shfl_xor(v, m);
+                return v;
+            };
+            const float m0 = red[lo].x;
+            float m = 0.f, a = 0.f;
+            each([&](float count, const float2 &v) { m = fmaf(count, v.x - m0, m); });
+            m = m0 + sum(m) / ((float)rows * (float)w);
+            each([&](float count, const float2 &v) { a += fmaf(count, (v.x - m) * (v.x - m), v.y); });
+            a = sum(a);
+            if (l == 0) part[(unit * k.tiles + tile) * G + g] = make_float2(m, a);
         }
         __syncthreads();
     }
 }
 
-// mean and rstd of a (batch, group) from its chunks' sums: a wave each
-template <typename T>
-__global__ void __launch_bounds__(64) norm_finish_kernel(const T *__restrict__ x, const float2 *__restrict__ part,
-                                                         float *__restrict__ mean, float *__restrict__ rstd, int64_t BG,
-                                                         int64_t P, int C, int G, int Cg, int tile_c, float eps, Cut k) {
+// mean and rstd of a (batch, group) from its chunks' and tiles': a wave each
+__global__ void __launch_bounds__(64) norm_finish_kernel(const float2 *__restrict__ part, float *__restrict__ mean,
+                                                         float *__restrict__ rstd, int64_t BG, int64_t P, int G, int Cg,
+                                                         int tile_c, float eps, Cut k) {
     for (int64_t i = blockIdx.x; i < BG; i += gridDim.x) {
         const int64_t b = i / G;
         const int g = (int)(i - b * G);
         const int t0 = g * Cg / tile_c, nt = ((g + 1) * Cg - 1) / tile_c - t0 + 1;
+        const double m0 = part[(b * k.chunks * k.tiles + t0) * G + g].x;
         double s = 0.0, q = 0.0;
         for (int j = threadIdx.x; j < k.chunks * nt; j += 64) {
-            const float2 v = part[((b * k.chunks + j / nt) * k.tiles + t0 + j % nt) * G + g];
-            s += v.x;
-            q += v.y;
+            const int chunk = j / nt, tile = t0 + j % nt;
+            const float2 v = part[((b * k.chunks + chunk) * k.tiles + tile) * G + g];
+            const int64_t first = chunk * k.rows, rows = P - first < k.rows ? P - first : k.rows;
+            const double n = (double)rows * (min((g + 1) * Cg, (tile + 1) * tile_c) - max(g * Cg, tile * tile_c)), d = v.x - m0;
+            s += n * d;
+            q += v.y + n * d * d;
         }
         s = wave_sum(s);
         q = wave_sum(q);
         if (threadIdx.x == 0) {
             const double n = (double)P * Cg, m = s / n;
             const double var = q / n - m * m;
-            mean[i] = (float)((double)(float)x[b * P * C + (int64_t)g * Cg] + m);
+            mean[i] = (float)(m0 + m);
             rstd[i] = (float)(1.0 / sqrt((var > 0.0 || var != var ? var : 0.0) + (double)eps));
         }
     }
@@ -731,8 +770,8 @@ template <typename T, int VEC> hipError_t forward(const NormArgs &a, hipStream_t
     const T *x = (const T *)a.x;
     norm_stats_kernel<T, VEC><<<grid_of(k), TB, 0, s>>>(x, (float2 *)a.part, a.pixels, C, G, Cg, k);
     if (hipError_t e = hipGetLastError()) return e;
-    norm_finish_kernel<T><<<grid_1d(a.batch * G), 64, 0, s>>>(x, (const float2 *)a.part, a.mean, a.rstd, a.batch * G,
-                                                              a.pixels, C, G, Cg, k.cols * VEC, a.eps, k);
+    norm_finish_kernel<<<grid_1d(a.batch * G), 64, 0, s>>>((const float2 *)a.part, a.mean, a.rstd, a.batch * G, a.pixels, G, Cg,
+                                                           k.cols * VEC, a.eps, k);
     if (hipError_t e = hipGetLastError()) return e;
     norm_apply_kernel<T, VEC><<<grid_of(k), TB, 0, s>>>(x, a.weight, a.bias, a.mean, a.rstd, (T *)a.y, a.pixels, C, G,
                                                         Cg, a.act, k);
