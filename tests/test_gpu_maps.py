@@ -103,6 +103,14 @@ def test_norm_of_large_groups_with_large_means_or_constant(shape, groups, dtype)
     assert torch.equal(y, b.view(-1, *[1] * (len(shape) - 2)).expand_as(y))
 
 
+@pytest.mark.parametrize("shape,groups", [((2, 16, 9, 7), 2)] + LARGE_GROUPS)
+def test_norm_of_spreads_whose_square_is_no_float32(shape, groups):
+    """The variance is infinite then, its deviation's reciprocal 0: results are the bias, not NaN, whatever holds the group."""
+    x, w, b, _ = norm_case(shape, torch.float32, spread=1e25)
+    y = tvdcn.group_norm_act(x, groups, w, b)
+    assert torch.equal(y, b.view(-1, *[1] * (len(shape) - 2)).expand_as(y))
+
+
 def test_norm_values_that_are_not_finite_stay_in_their_group():
     x, w, b, dy = norm_case((2, 32, 9, 9), torch.float32)
     ref = tvdcn.group_norm_act(x, 4, w, b, 1e-5, "silu")

@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(TB) norm_stats_kernel(const T *__restrict__ x,
                 for (int v = 0; v < VEC; ++v) {
                     const float step = s[v] * inv;
                     mean[v] += step;
-                    sq[v] += fmaf(-s[v], step, q[v]);
+                    sq[v] += q[v] > 3.402823466e38f ? q[v] : fmaf(-s[v], step, q[v]);   // (beyond float32: infinite, not a NaN)
                 }
             }
         }
