@@ -231,6 +231,21 @@ def test_float16_arguments_beyond_its_range(act, device):
 
 
 @pytest.mark.parametrize("device", ["cpu", "cuda"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_gelu_of_negative_arguments_is_rounded_once(dtype, device):
+    """Every value of the type from -12.9 to 0: half a step of the result, and 2^-14 of it for the distribution function in its tail
+    (3.3e-5), its product and the exponential's argument."""
+    x = torch.arange(-32768, 32768, dtype=torch.int32).to(torch.int16).view(dtype)
+    x = x[(x < 0) & (x > -12.9)]
+    x = torch.cat([x, x[:-x.numel() % 8]]).view(-1, 8).to(device)
+    y = tvdcn.pointwise_conv(x, torch.eye(8, dtype=dtype, device=device), None, None, "gelu")
+    # (by erfc: float64's own bits in the tail)
+    want, info = x.double() * torch.special.erfc(x.double() * -0.5 ** 0.5) / 2, torch.finfo(dtype)
+    off = (y.double() - want).abs() - (info.eps / 2 * (1 + 2.0 ** -14) + 2.0 ** -14) * want.abs() - info.tiny * info.eps / 2
+    assert off.max() <= 0, (x.flatten()[off.argmax()], y.flatten()[off.argmax()], want.flatten()[off.argmax()])
+
+
+@pytest.mark.parametrize("device", ["cpu", "cuda"])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("bad", [float("inf"), float("nan")])
 def test_gradients_that_a_shut_rectifier_drops(bad, dtype, device):
