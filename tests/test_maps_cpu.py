@@ -1,6 +1,8 @@
 """The operators on channels-last maps without a GPU: the host kernels against the float64 definitions, gradients against
 differences, refusals (Python, operators and C ABI), shapes without data, TorchScript, compilation and modules."""
 import ctypes
+import os
+import re
 
 import pytest
 import torch
@@ -237,6 +239,20 @@ def test_empty_maps():
         g = torch.ones(6, requires_grad=True)
         tvdcn.pointwise_conv(tvdcn.group_norm_act(x, 2, g), w).sum().backward()
         assert not w.grad.any() and not g.grad.any() and x.grad.shape == shape
+
+
+def test_inline_assembly_declares_the_registers_it_names():
+    """A scalar register that an asm statement writes by name stands in its list of clobbers."""
+    folder = os.path.join(os.path.dirname(tvdcn.extension.HIP_LIB_PATH), "csrc", "hip")
+    seen = 0
+    for name in sorted(os.listdir(folder)):
+        with open(os.path.join(folder, name)) as f:
+            source = f.read()
+        for text in re.findall(r"\basm\s*(?:volatile)?\s*\((.*?)\);", source, re.S):
+            for register in re.findall(r"s_mov_b32 (m0|vcc_lo|exec_lo|s\d+)\b", text):
+                seen += 1
+                assert '"%s"' % register in text, (name, text)
+    assert seen > 0
 
 
 # ---- C ABI ----

@@ -74,13 +74,17 @@ struct Product {
     bool sums;
 };
 
-// 64 lanes x 16 bytes from a buffer into 1 KB of LDS at `lds` (uniform)
+// 64 lanes x 16 bytes from a buffer into 1 KB of LDS at `lds` (uniform). m0 is declared as written: the compiler allocates it to
+// nothing, which it warns of, but may keep it set from one of its own uses to the next.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void load_to_lds(const u32x4 &rsrc, uint32_t offset, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                  :
                  : "s"(lds), "v"(offset), "s"(rsrc)
-                 : "memory");
+                 : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
 template <int N> constexpr int log2_of() { return N <= 1 ? 0 : 1 + log2_of<N / 2>(); }
 
