@@ -228,10 +228,10 @@ tvdcn_status tvdcn_expand_activation(int32_t dtype, int64_t rows, int64_t channe
 /*
  * Group normalisation, affine map and activation: y = act(weight * (x - mean) * rstd + bias), mean
  * and rstd = 1 / sqrt(variance + eps) over the pixels and the channels / groups channels of each
- * (image, group); weight and bias may be NULL (1 and 0). mean and rstd (batch x groups, float32)
- * are written by the forward and read by the backward. In the backward the input may be given as
- * its 8-bit map instead (input NULL, codes and exponents not). grad_input, grad_weight and
- * grad_bias may be NULL (not computed).
+ * (image, group); weight and bias may be NULL (1 and 0). mean and rstd (batch x groups, float32; a
+ * float's alignment will do) are written by the forward and read by the backward. In the backward
+ * the input may be given as its 8-bit map instead (input NULL, codes and exponents not).
+ * grad_input, grad_weight and grad_bias may be NULL (not computed).
  */
 typedef struct {
     int32_t dtype;       /* tvdcn_dtype */

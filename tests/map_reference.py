@@ -172,3 +172,26 @@ def make(shape, dtype, seed, device="cuda", spread=1.0, shift=0.0):
     if len(shape) > 2:
         x = x.movedim(1, -1).contiguous().movedim(-1, 1)
     return x.to(dtype).to(device)
+
+
+def layouts(device, dtype, shape, groups, out):
+    """Shape, strides and type of every result of every operator, the internal ones among them, for maps of this shape."""
+    ops = torch.ops.tvdcn
+    x, w = torch.zeros(shape, device=device, dtype=dtype), torch.zeros(out, shape[1], device=device, dtype=dtype)
+    p, b = torch.zeros(shape[1], device=device, dtype=dtype), torch.zeros(out, device=device, dtype=dtype)
+    every = [True] * 3
+    got = []
+    for act in range(len(ACTIVATIONS)):
+        y, stats = ops._group_norm_act_forward(x, groups, p, p, 1e-5, act)
+        got += [y, stats, *ops._group_norm_act_backward(y, x, None, None, p, p, stats, act, every)]
+        y, pre = ops._pointwise_conv_forward(x, w, b, None, act, True)
+        got += [y, pre, *ops._pointwise_conv_backward(y, x, None, None, w, pre, act, every)]
+        if dtype != torch.float64:
+            codes, exponents = ops.compress_activation(x)
+            got += [codes, exponents, ops.expand_activation(codes, exponents, dtype)]
+            got += ops._group_norm_act_backward(x, None, codes, exponents, p, p, stats, act, every)
+            got += ops._pointwise_conv_backward(y, None, codes, exponents, w, pre, act, every)
+    return [(tuple(t.shape), t.stride(), t.dtype) for t in got]
+
+
+LAYOUT_SHAPES = [((3, 42, 4, 5), 7, 10), ((1, 8, 9), 1, 8), ((5, 6), 2, 3), ((2, 3, 1, 2, 4), 3, 1), ((0, 6, 4), 2, 4), ((2, 6, 0), 3, 4)]

@@ -5,7 +5,8 @@ import pytest
 import torch
 
 import tvdcn
-from map_reference import ACTIVATIONS, as_map, as_rows, check, kept, make, norm, pointwise, value
+from map_reference import (ACTIVATIONS, LAYOUT_SHAPES, as_map, as_rows, check, kept, layouts, make, norm, pointwise,
+                           value)
 
 pytestmark = pytest.mark.gpu
 DTYPES = [torch.float32, torch.float16, torch.bfloat16]
@@ -344,6 +345,31 @@ def test_memory_orders_and_alignment():
             assert torch.equal(p, q)
     wt = make((48, 32), torch.float16, 7).t()
     assert torch.equal(tvdcn.pointwise_conv(base, wt[:, :, None, None]), tvdcn.pointwise_conv(base, wt.contiguous()))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_shapes_without_data_have_the_layouts_of_the_results(dtype):
+    for shape, groups, out in LAYOUT_SHAPES:
+        assert layouts("meta", dtype, shape, groups, out) == layouts("cuda", dtype, shape, groups, out), shape
+
+
+@pytest.mark.parametrize("keep", [False, True])
+def test_compiled_training_step(keep):
+    """Forward and backward through torch.compile's tracing, statistics of 21 groups among what it keeps."""
+    x, dy = make((3, 42, 5, 4), torch.float32, 1), make((3, 10, 5, 4), torch.float32, 2)
+    ps = [make((42,), torch.float32, 3), make((42,), torch.float32, 4), make((10, 42), torch.float32, 5), make((10,), torch.float32, 6)]
+
+    def block(x, g, s, w, b):
+        y = tvdcn.group_norm_act(x, 7, g, s, activation="silu", keep_int8=keep)
+        return tvdcn.pointwise_conv(y, w, b, None, "gelu", keep)
+
+    got = []
+    for f in (block, torch.compile(block, backend="aot_eager", fullgraph=True)):
+        leaves = [leaf(t) for t in (x, *ps)]
+        y = f(*leaves)
+        got.append([y.detach(), *torch.autograd.grad(y, leaves, dy)])
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
 
 
 def test_empty_maps():

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import tvdcn
-from map_reference import ACTIVATIONS, as_map, as_rows, check, kept, make, norm, pointwise
+from map_reference import ACTIVATIONS, LAYOUT_SHAPES, as_map, as_rows, check, kept, layouts, make, norm, pointwise
 
 DTYPES = [torch.float64, torch.float32, torch.float16, torch.bfloat16]
 OPS = torch.ops.tvdcn
@@ -233,6 +233,13 @@ def test_modules_script_and_compile(keep):
     assert torch.allclose(tvdcn.pointwise_conv(x, conv.weight, conv.bias), conv(x), atol=1e-5)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_shapes_without_data_have_the_layouts_of_the_results(dtype):
+    """What compilation plans with: sizes, strides and types of the Meta kernels are the host kernels'."""
+    for shape, groups, out in LAYOUT_SHAPES:
+        assert layouts("meta", dtype, shape, groups, out) == layouts("cpu", dtype, shape, groups, out), shape
+
+
 def test_empty_maps():
     for shape in ((0, 6, 4), (2, 6, 0)):
         x, w = torch.zeros(shape, requires_grad=True), torch.zeros(4, 6, requires_grad=True)
@@ -367,3 +374,12 @@ def test_c_abi_refuses_pointers_and_workspaces(lib):
     # rows of none: nothing to do, no pointers needed
     assert f(ctypes.byref(point_desc(rows=0)), None, None, None, None, None, None, None, 0, None) == SUCCESS
     assert lib.tvdcn_group_norm_act_forward(ctypes.byref(norm_desc(batch=0)), None, None, None, None, None, None, None, 0, None) == SUCCESS
+
+
+def test_c_abi_statistics_are_single_floats(lib):
+    p, big, d = P(4096), 1 << 40, ctypes.byref(norm_desc(pixels=1 << 20))
+    f, b = lib.tvdcn_group_norm_act_forward, lib.tvdcn_group_norm_act_backward
+    assert b(d, p, p, None, None, p, p, P(4100), P(4116), None, None, None, p, big, None) == SUCCESS   # (nothing asked for)
+    assert b(d, p, p, None, None, p, p, P(4098), p, None, None, None, p, big, None) == INVALID
+    assert b(d, p, p, None, None, p, p, p, None, p, p, p, p, big, None) == INVALID
+    assert f(d, p, p, p, p, P(4098), p, p, big, None) == INVALID and f(d, p, p, p, p, p, None, p, big, None) == INVALID

@@ -44,6 +44,13 @@ tvdcn_status check_pointers(const char *what, std::initializer_list<const void *
     return TVDCN_STATUS_SUCCESS;
 }
 
+// statistics: single floats
+tvdcn_status check_floats(std::initializer_list<const void *> pointers) {
+    for (const void *p : pointers)
+        if (reinterpret_cast<uintptr_t>(p) & 3) return invalid("statistics must be 4-byte aligned");
+    return TVDCN_STATUS_SUCCESS;
+}
+
 tvdcn_status check_workspace(const void *workspace, size_t have, size_t need) {
     if (have < need || (need > 0 && !workspace))
         return api_fail(TVDCN_STATUS_WORKSPACE_TOO_SMALL, "workspace too small: " + std::to_string(have) + " bytes, " +
@@ -151,7 +158,9 @@ tvdcn_status tvdcn_group_norm_act_forward(const tvdcn_norm_desc *desc, const voi
     RETURN_IF(norm_args(desc, a));
     api_clear_error();
     if (a.batch == 0 || a.pixels == 0) return TVDCN_STATUS_SUCCESS;
-    RETURN_IF(check_pointers(NORM, {input, output, mean, rstd}, {weight, bias}));
+    RETURN_IF(check_pointers(NORM, {input, output}, {weight, bias}));
+    if (!mean || !rstd) return invalid("group_norm_act: null tensor");
+    RETURN_IF(check_floats({mean, rstd}));
     RETURN_IF(check_workspace(workspace, workspace_bytes, norm_bytes(a, false)));
     a.x = input;
     a.weight = weight;
@@ -172,11 +181,12 @@ tvdcn_status tvdcn_group_norm_act_backward(const tvdcn_norm_desc *desc, const vo
     NormArgs a;
     RETURN_IF(norm_args(desc, a));
     api_clear_error();
-    RETURN_IF(check_pointers(NORM, {}, {grad_out, input, codes, exponents, weight, bias, mean, rstd, grad_input,
-                                        grad_weight, grad_bias}));
+    RETURN_IF(check_pointers(NORM, {}, {grad_out, input, codes, exponents, weight, bias, grad_input, grad_weight, grad_bias}));
+    RETURN_IF(check_floats({mean, rstd}));
     if (a.batch > 0 && a.pixels > 0) {
         RETURN_IF(check_source(NORM, input, codes, exponents));
-        RETURN_IF(check_pointers(NORM, {grad_out, mean, rstd}, {}));
+        RETURN_IF(check_pointers(NORM, {grad_out}, {}));
+        if (!mean || !rstd) return invalid("group_norm_act: null tensor");
         RETURN_IF(check_workspace(workspace, workspace_bytes, norm_bytes(a, true)));
     }
     if (!grad_input && !grad_weight && !grad_bias) return TVDCN_STATUS_SUCCESS;

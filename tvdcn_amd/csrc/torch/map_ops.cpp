@@ -189,6 +189,7 @@ Tensor expand_meta(const Tensor &codes, const Tensor &exponents, at::ScalarType 
 }
 
 Two compress_cpu(const Tensor &x) {
+    if (x.numel() == 0) return compress_meta(x);   // (empty tensors of x's device)
     check_compress(x);
     const int64_t C = x.size(1), B = blocks_of(C);
     // in float64 the scaling is exact for every float32
@@ -262,15 +263,13 @@ Two norm_forward_hip(const Tensor &x, int64_t groups, MaybeTensor weight, MaybeT
     c10::DeviceGuard guard(x.device());
     const Tensor r = rows_of(x), w = flat(weight), b = flat(bias);
     const tvdcn_norm_desc d{map_dtype(x.scalar_type(), NORM), (int32_t)act, x.size(0), pixels_of(x), x.size(1), groups, eps};
-    // (the second half starts on a multiple of 16 bytes)
-    const int64_t half = (x.size(0) * groups + 3) / 4 * 4;
     Tensor y = new_map(x.sizes(), x.options());
-    Tensor stats = at::empty_strided({2, x.size(0), groups}, {half, groups, 1}, x.options().dtype(at::kFloat));
+    Tensor stats = at::empty({2, x.size(0), groups}, x.options().dtype(at::kFloat));
     if (x.numel() == 0) return {y, stats.zero_()};
     const size_t n = tvdcn_group_norm_act_forward_workspace_size(&d);
     const Tensor work = n ? bytes(x, n) : Tensor();
     float *mean = (float *)ptr(stats);
-    check_status(tvdcn_group_norm_act_forward(&d, ptr(r), ptr(w), ptr(b), ptr(y), mean, mean + half, ptr(work), n, stream_of(x)), NORM);
+    check_status(tvdcn_group_norm_act_forward(&d, ptr(r), ptr(w), ptr(b), ptr(y), mean, mean + x.size(0) * groups, ptr(work), n, stream_of(x)), NORM);
     return {y, stats};
 }
 Three norm_backward_hip(const Tensor &grad, MaybeTensor input, MaybeTensor codes, MaybeTensor exponents, MaybeTensor weight,
@@ -280,11 +279,7 @@ Three norm_backward_hip(const Tensor &grad, MaybeTensor input, MaybeTensor codes
     const Tensor g = rows_of(grad), r = rows_of(input), q = rows_of(codes), e = rows_of(exponents);
     const Tensor w = flat(weight), b = flat(bias);
     const int64_t C = grad.size(1), groups = stats_.size(2);
-    Tensor stats = stats_;
-    if (stats.numel() > 0 && (stats.stride(2) != 1 || (stats.size(1) > 1 && stats.stride(1) != groups) || stats.stride(0) % 4 || !is_aligned(stats))) {
-        stats = at::empty_strided(stats_.sizes(), {(grad.size(0) * groups + 3) / 4 * 4, groups, 1}, stats_.options());
-        stats.copy_(stats_);
-    }
+    const Tensor stats = stats_.contiguous();
     const float *mean = (const float *)ptr(stats);
     const tvdcn_norm_desc d{map_dtype(grad.scalar_type(), NORM), (int32_t)act, grad.size(0), pixels_of(grad), C, groups, 0.0};
     Tensor dx, dw, db;
@@ -294,7 +289,7 @@ Three norm_backward_hip(const Tensor &grad, MaybeTensor input, MaybeTensor codes
     const size_t n = tvdcn_group_norm_act_backward_workspace_size(&d);
     const Tensor work = n ? bytes(grad, n) : Tensor();
     check_status(tvdcn_group_norm_act_backward(&d, ptr(g), ptr(r), (const int8_t *)ptr(q), (const uint8_t *)ptr(e), ptr(w), ptr(b),
-                                               mean, mean ? mean + stats.stride(0) : nullptr, ptr(dx), ptr(dw), ptr(db),
+                                               mean, mean ? mean + grad.size(0) * groups : nullptr, ptr(dx), ptr(dw), ptr(db),
                                                ptr(work), n, stream_of(grad)),
                  "group_norm_act backward");
     return {dx, dw, db};
