@@ -290,6 +290,23 @@ def test_only_the_gradients_asked_for(dtype):
         assert torch.equal(torch.autograd.grad(y, ts[i], dx)[0], full[1 + i])
 
 
+@pytest.mark.parametrize("keep", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,channels,out", [(300, 24, 40), (129, 71, 33), (20003, 1032, 1024)])
+def test_pointwise_through_a_frozen_weight(rows, channels, out, dtype, keep):
+    """Gradients of the input and the bias without an input kept, which changes before the backward: the same to the bit."""
+    x, w, b = make((rows, channels), dtype, 1), make((out, channels), dtype, 2, spread=channels ** -0.5), make((out,), dtype, 3)
+    dy = make((rows, out), dtype, 4)
+    want = run_pointwise(x, w, b, None, "gelu", dy, keep)
+    first, bias = leaf(x), leaf(b)
+    x2 = first * 1.0
+    y = tvdcn.pointwise_conv(x2, w, bias, None, "gelu", keep)
+    x2.detach().add_(1)
+    dx, db = torch.autograd.grad(y, [first, bias], dy)
+    for g, r in zip((y, dx, db), (want[0], want[1], want[3])):
+        assert torch.equal(g, r)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("shape", [(2, 64, 9, 7), (3, 71, 40), (1, 33), (5, 3, 2, 3, 4), (1, 1024, 31)])
 def test_round_trip(shape, dtype):

@@ -190,6 +190,31 @@ def test_input_changed_before_the_backward_is_noticed():
     y.sum().backward()
 
 
+@pytest.mark.parametrize("keep", [False, True])
+@pytest.mark.parametrize("act", ACTIVATIONS)
+def test_a_frozen_weight_keeps_no_input(act, keep):
+    """Only the weight's gradient reads the input: without it neither the map nor its codes are kept, and it may change."""
+    x, w = torch.randn(2, 6, 3, 5), torch.randn(4, 6)
+    for i, t in enumerate((x, torch.randn(4), torch.randn(2, 4, 3, 5))):   # the gradient of the input, the bias, the residual
+        kept = []
+        args = [x.clone(), w, torch.randn(4), torch.randn(2, 4, 3, 5)]
+        args[(0, 2, 3)[i]] = t.clone().requires_grad_(True)
+        if i == 0:
+            args[0] = args[0] * 1.0   # (a result, that may change in place)
+        with torch.autograd.graph.saved_tensors_hooks(lambda v: kept.append(v) or v, lambda v: v):
+            y = tvdcn.pointwise_conv(*args, act, keep)
+        assert not any(v.shape == x.shape or v.dtype in (torch.int8, torch.uint8) for v in kept)
+        if i:
+            args[0].add_(1)
+        y.sum().backward()
+    # the operator asks for an input where the weight's gradient is asked for
+    g = torch.randn(2, 4, 3, 5)
+    dx, dw, db = OPS._pointwise_conv_backward(g, None, None, None, w, None, 0, [True, False, True])
+    assert dx.shape == x.shape and dw is None and db.shape == (4,)
+    with pytest.raises(RuntimeError, match="expected the input"):
+        OPS._pointwise_conv_backward(g, None, None, None, w, None, 0, [True, True, True])
+
+
 def test_results_are_channels_last():
     for shape in ((2, 6, 4, 5), (2, 6, 4), (2, 6, 3, 4, 5), (3, 6)):
         for device in ("cpu", "meta"):

@@ -230,10 +230,10 @@ void check_norm(const Tensor &x, int64_t groups, MaybeTensor weight, MaybeTensor
     check_like(x, weight, "weight", {x.size(1)}, NORM);
     check_like(x, bias, "bias", {x.size(1)}, NORM);
 }
-// The backward's input: the map, or its 8-bit form, of the gradient's shape
+// The backward's input: the map, or its 8-bit form, of the gradient's shape; needed: not to be left out
 void check_source(const Tensor &grad, MaybeTensor input, MaybeTensor codes, MaybeTensor exponents, int64_t channels,
-                  const char *name) {
-    TORCH_CHECK(has(input) != has(codes) && has(codes) == has(exponents), name,
+                  const char *name, bool needed) {
+    TORCH_CHECK(!(has(input) && has(codes)) && (has(input) || has(codes) || !needed) && has(codes) == has(exponents), name,
                 " backward: expected the input, or its codes and exponents");
     check_like(grad, input, "input", map_shape(grad, channels), name);
     if (has(codes)) {
@@ -247,7 +247,7 @@ void check_norm_backward(const Tensor &grad, MaybeTensor input, MaybeTensor code
                          MaybeTensor weight, MaybeTensor bias, const Tensor &stats, int64_t activation) {
     check_map(grad, NORM);
     check_activation(activation, NORM);
-    check_source(grad, input, codes, exponents, grad.size(1), NORM);
+    check_source(grad, input, codes, exponents, grad.size(1), NORM, true);
     check_like(grad, weight, "weight", {grad.size(1)}, NORM);
     check_like(grad, bias, "bias", {grad.size(1)}, NORM);
     TORCH_CHECK(stats.dim() == 3 && stats.size(0) == 2 && stats.size(1) == grad.size(0) && stats.size(2) > 0 &&
@@ -394,11 +394,11 @@ at::ScalarType argument_type(const Tensor &x, int64_t act) {
     return x.scalar_type() == at::kBFloat16 && (act == TVDCN_ACT_SILU || act == TVDCN_ACT_GELU) ? at::kHalf : x.scalar_type();
 }
 void check_pointwise_backward(const Tensor &grad, MaybeTensor input, MaybeTensor codes, MaybeTensor exponents,
-                              const Tensor &weight, MaybeTensor pre, int64_t activation) {
+                              const Tensor &weight, MaybeTensor pre, int64_t activation, bool weight_grad) {
     check_map(grad, POINT);
     check_weight(grad, weight, grad.size(1), 0);
     check_activation(activation, POINT);
-    check_source(grad, input, codes, exponents, weight.size(1), POINT);
+    check_source(grad, input, codes, exponents, weight.size(1), POINT, weight_grad);   // (only the weight's gradient reads it)
     TORCH_CHECK(activation == TVDCN_ACT_NONE || has(pre), POINT, " backward: the activation's argument is missing");
     if (activation != TVDCN_ACT_NONE)
         TORCH_CHECK(pre->sizes() == grad.sizes() && pre->scalar_type() == argument_type(grad, activation) &&
@@ -424,7 +424,7 @@ Two point_forward_hip(const Tensor &x, const Tensor &weight, MaybeTensor bias, M
 }
 Three point_backward_hip(const Tensor &grad, MaybeTensor input, MaybeTensor codes, MaybeTensor exponents, const Tensor &weight,
                          MaybeTensor pre, int64_t act, std::array<bool, 3> want) {
-    check_pointwise_backward(grad, input, codes, exponents, weight, pre, act);
+    check_pointwise_backward(grad, input, codes, exponents, weight, pre, act, want[1]);
     c10::DeviceGuard guard(grad.device());
     const Tensor g = rows_of(grad), r = rows_of(input), q = rows_of(codes), e = rows_of(exponents), p = rows_of(pre);
     const Tensor w = flat(maybe(weight));
@@ -450,7 +450,7 @@ Two point_forward_meta(const Tensor &x, const Tensor &weight, MaybeTensor bias, 
 }
 Three point_backward_meta(const Tensor &grad, MaybeTensor input, MaybeTensor codes, MaybeTensor exponents,
                           const Tensor &weight, MaybeTensor pre, int64_t act, std::array<bool, 3> want) {
-    check_pointwise_backward(grad, input, codes, exponents, weight, pre, act);
+    check_pointwise_backward(grad, input, codes, exponents, weight, pre, act, want[1]);
     const auto o = grad.options();
     return {want[0] ? new_map(map_shape(grad, weight.size(1)), o) : Tensor(), want[1] ? at::empty(weight.sizes(), o) : Tensor(),
             want[2] ? at::empty({weight.size(0)}, o) : Tensor()};
@@ -476,7 +476,7 @@ Two point_forward_cpu(const Tensor &x, const Tensor &weight, MaybeTensor bias, M
 }
 Three point_backward_cpu(const Tensor &grad, MaybeTensor input, MaybeTensor codes, MaybeTensor exponents, const Tensor &weight,
                          MaybeTensor pre, int64_t act, std::array<bool, 3> want) {
-    check_pointwise_backward(grad, input, codes, exponents, weight, pre, act);
+    check_pointwise_backward(grad, input, codes, exponents, weight, pre, act, want[1]);
     const auto t = wide_type(grad), out = grad.scalar_type();
     const int64_t N = weight.size(0), K = weight.size(1);
     Tensor dz = to_rows(grad).to(t).reshape({-1, N});
@@ -605,10 +605,10 @@ class PointFunction : public torch::autograd::Function<PointFunction> {
         const bool slope = act != TVDCN_ACT_NONE && (needs(x) || needs(weight) || needs(bias));
         Two r = point_fwd().call(x, weight, bias, residual, act, slope && !by_y);
         const Tensor y = std::get<0>(r), pre = !slope ? Tensor() : by_y ? y : std::get<1>(r);
-        Tensor input = x, codes, exps;
-        if (keep_int8 && needs(weight)) {
-            std::tie(codes, exps) = compress_op().call(x);
-            input = Tensor();
+        Tensor input, codes, exps;   // (only the weight's gradient reads them)
+        if (needs(weight)) {
+            if (keep_int8) std::tie(codes, exps) = compress_op().call(x);
+            else input = x;
         }
         ctx->save_for_backward({input, codes, exps, weight, pre});
         ctx->saved_data["act"] = act;
