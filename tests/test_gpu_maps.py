@@ -104,6 +104,17 @@ def test_norm_of_large_groups_with_large_means_or_constant(shape, groups, dtype)
     assert torch.equal(y, b.view(-1, *[1] * (len(shape) - 2)).expand_as(y))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape,groups", LARGE_GROUPS + [((2, 64, 100, 110), 2), ((1, 40, 90, 100), 5)])
+def test_norm_of_large_groups_kept_in_8_bits(shape, groups, dtype):
+    """The backward in two passes over codes and exponents: whole blocks of 32 channels, short last ones, channels one by one."""
+    for i, act in enumerate(ACTIVATIONS):
+        x, w, b, dy = norm_case(shape, dtype, seed=10 * i)
+        got = run_norm(x, groups, w, b, act, dy, keep=True)
+        check(got, norm(x, groups, w, b, 1e-5, act, dy, keep_int8=True), (shape, act))
+        assert torch.equal(got[0], tvdcn.group_norm_act(x, groups, w, b, 1e-5, act))
+
+
 @pytest.mark.parametrize("shape,groups", [((2, 16, 9, 7), 2)] + LARGE_GROUPS)
 def test_norm_of_spreads_whose_square_is_no_float32(shape, groups):
     """The variance is infinite then, its deviation's reciprocal 0: results are the bias, not NaN, whatever holds the group."""
