@@ -668,7 +668,8 @@ Tensor point_direct(const Tensor &x, const Tensor &weight, MaybeTensor bias, May
 }
 
 // autocast: the normalisation keeps the map's type (its sums are float32 whatever that is) and takes its parameters in
-// it; the pointwise convolution runs in the autocast type, as torch's matrix products do
+// it, rounded where that has 16 bits, as a matrix product's weights are there: parameters have the map's type everywhere. The
+// pointwise convolution runs in the autocast type, as torch's matrix products do
 Tensor cast(at::ScalarType t, const Tensor &x) { return at::autocast::cached_cast(t, x, c10::DeviceType::CUDA); }
 optional<Tensor> cast(at::ScalarType t, MaybeTensor x) { return has(x) ? optional<Tensor>(cast(t, *x)) : optional<Tensor>(); }
 

@@ -26,14 +26,15 @@ def group_norm_act(input: Tensor, num_groups: int, weight: Optional[Tensor] = No
         input (Tensor[batch, channels, \*size]): the map; channels-last memory (``torch.channels_last`` in 2D) is read
             as it is, any other is copied first. (rows, channels) is a map without a grid.
         num_groups (int): divides the channels.
-        weight, bias (Tensor[channels]): of the input's type; 1 and 0 where absent.
+        weight, bias (Tensor[channels]): of the input's type (autocast rounds them to it); 1 and 0 where absent.
         eps (float): added to the variance.
         activation (str): "none", "relu", "silu" or "gelu" (with the error function).
         keep_int8 (bool): the input is kept for the backward in 8 bits (see :func:`compress_activation`), and the
             backward takes the gradients at the values kept. The output does not change.
 
     Returns:
-        Tensor[batch, channels, \*size]: channels-last.
+        Tensor[batch, channels, \*size]: channels-last. First derivatives by backward only: second ones and forward-mode
+        ones raise.
     """
     if not torch.jit.is_scripting():
         _log_api_usage_once(group_norm_act)

@@ -36,7 +36,8 @@ def pointwise_conv(input: Tensor, weight: Tensor, bias: Optional[Tensor] = None,
     to the input's type before the products. float64 runs on the CPU only.
 
     Returns:
-        Tensor[batch, out_channels, \*size]: channels-last.
+        Tensor[batch, out_channels, \*size]: channels-last. First derivatives by backward only: second ones and forward-mode
+        ones raise.
     """
     if not torch.jit.is_scripting():
         _log_api_usage_once(pointwise_conv)
