@@ -103,6 +103,7 @@ template <bool PRECISE> __device__ __forceinline__ float quotient(float a, float
     return PRECISE ? a / b : a * __builtin_amdgcn_rcpf(b);
 }
 
+// (silu below about -87: e^-z is no float32, or its reciprocal none of full precision; results of under 2e-36 are 0)
 template <bool PRECISE> __device__ __forceinline__ float act_value(float z, int act) {
     switch (act) {
         case TVDCN_ACT_RELU: return z < 0.f ? 0.f : z;   // (a NaN stays one)
