@@ -4,129 +4,16 @@
 // that is not comes in as a copy) and every result is a channels-last map. The CUDA kernels check, allocate results
 // and workspace from the caching allocator and call the C ABI on the current stream; the CPU kernels compute the same
 // definitions with ATen in float32 (float64 for float64 maps).
-#include <ATen/ATen.h>
-#include <ATen/autocast_mode.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
-#include <torch/autograd.h>
-#include <torch/library.h>
-
 #include <array>
 #include <cmath>
 #include <tuple>
-#include <vector>
 
-#include "tvdcn_hip.h"
+#include "map_tensors.h"
 
 namespace tvdcn_amd {
 namespace {
 
-using at::Tensor;
-using c10::optional;
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
-typedef std::tuple<Tensor, Tensor> Two;
-typedef std::tuple<Tensor, Tensor, Tensor> Three;
-typedef const optional<Tensor> &MaybeTensor;
-
 constexpr int64_t kBlock = 32;   // channels of an 8-bit map that share an exponent
-
-bool has(MaybeTensor t) { return t.has_value() && t->defined(); }
-Tensor get(MaybeTensor t) { return has(t) ? *t : Tensor(); }
-optional<Tensor> maybe(const Tensor &t) { return t.defined() ? optional<Tensor>(t) : optional<Tensor>(); }
-
-int32_t map_dtype(at::ScalarType t, const char *name) {
-    switch (t) {
-        case at::kFloat: return TVDCN_DTYPE_FLOAT32;
-        case at::kHalf: return TVDCN_DTYPE_FLOAT16;
-        case at::kBFloat16: return TVDCN_DTYPE_BFLOAT16;
-        default: TORCH_CHECK(false, name, ": unsupported dtype ", t, " on the GPU (expected float32, float16 or bfloat16)");
-    }
-    return -1;
-}
-
-void check_map(const Tensor &x, const char *name) {
-    TORCH_CHECK(x.dim() >= 2, name, ": expected a (batch, channels, *size) input, got ", x.dim(), " dimensions");
-    TORCH_CHECK(x.size(1) > 0, name, ": the input needs channels");
-    const auto t = x.scalar_type();
-    TORCH_CHECK(t == at::kFloat || t == at::kDouble || t == at::kHalf || t == at::kBFloat16, name, ": unsupported dtype ", t,
-                " (expected float32/64, float16, bfloat16)");
-}
-
-void check_like(const Tensor &x, MaybeTensor t, const char *what, at::IntArrayRef sizes, const char *name) {
-    if (!has(t)) return;
-    TORCH_CHECK(t->sizes() == sizes, name, ": expected ", what, " of shape ", sizes, ", got ", t->sizes());
-    TORCH_CHECK(t->scalar_type() == x.scalar_type(), name, ": expected ", what, " of dtype ", x.scalar_type(), ", got ",
-                t->scalar_type());
-    TORCH_CHECK(t->device() == x.device(), name, ": expected all tensors on ", x.device(), ", but ", what, " is on ",
-                t->device());
-}
-
-void check_activation(int64_t activation, const char *name) {
-    TORCH_CHECK(activation >= TVDCN_ACT_NONE && activation <= TVDCN_ACT_GELU, name, ": unknown activation ", activation);
-}
-
-// Dense channels-last memory: the last axes' strides under a channel stride of one
-bool is_rows(const Tensor &x) {
-    const auto sizes = x.sizes(), strides = x.strides();
-    const int64_t n = x.dim();
-    int64_t run = sizes[1];
-    if (sizes[1] > 1 && strides[1] != 1) return false;
-    for (int64_t i = n - 1; i >= 2; --i) {
-        if (sizes[i] > 1 && strides[i] != run) return false;
-        run *= sizes[i];
-    }
-    return sizes[0] <= 1 || strides[0] == run || x.numel() == 0;
-}
-bool is_aligned(const Tensor &x) { return x.is_meta() || (reinterpret_cast<uintptr_t>(x.data_ptr()) & 15) == 0; }
-// an empty map of these sizes in channels-last memory
-Tensor new_map(at::IntArrayRef sizes, const at::TensorOptions &options) {
-    const size_t n = sizes.size();
-    c10::SmallVector<int64_t, 6> strides(n);
-    int64_t run = 1;
-    strides[1] = run, run *= std::max<int64_t>(sizes[1], 1);
-    for (size_t i = n - 1; i >= 2; --i) strides[i] = run, run *= std::max<int64_t>(sizes[i], 1);
-    strides[0] = run;
-    return at::empty_strided(sizes, strides, options);
-}
-// the map with its channels contiguous per pixel, 16-byte aligned: itself, or a copy
-Tensor rows_of(const Tensor &x) {
-    if (is_rows(x) && is_aligned(x)) return x;
-    return new_map(x.sizes(), x.options()).copy_(x);
-}
-Tensor rows_of(MaybeTensor x) { return has(x) ? rows_of(*x) : Tensor(); }
-// [batch, *size, channels] (host kernels)
-Tensor to_rows(const Tensor &x) { return x.dim() == 2 ? x.contiguous() : x.movedim(1, -1).contiguous(); }
-Tensor flat(MaybeTensor v) {   // a parameter, contiguous and 16-byte aligned
-    if (!has(v)) return Tensor();
-    Tensor r = v->contiguous();
-    return (reinterpret_cast<uintptr_t>(r.data_ptr()) & 15) == 0 ? r : r.clone();
-}
-// an empty channels-last map of x's batch and size with `channels` channels, as rows
-Tensor new_rows(const Tensor &x, int64_t channels, at::TensorOptions options) {
-    std::vector<int64_t> s{x.size(0)};
-    for (int64_t i = 2; i < x.dim(); ++i) s.push_back(x.size(i));
-    s.push_back(channels);
-    return at::empty(s, options);
-}
-Tensor to_map(const Tensor &rows) { return rows.dim() == 2 ? rows : rows.movedim(-1, 1); }
-std::vector<int64_t> map_shape(const Tensor &x, int64_t channels) {
-    std::vector<int64_t> s = x.sizes().vec();
-    s[1] = channels;
-    return s;
-}
-int64_t pixels_of(const Tensor &x) {
-    int64_t n = 1;
-    for (int64_t i = 2; i < x.dim(); ++i) n *= x.size(i);
-    return n;
-}
-
-void check_status(tvdcn_status st, const char *what) {
-    TORCH_CHECK(st == TVDCN_STATUS_SUCCESS, what, " failed (status ", (int)st, "): ", tvdcn_last_error());
-}
-void *stream_of(const Tensor &t) { return (void *)c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
-void *ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
-Tensor bytes(const Tensor &x, size_t n) { return at::empty({(int64_t)n}, x.options().dtype(at::kByte)); }
 
 // ---------------------------------------------------------------------------
 // compress_activation / expand_activation
@@ -308,14 +195,6 @@ Three norm_backward_meta(const Tensor &grad, MaybeTensor input, MaybeTensor code
             want[2] ? at::empty({C}, grad.options()) : Tensor()};
 }
 
-at::ScalarType wide_type(const Tensor &t) { return t.scalar_type() == at::kDouble ? at::kDouble : at::kFloat; }
-
-Tensor act_value(const Tensor &z, int64_t act) {
-    if (act == TVDCN_ACT_RELU) return at::relu(z);
-    if (act == TVDCN_ACT_SILU) return z * at::sigmoid(z);
-    if (act == TVDCN_ACT_GELU) return z * at::erfc(z * -M_SQRT1_2) * 0.5;
-    return z;
-}
 // d act'(z); zero where a rectifier is shut, also of a gradient that is not finite
 Tensor act_slopes(const Tensor &d, const Tensor &z, int64_t act) {
     if (act == TVDCN_ACT_RELU) return d.masked_fill(z <= 0, 0.0);
@@ -501,67 +380,11 @@ using PointFwd = Two(const Tensor &, const Tensor &, MaybeTensor, MaybeTensor, i
 using PointBwd = Three(const Tensor &, MaybeTensor, MaybeTensor, MaybeTensor, const Tensor &, MaybeTensor, int64_t,
                        std::array<bool, 3>);
 
-template <typename Sig> c10::TypedOperatorHandle<Sig> op_of(const char *name) {
-    return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").template typed<Sig>();
-}
 auto &norm_fwd() { static auto op = op_of<NormFwd>("tvdcn::_group_norm_act_forward"); return op; }
 auto &norm_bwd() { static auto op = op_of<NormBwd>("tvdcn::_group_norm_act_backward"); return op; }
 auto &point_fwd() { static auto op = op_of<PointFwd>("tvdcn::_pointwise_conv_forward"); return op; }
 auto &point_bwd() { static auto op = op_of<PointBwd>("tvdcn::_pointwise_conv_backward"); return op; }
 auto &compress_op() { static auto op = op_of<Two(const Tensor &)>("tvdcn::compress_activation"); return op; }
-
-// A node that raises where a second derivative is asked for. all: the n gradients, then the tensors that they depend on.
-class NoSecondDerivative : public torch::autograd::Function<NoSecondDerivative> {
-   public:
-    static variable_list forward(AutogradContext *ctx, at::TensorList all, int64_t n, const std::string &name) {
-        at::AutoDispatchBelowADInplaceOrView guard;
-        ctx->saved_data["name"] = name;
-        variable_list out;
-        for (int64_t i = 0; i < n; ++i) out.push_back(all[i].alias());
-        return out;
-    }
-    static variable_list backward(AutogradContext *ctx, const variable_list &) {
-        TORCH_CHECK(false, "double backwards on ", ctx->saved_data["name"].toStringRef(), " not supported");
-        return {};
-    }
-};
-
-// Which gradients are asked for: the node's edges are those of the tensors that were given
-bool wanted(AutogradContext *ctx, const char *edge) {
-    const int64_t i = ctx->saved_data[edge].toInt();
-    return i >= 0 && ctx->needs_input_grad(i);
-}
-
-// Forward-mode derivatives have no formula here: a tangent that an input brings is refused, not dropped
-void check_no_tangents(const char *name, std::initializer_list<Tensor> ts) {
-    for (const Tensor &t : ts)
-        TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), name, ": forward-mode derivatives (jvp) are not supported");
-}
-
-bool needs(const Tensor &t) { return t.defined() && t.requires_grad(); }
-bool needs(MaybeTensor t) { return has(t) && t->requires_grad(); }
-
-// The gradients (undefined where not wanted), with the raising node where a graph of the backward is made
-variable_list with_node(const Three &g, const variable_list &used, const char *name) {
-    variable_list r{std::get<0>(g), std::get<1>(g), std::get<2>(g)};
-    bool graph = false;
-    if (at::GradMode::is_enabled())
-        for (const Tensor &t : used) graph = graph || needs(t);
-    if (!graph) return r;
-    variable_list there, in;
-    for (const Tensor &t : r)
-        if (t.defined()) there.push_back(t);
-    for (const Tensor &t : used)
-        if (t.defined()) in.push_back(t);
-    if (there.empty()) return r;
-    const size_t n = there.size();
-    there.insert(there.end(), in.begin(), in.end());
-    const variable_list made = NoSecondDerivative::apply(at::TensorList(there), (int64_t)n, std::string(name));
-    size_t at = 0;
-    for (Tensor &t : r)
-        if (t.defined()) t = made[at++];
-    return r;
-}
 
 class NormFunction : public torch::autograd::Function<NormFunction> {
    public:
@@ -631,13 +454,6 @@ class PointFunction : public torch::autograd::Function<PointFunction> {
     }
 };
 
-bool any_grad(std::initializer_list<Tensor> ts) {
-    if (!at::GradMode::is_enabled()) return false;
-    for (const Tensor &t : ts)
-        if (needs(t)) return true;
-    return false;
-}
-
 Tensor norm_autograd(const Tensor &x, int64_t groups, MaybeTensor weight, MaybeTensor bias, double eps, int64_t act,
                      bool keep_int8) {
     check_no_tangents(NORM, {x, get(weight), get(bias)});
@@ -670,8 +486,6 @@ Tensor point_direct(const Tensor &x, const Tensor &weight, MaybeTensor bias, May
 // autocast: the normalisation keeps the map's type (its sums are float32 whatever that is) and takes its parameters in
 // it, rounded where that has 16 bits, as a matrix product's weights are there: parameters have the map's type everywhere. The
 // pointwise convolution runs in the autocast type, as torch's matrix products do
-Tensor cast(at::ScalarType t, const Tensor &x) { return at::autocast::cached_cast(t, x, c10::DeviceType::CUDA); }
-optional<Tensor> cast(at::ScalarType t, MaybeTensor x) { return has(x) ? optional<Tensor>(cast(t, *x)) : optional<Tensor>(); }
 
 Tensor norm_autocast(const Tensor &x, int64_t groups, MaybeTensor weight, MaybeTensor bias, double eps, int64_t act,
                      bool keep_int8) {
