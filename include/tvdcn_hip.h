@@ -281,6 +281,68 @@ tvdcn_status tvdcn_pointwise_conv_backward(const tvdcn_pointwise_desc *desc, con
                                            const void *pre, void *grad_input, void *grad_weight, void *grad_bias,
                                            void *workspace, size_t workspace_bytes, void *stream);
 
+/*
+ * Operators that take a row (the channels of a pixel) as one vector; rows x channels as above, and
+ * the same rules. Results do not share memory with operands.
+ *
+ * Root-mean-square normalisation: s = input + residual (rounded to the map's type; the input itself
+ * where residual is NULL), output = weight * s * rstd, rstd = 1 / sqrt(mean(s^2) + eps) over a row's
+ * channels; weight may be NULL (1). sum receives s (only with a residual), rstd (rows, float32, may be
+ * NULL) is read by the backward. eps: a normal float32 above zero. The backward takes what was
+ * normalised (s) and the gradients of output and sum (grad_sum may be NULL: zero); grad_input (the
+ * residual's too) and grad_weight may be NULL (not computed).
+ */
+typedef struct {
+    int32_t dtype;       /* tvdcn_dtype */
+    int64_t rows;
+    int64_t channels;
+    double eps;
+} tvdcn_rms_norm_desc;
+tvdcn_status tvdcn_rms_norm_forward(const tvdcn_rms_norm_desc *desc, const void *input, const void *residual,
+                                    const void *weight, void *sum, void *output, float *rstd, void *stream);
+size_t tvdcn_rms_norm_backward_workspace_size(const tvdcn_rms_norm_desc *desc);
+tvdcn_status tvdcn_rms_norm_backward(const tvdcn_rms_norm_desc *desc, const void *grad_out, const void *grad_sum,
+                                     const void *normalised, const float *rstd, const void *weight, void *grad_input,
+                                     void *grad_weight, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * 8 bits with a scale per row: scale = max(max |x| * (1 / 127), 2^-126) in float32 (at most the
+ * largest of which 127 are finite), and codes x / scale rounded to the nearest integer, ties to
+ * even (the quotient as if exact). A code stands for code * scale. A row that holds an infinity or a
+ * NaN has codes 0 and the scale NaN: it stands for NaN. A weight (out x in) has a scale per output
+ * channel so. tvdcn_rms_norm_int8 does this to the normalised row, held in float32. codes: rows x
+ * channels; scales: rows, float32.
+ */
+tvdcn_status tvdcn_quantize_int8(int32_t dtype, int64_t rows, int64_t channels, const void *input, int8_t *codes,
+                                 float *scales, void *stream);
+tvdcn_status tvdcn_dequantize_int8(int32_t dtype, int64_t rows, int64_t channels, const int8_t *codes,
+                                   const float *scales, void *output, void *stream);
+tvdcn_status tvdcn_rms_norm_int8(const tvdcn_rms_norm_desc *desc, const void *input, const void *residual,
+                                 const void *weight, void *sum, int8_t *codes, float *scales, void *stream);
+
+/*
+ * The pointwise convolution of 8-bit rows with 8-bit weights:
+ * output = act(scale * weight_scale * sum(code * weight_code) + bias) + residual, the sums in whole
+ * numbers. The descriptor's dtype is that of output, bias and residual (may be NULL); at most 131071 input
+ * channels.
+ */
+size_t tvdcn_pointwise_conv_int8_workspace_size(const tvdcn_pointwise_desc *desc);
+tvdcn_status tvdcn_pointwise_conv_int8(const tvdcn_pointwise_desc *desc, const int8_t *codes, const float *scales,
+                                       const int8_t *weight_codes, const float *weight_scales, const void *bias,
+                                       const void *residual, void *output, void *workspace, size_t workspace_bytes,
+                                       void *stream);
+
+/*
+ * Dropout with a mask that follows from the seed and a value's place: output = (kept ? input /
+ * (1 - p) : 0) + residual (may be NULL) over n values. p in [0, 1] is rounded to a multiple of 2^-16.
+ * Bits: Philox4x32-10, key = the two halves of *seed (device memory, 8-byte aligned), counter =
+ * (i / 8, 0, 0) as 64 + 32 + 32 bits; value i has the low (i even) or high half of word i % 8 / 2 and is
+ * dropped where that is below 65536 p. The same call without a residual on output's gradient gives
+ * input's.
+ */
+tvdcn_status tvdcn_seeded_dropout(int32_t dtype, int64_t n, double p, const int64_t *seed, const void *input,
+                                  const void *residual, void *output, void *stream);
+
 /* Thread-local text of the last error (empty string when none). */
 const char *tvdcn_last_error(void);
 
@@ -307,8 +369,11 @@ enum {
     TVDCN_KERNEL_MASK_SOFTMAX = 5,
     TVDCN_KERNEL_GROUP_NORM = 6,
     TVDCN_KERNEL_POINTWISE = 7,
-    TVDCN_KERNEL_INT8_MAP = 8,      /* 8-bit maps, compress and expand */
-    TVDCN_KERNEL_FAMILIES = 9
+    TVDCN_KERNEL_INT8_MAP = 8,      /* 8-bit maps: compress, expand, quantize, dequantize */
+    TVDCN_KERNEL_RMS_NORM = 9,
+    TVDCN_KERNEL_POINTWISE_INT8 = 10,
+    TVDCN_KERNEL_DROPOUT = 11,
+    TVDCN_KERNEL_FAMILIES = 12
 };
 void tvdcn_kernel_timer_enable(int32_t enable);
 tvdcn_status tvdcn_kernel_timer_read(int32_t family, double *total_ms, int64_t *launches);

@@ -17,7 +17,8 @@ from tvdcn_amd.extension import (  # noqa: F401
 from tvdcn_amd.ops import *  # noqa: F401,F403
 
 for _name in ("ops", "ops.activations", "ops.activations.mask_sigmoid", "ops.activations.mask_softmax",
-              "ops.deform_conv", "ops.deform_conv_transpose", "ops.group_norm", "ops.int8_maps", "ops.pointwise",
+              "ops.deform_conv", "ops.deform_conv_transpose", "ops.dropout", "ops.group_norm", "ops.int8_maps", "ops.pointwise",
+              "ops.pointwise_int8", "ops.rms_norm",
               "extension", "utils", "_version"):
     _sys.modules[f"{__name__}.{_name}"] = _sys.modules[f"{_impl.__name__}.{_name}"]
 del _name
