@@ -1,8 +1,17 @@
 // The pointwise convolution of an 8-bit map with 8-bit weights: y = act(sx sw sum(q qw) + b) + r, with a scale sx per row and sw per
 // output channel. The sums are whole numbers, exact in 32 bits up to 131071 channels (2^17 products of at most 2^14).
 //
-// The kernels are those of product_kernels.h on 16x16x64 MFMAs: twice the products per instruction and byte of the 16-bit ones.
-// Channels that are no multiple of 16 are copied to rows that are, with zeros behind them.
+// Large products take the tiles of product_kernels.h on 16x16x64 MFMAs: twice the products per instruction and byte of the 16-bit
+// ones. Channels that are no multiple of 16 are copied to rows that are, with zeros behind them. Small products have a kernel of
+// their own, without copies.
+//
+// 8192 x 8192 to 8192 runs at 2570 TOP/s (a plain library product of 8-bit integers: 2150). With few channels the results bound it:
+// 65536 x 2048 to 512 takes 70 us, 86 with a residual and 83 with gelu, of which 53 are products; 65536 x 512 to 2048 108, 175 and
+// 158. A tile's stores, and the residual's loads before them, come from all CUs at about the same time, and nothing overlaps them:
+// two workgroups of 256 x 128 to a CU, one storing while the other multiplies, ran at 1920 TOP/s and were slower throughout (89, 106
+// and 98 us for the former).
+#include <cmath>
+
 #include "product_kernels.h"
 #include "rows.h"
 
@@ -35,20 +44,155 @@ __global__ void __launch_bounds__(TB) pad_codes_kernel(CodeCopy first, CodeCopy 
     }
 }
 
+// Small products, straight from memory (the caches) to the MFMAs: a lane's 16 bytes along the reduction are 16 bytes of a row, at
+// any alignment, so neither LDS stages nor copies are needed, and there are workgroups enough where 64 x 64 tiles leave most of the
+// chip idle: 1 x 2048 to 512 takes 3.8 us (64 x 64 tiles 8.4), 256 x 512 to 2048 5.5 (5.8), 2048 x 71 to 101 3.8 (7.7 with its copy).
+// A workgroup has 16 columns of 16 MF rows; its four waves take 64 bytes of the reduction in turn and add up through LDS.
+//
+// WHOLE: rows of whole 16 bytes. Otherwise (at least 16 bytes a row) the 16 bytes at a row's end are read and shifted down, which
+// leaves zeros behind it.
+template <bool WHOLE> __device__ __forceinline__ i32x4 load_codes(const int8_t *row, int k, int K) {
+    if constexpr (WHOLE) {
+        return k < K ? *reinterpret_cast<const i32x4 *>(row + k) : i32x4{0, 0, 0, 0};
+    } else {
+        if (k >= K) return i32x4{0, 0, 0, 0};
+        const int over = max(k + 16 - K, 0);   // bytes past the row's end
+        uint32_t v[4];
+        __builtin_memcpy(v, row + (k - over), 16);
+        if (over) {
+            if (over & 8) v[0] = v[2], v[1] = v[3], v[2] = v[3] = 0;
+            if (over & 4) v[0] = v[1], v[1] = v[2], v[2] = v[3], v[3] = 0;
+            const int bits = (over & 3) * 8;
+            v[0] = __builtin_amdgcn_alignbit(v[1], v[0], bits), v[1] = __builtin_amdgcn_alignbit(v[2], v[1], bits);
+            v[2] = __builtin_amdgcn_alignbit(v[3], v[2], bits), v[3] >>= bits;
+        }
+        return i32x4{(int)v[0], (int)v[1], (int)v[2], (int)v[3]};
+    }
+}
+
+template <typename T, int MF, bool WHOLE>
+__global__ void __launch_bounds__(TB) direct_product_kernel(Product p, const int8_t *__restrict__ x, const int8_t *__restrict__ w, int K) {
+    constexpr int WAVES = TB / 64, STEP = WAVES * 64;
+    constexpr int AHEAD = MF == 1 ? 8 : 4;   // steps whose loads are in flight together
+    static_assert(MF <= WAVES, "");
+    __shared__ i32x4 red[WAVES][MF][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, r = lane & 15;
+    const int total = p.tiles_r * p.tiles_c, id = blockIdx.x, per = total / 8, extra = total % 8, xcd = id % 8;
+    const int tile = xcd * per + min(xcd, extra) + id / 8;   // an XCD has neighbouring tiles, columns first
+    const int row0 = tile / p.tiles_c * (16 * MF), col0 = tile % p.tiles_c * 16;
+    // (rows and columns beyond the edge repeat the last ones: their results are not stored)
+    const int8_t *from_w = w + (int64_t)min(col0 + r, p.cols - 1) * K, *from_x[MF];
+#pragma unroll
+    for (int j = 0; j < MF; ++j) from_x[j] = x + (int64_t)min(row0 + j * 16 + r, p.rows - 1) * K;
+    i32x4 acc[MF];
+#pragma unroll
+    for (int j = 0; j < MF; ++j) acc[j] = i32x4{0, 0, 0, 0};
+    for (int k0 = wave * 64; k0 < K; k0 += AHEAD * STEP) {
+        i32x4 a[AHEAD], b[AHEAD][MF];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int k = k0 + u * STEP + q * 16;
+            if (u && k0 + u * STEP >= K) break;   // (uniform)
+            a[u] = load_codes<WHOLE>(from_w, k, K);
+#pragma unroll
+            for (int j = 0; j < MF; ++j) b[u][j] = load_codes<WHOLE>(from_x[j], k, K);
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            if (u && k0 + u * STEP >= K) break;
+#pragma unroll
+            for (int j = 0; j < MF; ++j) acc[j] = mfma(a[u], b[u][j], acc[j]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < MF; ++j) red[wave][j][lane] = acc[j];
+    __syncthreads();
+    if (wave >= MF) return;
+    // wave j stores fragment j: a lane has four columns of a row
+    i32x4 sum = red[0][wave][lane];
+#pragma unroll
+    for (int k = 1; k < WAVES; ++k) sum += red[k][wave][lane];
+    const int row = row0 + wave * 16 + r, col = col0 + q * 4;
+    if (row >= p.rows) return;
+    const float sr = p.scale_r[row];
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = (float)sum[e] * sr * p.scale_c[min(col + e, p.cols - 1)];
+    emit<T, 4>(p, 0, row, col, v);
+}
+
+// ---- host ----
+
+// Which kernel a product takes: the least of what they are measured to take, in microseconds. A launch, with the loads and results that
+// nothing overlaps, and so much per 128 bytes of the reduction; then the rounds after the first of a full chip (for the direct
+// kernel, the workgroups after the first 256). Tiles along the reduction are rows of 16 bytes: others are copied first. The
+// 256-wide tiles write whole eights of columns.
+//                         direct  64 x 64  128 x 128  256 x 128  256 x 256   (measured; us)
+//   64 x 512 to 512          4.0      5.5      10.3       9.8       13.3
+//   950 x 256 to 256         3.7      5.0      10.4       8.4       11.5
+//   4096 x 512 to 512       13.9      7.3      12.2      10.8       14.7
+//   4096 x 333 to 264       13.5      9.5      14.6      13.0       16.4
+//   8601 x 2048 to 512      78       23.0      23.3      22.8       31.0
+//   32768 x 256 to 256      34       15.5      14.1      11.4       14.3
+//   32768 x 512 to 2048    339      101        88        66         54
+//   32768 x 2048 to 2048  1133      287       202       170        133
+enum Kernel { DIRECT, SMALL, BIG, HALF, WIDE };
+double kernel_cost(Kernel k, int64_t rows, int64_t cols, int64_t in) {
+    auto tiles = [&](int r, int c) { return (double)ceil_div(rows, r) * ceil_div(cols, c); };
+    auto later = [&](int r, int c, int slots) { return std::ceil(tiles(r, c) / slots) - 1; };
+    auto filled = [&](int r, int c, int slots) { return std::min(1.0, tiles(r, c) / slots); };
+    const double steps = (double)ceil_div(in, 128), copy = in % 16 ? 2.5 + (rows + cols) * in * 0.45e-6 : 0;
+    switch (k) {
+        case DIRECT: return 2.8 + 2.3e-3 * in + std::max(0.0, tiles(rows <= 16 ? 16 : 64, 16) - 256) * (1.7e-3 + 8e-6 * in) * (in % 16 ? 1.9 : 1);
+        case SMALL: return copy + 4.2 + 0.33 * steps + later(64, 64, 512) * (1.6 + 0.41 * steps);
+        case BIG: return copy + 8.8 + 0.67 * steps + 4.5 * filled(128, 128, 512) + later(128, 128, 512) * (6 + 1.25 * steps);
+        case HALF: return copy + 6.5 + 0.87 * steps + 3.5 * filled(256, 128, 256) + later(256, 128, 256) * (4 + 0.93 * steps);
+        default: return copy + 8.4 + 1.26 * steps + 5 * filled(256, 256, 256) + later(256, 256, 256) * (5 + 1.7 * steps);
+    }
+}
+Kernel choose(const Int8ProductArgs &a) {
+    Kernel best = SMALL;
+    for (Kernel k : {DIRECT, BIG, HALF, WIDE}) {
+        if (k == DIRECT ? a.in < 16 : k >= HALF && a.out % 8 != 0) continue;
+        if (kernel_cost(k, a.rows, a.out, a.in) < kernel_cost(best, a.rows, a.out, a.in)) best = k;
+    }
+    return best;
+}
+
 struct Plan {
+    Kernel kernel;
     int64_t pitch;
     bool copies;
-    size_t w_at, x_at, bytes;
+    size_t x_at, bytes;
 };
 Plan plan(const Int8ProductArgs &a) {
     Plan k{};
-    k.pitch = round_up(a.in, 16);
-    k.copies = a.in % 16 != 0;
+    k.kernel = choose(a);
+    k.copies = a.in % 16 != 0 && k.kernel != DIRECT;
+    k.pitch = k.copies ? round_up(a.in, 16) : a.in;
     if (k.copies) {
         k.x_at = round_up(a.out * k.pitch, 256);
         k.bytes = k.x_at + a.rows * k.pitch;
     }
     return k;
+}
+
+template <typename T, int MF> hipError_t launch_direct(Product &p, const int8_t *x, const int8_t *w, int K, hipStream_t s) {
+    p.tiles_r = (int)ceil_div(p.rows, 16 * MF);
+    p.tiles_c = (int)ceil_div(p.cols, 16);
+    const auto kernel = K % 16 == 0 ? direct_product_kernel<T, MF, true> : direct_product_kernel<T, MF, false>;
+    kernel<<<(unsigned)(p.tiles_r * p.tiles_c), TB, 0, s>>>(p, x, w, K);
+    return hipGetLastError();
+}
+
+template <typename T> hipError_t launch_one(Kernel kernel, Product &p, const int8_t *x, const int8_t *w, int K, hipStream_t s) {
+    switch (kernel) {
+        case WIDE: return launch_wide<T, false, false, 4, Codes>(p, s);
+        case HALF: return launch_wide<T, false, false, 2, Codes>(p, s);
+        case BIG: return launch_tiles<T, false, false, 2, 2, 4, 4, 2, 2, Codes>(p, s);
+        case SMALL: return launch_tiles<T, false, false, 2, 2, 2, 2, 3, 2, Codes>(p, s);
+        default: return p.rows <= 16 ? launch_direct<T, 1>(p, x, w, K, s) : launch_direct<T, 4>(p, x, w, K, s);
+    }
 }
 
 template <typename T> hipError_t product(const Int8ProductArgs &a, hipStream_t s) {
@@ -72,22 +216,14 @@ template <typename T> hipError_t product(const Int8ProductArgs &a, hipStream_t s
     p.act = a.act;
     p.scale_c = a.weight_scales;
     // rows in runs whose workgroups HIP takes in one launch
-    const int64_t run = (int64_t)(1 << 22) / ceil_div(a.out, 64) * 64;
+    const int64_t run = (int64_t)(1 << 21) / ceil_div(a.out, 64) * 64;
     for (int64_t first = 0; first < a.rows; first += run) {
         p.rows = (int)std::min(a.rows - first, run);
         p.R = {x + first * k.pitch, half, p.rows * half, half, p.rows};
         p.out = (T *)a.y + first * a.out;
         p.residual = a.residual ? (const T *)a.residual + first * a.out : nullptr;
         p.scale_r = a.scales + first;
-        const double steps = (double)ceil_div(half, 64);
-        auto tiles = [&](int r, int c) { return ceil_div(p.rows, r) * ceil_div(p.cols, c); };
-        hipError_t e;
-        (void)steps;
-        if (p.cols % 8 == 0 && tiles(256, 256) >= 256) e = launch_wide<T, false, false, 4, Codes>(p, s);
-        else if (p.cols % 8 == 0 && tiles(256, 128) >= 256) e = launch_wide<T, false, false, 2, Codes>(p, s);
-        else if (tiles(128, 128) >= 512) e = launch_tiles<T, false, false, 2, 2, 4, 4, 2, 2, Codes>(p, s);
-        else e = launch_tiles<T, false, false, 2, 2, 2, 2, 3, 2, Codes>(p, s);
-        if (e) return e;
+        if (hipError_t e = launch_one<T>(k.kernel, p, x + first * k.pitch, w, (int)k.pitch, s)) return e;
     }
     return hipSuccess;
 }

@@ -425,8 +425,8 @@ template <bool TM, bool PERM, int ES> struct SubTile {
 
 // The results of a tile of 256 rows: acc[i][j] are the fragments of columns i and rows j, `first` + 32 j this lane's rows, col0 its
 // wave's first column, q its quarter of a fragment's columns.
-template <typename T, bool CT, int FC, typename Sum>
-__device__ __forceinline__ void store_results(const Product &p, const Sum (&acc)[FC][8], int split, int first, int col0, int q) {
+template <typename T, bool CT, int FC>
+__device__ __forceinline__ void store_results(const Product &p, const fvec4 (&acc)[FC][8], int split, int first, int col0, int q) {
             // Results: a lane's columns are the same in all its rows. What is read on the way comes ahead of its use: the bias once,
             // the residual a row ahead of the stores.
             constexpr int RUN = CT ? 4 : 8, RUNS = 4 * FC / RUN;
@@ -445,18 +445,6 @@ __device__ __forceinline__ void store_results(const Product &p, const Sum (&acc)
                 for (int r = 0; r < RUNS; ++r)
                     if (col_of(r) < p.cols) bias[r] = *reinterpret_cast<const Run *>((const T *)p.bias + col_of(r));
             if (p.residual) residual(first);
-            constexpr bool CODES = std::is_same<Sum, i32x4>::value;
-            float scale[CODES ? RUNS : 1][RUN], scale_r[CODES ? 8 : 1];
-            if constexpr (CODES) {
-#pragma unroll
-                for (int r = 0; r < RUNS; ++r) {
-                    const int col = col_of(r) < p.cols ? col_of(r) : 0;
-#pragma unroll
-                    for (int e = 0; e < RUN; ++e) scale[r][e] = p.scale_c[col + e];
-                }
-#pragma unroll
-                for (int j = 0; j < 8; ++j) scale_r[j] = p.scale_r[first + j * 32 < p.rows ? first + j * 32 : 0];
-            }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int row = first + j * 32;
@@ -470,9 +458,6 @@ __device__ __forceinline__ void store_results(const Product &p, const Sum (&acc)
                     float v[RUN];
 #pragma unroll
                     for (int e = 0; e < RUN; ++e) v[e] = CT ? acc[r][j][e] : acc[r * 2 + e / 4][j][e % 4];
-                    if constexpr (CODES)
-#pragma unroll
-                        for (int e = 0; e < RUN; ++e) v[e] = v[e] * scale_r[j] * scale[r][e];
                     if (row >= p.rows || col >= p.cols) continue;
                     const int64_t at_o = (int64_t)row * p.cols + col;
                     if (p.sums) {
@@ -498,6 +483,65 @@ __device__ __forceinline__ void store_results(const Product &p, const Sum (&acc)
                     *reinterpret_cast<Run *>((T *)p.out + at_o) = o;
                 }
             }
+}
+
+// The same of 8-bit operands, scaled by row and column. Their products take half the time, so what is read on the way weighs
+// twice: everything is asked for at once, the residual AHEAD rows before its use.
+// row0, col0: the tile's (uniform) first row and column; lane_row, lane_col: from there to the lane's first.
+template <typename T, int FC>
+__device__ __forceinline__ void store_scaled(const Product &p, const i32x4 (&acc)[FC][8], int row0, int col0, int lane_row, int lane_col) {
+    constexpr int RUN = 8, RUNS = FC / 2, AHEAD = 2;
+    typedef Pack<T, RUN> Run;
+    typedef Pack<float, RUN> Scales;
+    const int rows = p.rows - row0 - lane_row, cols = p.cols - col0 - lane_col;   // from the lane's first to the edge
+    const uint32_t off = (uint32_t)lane_row * (uint32_t)p.cols + (uint32_t)lane_col;
+    const int64_t origin = (int64_t)row0 * p.cols + col0;
+    Run bias[RUNS] = {}, ahead[AHEAD][RUNS] = {};
+    Scales scale[RUNS];
+    float scale_r[8];
+    auto residual = [&](int j) {
+        const T *from = (const T *)p.residual + origin + (int64_t)j * 32 * p.cols;
+#pragma unroll
+        for (int r = 0; r < RUNS; ++r)
+            if (j * 32 < rows && r * 32 < cols) ahead[j % AHEAD][r] = *reinterpret_cast<const Run *>(from + (off + r * 32));
+    };
+#pragma unroll
+    for (int j = 0; j < 8; ++j) scale_r[j] = p.scale_r[row0 + (j * 32 < rows ? lane_row + j * 32 : 0)];
+#pragma unroll
+    for (int r = 0; r < RUNS; ++r) scale[r] = *reinterpret_cast<const Scales *>(p.scale_c + col0 + (r * 32 < cols ? lane_col + r * 32 : 0));
+    if (p.bias)
+#pragma unroll
+        for (int r = 0; r < RUNS; ++r)
+            if (r * 32 < cols) bias[r] = *reinterpret_cast<const Run *>((const T *)p.bias + col0 + (lane_col + r * 32));
+    if (p.residual)
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) residual(j);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        T *to = (T *)p.out + origin + (int64_t)j * 32 * p.cols;
+        Run res[RUNS];
+#pragma unroll
+        for (int r = 0; r < RUNS; ++r) res[r] = ahead[j % AHEAD][r];
+        if (p.residual && j + AHEAD < 8) residual(j + AHEAD);
+#pragma unroll
+        for (int r = 0; r < RUNS; ++r) {
+            float v[RUN];
+#pragma unroll
+            for (int e = 0; e < RUN; ++e) v[e] = (float)acc[r * 2 + e / 4][j][e % 4] * scale_r[j] * scale[r].v[e];
+            if (p.bias)
+#pragma unroll
+                for (int e = 0; e < RUN; ++e) v[e] += (float)bias[r].v[e];
+            act_values<is_f32<T>(), RUN>(v, p.act);
+            if (p.residual)
+#pragma unroll
+                for (int e = 0; e < RUN; ++e) v[e] += (float)res[r].v[e];
+            Run o;
+#pragma unroll
+            for (int e = 0; e < RUN; ++e) o.v[e] = (T)v[e];
+            if (j * 32 < rows && r * 32 < cols) *reinterpret_cast<Run *>(to + (off + r * 32)) = o;
+        }
+        __builtin_amdgcn_sched_barrier(0);   // (a row's values at a time: more at once do not fit the registers)
+    }
 }
 
 // A workgroup's tiles: the XCD's run of neighbouring ones (columns first), its workgroups in turn
@@ -689,7 +733,10 @@ __global__ void __launch_bounds__(512, 2) wide_product_kernel(Product p) {
             phase(std::integral_constant<int, 3>());
         }
         if (!wr) asm volatile("s_barrier" ::: "memory");   // level again
-        store_results<T, CT, FC>(p, acc, tile.split, tile.row0 + wr * 16 + (lane & 15), tile.col0 + wc * 16 * FC, lane >> 4);
+        if constexpr (std::is_same<E, Codes>::value)
+            store_scaled<T, FC>(p, acc, tile.row0, tile.col0, wr * 16 + (lane & 15), wc * 16 * FC + (lane >> 4) * 8);
+        else
+            store_results<T, CT, FC>(p, acc, tile.split, tile.row0 + wr * 16 + (lane & 15), tile.col0 + wc * 16 * FC, lane >> 4);
         // the loads' counts above are of loads alone
         asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
     }
