@@ -7,11 +7,12 @@
 //
 // Bound by memory: a row stays in registers between the sums over it and its results, so every value is read once and written
 // once. Rows are laid over as few lanes as hold them (a power of two, up to a wave, N accesses of 16 bytes each: several short
-// rows to a wave), rows beyond a wave's registers over a workgroup, rows beyond that are read twice. Rows whose size is no
-// multiple of 16 bytes are read and written by the same accesses, unaligned, and by single values at their ends.
+// rows to a wave), rows beyond a wave's registers over a workgroup, rows beyond that are read twice.
+// (Rows that end within an access: Fit, below.)
 //
 // Sums are float32, in a fixed order. Squares beyond float32 are summed again at 2^-140 of their size.
 #include <algorithm>
+#include <type_traits>
 
 #include "rows.h"
 
@@ -20,59 +21,84 @@ namespace {
 
 constexpr int TB = 256;
 constexpr int HELD = 4;         // accesses of a lane that holds its part of a long row
-constexpr int MOST_TB = 1024;
-constexpr int GRAD_TB = 512;    // backward: three maps and the weight's gradient are held (at 1024 lanes they do not fit)
+constexpr int HELD_TB = 512;    // lanes that hold a long row (at 1024 there are registers for less than their accesses)
+constexpr int LONG_TB = 1024;   // lanes that read a longer one in turn
 constexpr float LEAST_SCALE = 1.1754943508222875e-38f;   // 2^-126
 constexpr float MOST_SCALE = 2.6793883890187504e+36f;     // 127 of it are finite
 
 template <typename T> constexpr int vec() { return 16 / (int)sizeof(T); }
 
-// N elements at any address that their type allows
-template <typename T, int N> struct __attribute__((packed, aligned(sizeof(T)))) Loose {
+// How a row's accesses of VEC = 16 / sizeof(T) elements lie: WHOLE rows are made of whole ones, aligned; a LOOSE row's last one ends
+// with the row and repeats elements of the one before it, which count once in the row's sums and are stored twice, the same
+// (unaligned); TINY rows are shorter than one, and read and written by single elements.
+enum Fit { WHOLE, LOOSE, TINY };
+
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+template <typename T, int N> struct __attribute__((packed, aligned(sizeof(T)))) Unaligned {
     T v[N];
 };
+template <typename T> struct Values {
+    T v[vec<T>()];
+};
 
-// VEC elements of a row, of which `left` are in it: WHOLE rows are made of whole accesses
-template <typename T, int VEC, bool WHOLE> __device__ __forceinline__ void load(const T *p, int left, T *o) {
-    if constexpr (WHOLE) {
-        Pack<T, VEC> k{};
-        if (left > 0) k = *reinterpret_cast<const Pack<T, VEC> *>(p);
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) o[v] = k.v[v];
-    } else if (left >= VEC) {
-        const Loose<T, VEC> k = *reinterpret_cast<const Loose<T, VEC> *>(p);
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) o[v] = k.v[v];
+// A lane's access i of a row: its first element, how many of its elements are another access's, whether it has any of its own
+template <typename T, int FIT> struct Place {
+    int c, over;
+    bool on;
+    __device__ __forceinline__ Place(int i, int C) {
+        constexpr int VEC = vec<T>();
+        const int at = i * VEC;
+        on = at < C;
+        c = FIT == LOOSE ? min(at, C - VEC) : at;
+        over = FIT == LOOSE ? at - c : 0;
+    }
+    __device__ __forceinline__ bool own(int v) const { return FIT != LOOSE || v >= over; }
+};
+
+// (outside the row: zeros, or what another access has)
+template <typename T, int FIT> __device__ __forceinline__ u32x4 load(const T *row, const Place<T, FIT> &k, int C) {
+    if constexpr (FIT == WHOLE) {
+        return k.on ? *reinterpret_cast<const u32x4 *>(row + k.c) : u32x4{0, 0, 0, 0};
+    } else if constexpr (FIT == LOOSE) {
+        return __builtin_bit_cast(u32x4, *reinterpret_cast<const Unaligned<T, vec<T>()> *>(row + k.c));
     } else {
+        Values<T> o{};
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) o[v] = v < left ? p[v] : (T)0;
+        for (int v = 0; v < vec<T>() - 1; ++v)
+            if (k.c + v < C) o.v[v] = row[k.c + v];
+        return __builtin_bit_cast(u32x4, o);
     }
 }
-template <typename T, int VEC, bool WHOLE> __device__ __forceinline__ void store(T *p, int left, const T *o) {
-    if constexpr (WHOLE) {
-        Pack<T, VEC> k;
+template <typename T, int FIT, typename D> __device__ __forceinline__ void store(D *row, const Place<T, FIT> &k, int C, const D *o) {
+    constexpr int VEC = vec<T>();
+    if (!k.on) return;
+    if constexpr (FIT == WHOLE) {
+        Pack<D, VEC> p;
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) k.v[v] = o[v];
-        if (left > 0) *reinterpret_cast<Pack<T, VEC> *>(p) = k;
-    } else if (left >= VEC) {
-        Loose<T, VEC> k;
+        for (int v = 0; v < VEC; ++v) p.v[v] = o[v];
+        *reinterpret_cast<Pack<D, VEC> *>(row + k.c) = p;
+    } else if constexpr (FIT == LOOSE) {
+        Unaligned<D, VEC> p;
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) k.v[v] = o[v];
-        *reinterpret_cast<Loose<T, VEC> *>(p) = k;
+        for (int v = 0; v < VEC; ++v) p.v[v] = o[v];
+        *reinterpret_cast<Unaligned<D, VEC> *>(row + k.c) = p;
     } else {
 #pragma unroll
-        for (int v = 0; v < VEC; ++v)
-            if (v < left) p[v] = o[v];
+        for (int v = 0; v < VEC - 1; ++v)
+            if (k.c + v < C) row[k.c + v] = o[v];
     }
 }
-template <typename T, int VEC> __device__ __forceinline__ void widen(const T *o, float *f) {
+template <typename T> __device__ __forceinline__ void widen(const u32x4 &raw, float *f) {
+    const Values<T> o = __builtin_bit_cast(Values<T>, raw);
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) f[v] = (float)o[v];
+    for (int v = 0; v < vec<T>(); ++v) f[v] = (float)o.v[v];
 }
-template <typename T, int VEC> __device__ __forceinline__ void narrow(const float *f, T *o) {
+template <typename T> __device__ __forceinline__ void narrow(const float *f, T *o) {
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) o[v] = (T)f[v];
+    for (int v = 0; v < vec<T>(); ++v) o[v] = (T)f[v];
 }
+// x as it is now: what is made of it from here on is made again, not kept from before
+__device__ __forceinline__ void anew(u32x4 &x) { asm volatile("" : "+v"(x)); }
 
 // The lanes of a row: 2^log2 of a wave, or a whole workgroup (`red`: a word per wave)
 struct Add {
@@ -141,77 +167,79 @@ struct RowKernelArgs {
     int8_t *codes;
 };
 
-template <typename T, int VEC> __device__ __forceinline__ void add_in_type(float *f, const T *r, T *sum) {
+// f += r, rounded to the type, which `sum` receives
+template <typename T> __device__ __forceinline__ void add_in_type(float *f, const u32x4 &r, T *sum) {
+    float g[vec<T>()];
+    widen<T>(r, g);
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-        sum[v] = (T)(f[v] + (float)r[v]);
+    for (int v = 0; v < vec<T>(); ++v) {
+        sum[v] = (T)(f[v] + g[v]);
         f[v] = (float)sum[v];
     }
 }
 
-// A lane has N accesses of a row, LANES apart. BLOCK: a workgroup's lanes, otherwise 2^log2 of a wave.
-template <typename T, int N, bool WHOLE, int MODE, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? MOST_TB : TB) row_kernel(RowKernelArgs a) {
+// A lane has N accesses of a row. BLOCK: a row is a workgroup's, otherwise 2^log2 lanes of a wave's. The next row's loads are on
+// their way while a row is worked on.
+template <typename T, int N, int FIT, int MODE, bool BLOCK>
+__global__ void __launch_bounds__(BLOCK ? HELD_TB : TB) row_kernel(RowKernelArgs a) {
     constexpr int VEC = vec<T>();
-    __shared__ float red[BLOCK ? MOST_TB / 64 : 1];
+    __shared__ float red[BLOCK ? HELD_TB / 64 : 1];
     const int t = threadIdx.x, C = a.channels;
     const int lanes = BLOCK ? (int)blockDim.x : 1 << a.log2, l = t & (lanes - 1);
     const int per = BLOCK ? 1 : TB >> a.log2;   // rows of a workgroup
+    const bool added = MODE != QUANTIZE && a.residual;
+    auto place = [&](int n) { return Place<T, FIT>(n * lanes + l, C); };
     float w[N][VEC];
     if constexpr (MODE != QUANTIZE)
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int c = (n * lanes + l) * VEC;
             if (a.weight) {
-                T o[VEC];
-                load<T, VEC, WHOLE>((const T *)a.weight + c, C - c, o);
-                widen<T, VEC>(o, w[n]);
+                widen<T>(load<T, FIT>((const T *)a.weight, place(n), C), w[n]);
             } else {
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) w[n][v] = 1.f;
             }
         }
-    for (int64_t row = (int64_t)blockIdx.x * per + (BLOCK ? 0 : t >> a.log2); row < a.rows; row += (int64_t)gridDim.x * per) {
+    u32x4 x[N], r[N];
+    auto fetch = [&](int64_t row) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) x[n] = load<T, FIT>((const T *)a.x + row * C, place(n), C);
+        if (added)
+#pragma unroll
+            for (int n = 0; n < N; ++n) r[n] = load<T, FIT>((const T *)a.residual + row * C, place(n), C);
+    };
+    const int64_t stride = (int64_t)gridDim.x * per;
+    int64_t row = (int64_t)blockIdx.x * per + (BLOCK ? 0 : t >> a.log2);
+    if (row < a.rows) fetch(row);
+    for (; row < a.rows; row += stride) {
         const int64_t at = row * C;
-        T x[N][VEC], r[N][VEC];
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int c = (n * lanes + l) * VEC;
-            load<T, VEC, WHOLE>((const T *)a.x + at + c, C - c, x[n]);
-        }
-        if (MODE != QUANTIZE && a.residual)
-#pragma unroll
-            for (int n = 0; n < N; ++n) {
-                const int c = (n * lanes + l) * VEC;
-                load<T, VEC, WHOLE>((const T *)a.residual + at + c, C - c, r[n]);
-            }
         float f[N][VEC];
 #pragma unroll
-        for (int n = 0; n < N; ++n) widen<T, VEC>(x[n], f[n]);
+        for (int n = 0; n < N; ++n) {
+            widen<T>(x[n], f[n]);
+            if (added) {
+                T sum[VEC];
+                add_in_type<T>(f[n], r[n], sum);
+                store<T, FIT>((T *)a.sum + at, place(n), C, sum);
+            }
+        }
+        if (row + stride < a.rows) fetch(row + stride);
         if constexpr (MODE != QUANTIZE) {
-            if (a.residual)
-#pragma unroll
-                for (int n = 0; n < N; ++n) {
-                    const int c = (n * lanes + l) * VEC;
-                    add_in_type<T, VEC>(f[n], r[n], x[n]);
-                    store<T, VEC, WHOLE>((T *)a.sum + at + c, C - c, x[n]);
-                }
-            float ss = 0.f;
-#pragma unroll
-            for (int n = 0; n < N; ++n)
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) ss = fmaf(f[n][v], f[n][v], ss);
-            ss = over_row<Add, BLOCK>(ss, a.log2, red);
-            float rstd = 1.f / sqrtf(fmaf(ss, a.inv_channels, a.eps));
-            if (is_infinite(ss)) {   // (the same for all lanes of the row)
-                ss = 0.f;
+            auto squares = [&](float down) {
+                float ss = 0.f;
 #pragma unroll
                 for (int n = 0; n < N; ++n)
 #pragma unroll
-                    for (int v = 0; v < VEC; ++v) ss = fmaf(f[n][v] * DOWN, f[n][v] * DOWN, ss);
-                ss = over_row<Add, BLOCK>(ss, a.log2, red);
-                rstd = DOWN / sqrtf(fmaf(ss, a.inv_channels, a.eps * DOWN2));
-            }
+                    for (int v = 0; v < VEC; ++v) {
+                        const float s = place(n).own(v) ? f[n][v] * down : 0.f;
+                        ss = fmaf(s, s, ss);
+                    }
+                return over_row<Add, BLOCK>(ss, a.log2, red);
+            };
+            const float ss = squares(1.f);
+            float rstd = 1.f / sqrtf(fmaf(ss, a.inv_channels, a.eps));
+            if (is_infinite(ss))   // (the same for all lanes of the row)
+                rstd = DOWN / sqrtf(fmaf(squares(DOWN), a.inv_channels, a.eps * DOWN2));
             if (a.rstd && l == 0) a.rstd[row] = rstd;
 #pragma unroll
             for (int n = 0; n < N; ++n)
@@ -221,123 +249,130 @@ __global__ void __launch_bounds__(BLOCK ? MOST_TB : TB) row_kernel(RowKernelArgs
         if constexpr (MODE == NORM) {
 #pragma unroll
             for (int n = 0; n < N; ++n) {
-                const int c = (n * lanes + l) * VEC;
                 T o[VEC];
-                narrow<T, VEC>(f[n], o);
-                store<T, VEC, WHOLE>((T *)a.y + at + c, C - c, o);
+                narrow<T>(f[n], o);
+                store<T, FIT>((T *)a.y + at, place(n), C, o);
             }
         } else {
-            float big = 0.f;   // (beyond the row's end: zeros)
+            float big = 0.f;   // (outside the row: zeros, another access's values, or NaN as all of the row)
 #pragma unroll
             for (int n = 0; n < N; ++n)
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) big = Most::of(big, (n * lanes + l) * VEC + v < C ? fabsf(f[n][v]) : 0.f);
+                for (int v = 0; v < VEC; ++v) big = Most::of(big, fabsf(f[n][v]));
             const float scale = scale_of(over_row<Most, BLOCK>(big, a.log2, red));
             if (l == 0) a.scales[row] = scale;
 #pragma unroll
             for (int n = 0; n < N; ++n) {
-                const int c = (n * lanes + l) * VEC;
                 int8_t q[VEC] = {};
                 if (scale == scale) codes_of<VEC>(f[n], scale, q);
-                store<int8_t, VEC, WHOLE>(a.codes + at + c, C - c, q);
+                store<T, FIT>(a.codes + at, place(n), C, q);
             }
         }
     }
 }
 
 // Rows beyond a workgroup's registers: read once for the sums (and written as the sum), once more for each result that needs them
-template <typename T, bool WHOLE, int MODE> __global__ void __launch_bounds__(MOST_TB) long_row_kernel(RowKernelArgs a) {
+template <typename T, int FIT, int MODE> __global__ void __launch_bounds__(LONG_TB) long_row_kernel(RowKernelArgs a) {
     constexpr int VEC = vec<T>();
-    __shared__ float red[MOST_TB / 64];
+    __shared__ float red[LONG_TB / 64];
     const int t = threadIdx.x, C = a.channels;
     const bool added = MODE != QUANTIZE && a.residual;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const int64_t at = row * C;
-        auto values = [&](int c, float *f, bool write) {
-            T x[VEC], r[VEC];
-            load<T, VEC, WHOLE>((const T *)a.x + at + c, C - c, x);
-            widen<T, VEC>(x, f);
+        auto values = [&](const Place<T, FIT> &k, float *f, bool write) {
+            widen<T>(load<T, FIT>((const T *)a.x + at, k, C), f);
             if (!added) return;
-            load<T, VEC, WHOLE>((const T *)a.residual + at + c, C - c, r);
-            add_in_type<T, VEC>(f, r, x);
-            if (write) store<T, VEC, WHOLE>((T *)a.sum + at + c, C - c, x);
+            T sum[VEC];
+            add_in_type<T>(f, load<T, FIT>((const T *)a.residual + at, k, C), sum);
+            if (write) store<T, FIT>((T *)a.sum + at, k, C, sum);
         };
         float rstd = 1.f;
         if constexpr (MODE != QUANTIZE) {
-            float ss = 0.f;
-            for (int c = t * VEC; c < C; c += MOST_TB * VEC) {
-                float f[VEC];
-                values(c, f, true);
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) ss = fmaf(f[v], f[v], ss);
-            }
-            ss = over_row<Add, true>(ss, 6, red);
-            rstd = 1.f / sqrtf(fmaf(ss, a.inv_channels, a.eps));
-            if (is_infinite(ss)) {
-                ss = 0.f;
-                for (int c = t * VEC; c < C; c += MOST_TB * VEC) {
+            auto squares = [&](float down) {
+                float ss = 0.f;
+                for (int i = t; i * VEC < C; i += LONG_TB) {
+                    const Place<T, FIT> k(i, C);
                     float f[VEC];
-                    values(c, f, false);
+                    values(k, f, down == 1.f);
 #pragma unroll
-                    for (int v = 0; v < VEC; ++v) ss = fmaf(f[v] * DOWN, f[v] * DOWN, ss);
+                    for (int v = 0; v < VEC; ++v) {
+                        const float s = k.own(v) ? f[v] * down : 0.f;
+                        ss = fmaf(s, s, ss);
+                    }
                 }
-                ss = over_row<Add, true>(ss, 6, red);
-                rstd = DOWN / sqrtf(fmaf(ss, a.inv_channels, a.eps * DOWN2));
-            }
+                return over_row<Add, true>(ss, 6, red);
+            };
+            const float ss = squares(1.f);
+            rstd = 1.f / sqrtf(fmaf(ss, a.inv_channels, a.eps));
+            if (is_infinite(ss)) rstd = DOWN / sqrtf(fmaf(squares(DOWN), a.inv_channels, a.eps * DOWN2));
             if (a.rstd && t == 0) a.rstd[row] = rstd;
         }
-        auto result = [&](int c, float *f) {
-            values(c, f, false);
+        auto result = [&](const Place<T, FIT> &k, float *f) {
+            values(k, f, false);
             if constexpr (MODE != QUANTIZE) {
-                T o[VEC];
-                if (a.weight) load<T, VEC, WHOLE>((const T *)a.weight + c, C - c, o);
+                float w[VEC];
+                if (a.weight) widen<T>(load<T, FIT>((const T *)a.weight, k, C), w);
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) f[v] = f[v] * rstd * (a.weight ? (float)o[v] : 1.f);
+                for (int v = 0; v < VEC; ++v) f[v] = f[v] * rstd * (a.weight ? w[v] : 1.f);
             }
         };
         if constexpr (MODE == NORM) {
-            for (int c = t * VEC; c < C; c += MOST_TB * VEC) {
+            for (int i = t; i * VEC < C; i += LONG_TB) {
+                const Place<T, FIT> k(i, C);
                 float f[VEC];
                 T o[VEC];
-                result(c, f);
-                narrow<T, VEC>(f, o);
-                store<T, VEC, WHOLE>((T *)a.y + at + c, C - c, o);
+                result(k, f);
+                narrow<T>(f, o);
+                store<T, FIT>((T *)a.y + at, k, C, o);
             }
         } else {
             float big = 0.f;
-            for (int c = t * VEC; c < C; c += MOST_TB * VEC) {
+            for (int i = t; i * VEC < C; i += LONG_TB) {
                 float f[VEC];
-                result(c, f);
+                result(Place<T, FIT>(i, C), f);
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) big = Most::of(big, c + v < C ? fabsf(f[v]) : 0.f);
+                for (int v = 0; v < VEC; ++v) big = Most::of(big, fabsf(f[v]));
             }
             const float scale = scale_of(over_row<Most, true>(big, 6, red));
             if (t == 0) a.scales[row] = scale;
-            for (int c = t * VEC; c < C; c += MOST_TB * VEC) {
+            for (int i = t; i * VEC < C; i += LONG_TB) {
+                const Place<T, FIT> k(i, C);
                 float f[VEC];
                 int8_t q[VEC] = {};
-                result(c, f);
+                result(k, f);
                 if (scale == scale) codes_of<VEC>(f, scale, q);
-                store<int8_t, VEC, WHOLE>(a.codes + at + c, C - c, q);
+                store<T, FIT>(a.codes + at, k, C, q);
             }
         }
     }
 }
 
-template <typename T, bool WHOLE>
+template <typename T, int FIT>
 __global__ void __launch_bounds__(TB) dequantize_kernel(int64_t rows, int C, int log2, const int8_t *__restrict__ codes,
                                                         const float *__restrict__ scales, T *__restrict__ y) {
     constexpr int VEC = vec<T>();
     const int lanes = 1 << log2, l = threadIdx.x & (lanes - 1), per = TB >> log2;
     for (int64_t row = (int64_t)blockIdx.x * per + (threadIdx.x >> log2); row < rows; row += (int64_t)gridDim.x * per) {
         const float scale = scales[row];
-        for (int c = l * VEC; c < C; c += lanes * VEC) {
-            int8_t q[VEC];
-            T o[VEC];
-            load<int8_t, VEC, WHOLE>(codes + row * C + c, C - c, q);
+        const int8_t *from = codes + row * C;
+        for (int i = l; i * VEC < C; i += lanes) {
+            const Place<T, FIT> k(i, C);
+            Unaligned<int8_t, VEC> q{};
+            if constexpr (FIT == WHOLE) {
+                const Pack<int8_t, VEC> p = *reinterpret_cast<const Pack<int8_t, VEC> *>(from + k.c);
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) o[v] = (T)((float)q[v] * scale);
-            store<T, VEC, WHOLE>(y + row * C + c, C - c, o);
+                for (int v = 0; v < VEC; ++v) q.v[v] = p.v[v];
+            } else if constexpr (FIT == LOOSE) {
+                q = *reinterpret_cast<const Unaligned<int8_t, VEC> *>(from + k.c);
+            } else {
+#pragma unroll
+                for (int v = 0; v < VEC - 1; ++v)
+                    if (k.c + v < C) q.v[v] = from[k.c + v];
+            }
+            T o[VEC];
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) o[v] = (T)((float)q.v[v] * scale);
+            store<T, FIT>(y + row * C, k, C, o);
         }
     }
 }
@@ -351,73 +386,86 @@ struct RowGradKernelArgs {
     const void *dy, *dsum, *x, *weight;
     const float *rstd;
     void *dx;
-    float *part;   // [workgroups][channels], or null
+    float *part;     // [workgroups][channels], or null
+    void *dweight;   // the weight's gradient itself, where one workgroup has all rows; or null
 };
 
-template <typename T, int N, bool WHOLE, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? GRAD_TB : TB) row_grad_kernel(RowGradKernelArgs a) {
+// Maps stay as they were read, in the map's type: the second use widens them again, since as float32 a long row of a 16-bit map
+// would fill the registers (65536 x 2048: 292 us so, two waves to a SIMD).
+template <typename T, int N, int FIT, bool BLOCK>
+__global__ void __launch_bounds__(BLOCK ? HELD_TB : TB) row_grad_kernel(RowGradKernelArgs a) {
     constexpr int VEC = vec<T>();
     extern __shared__ float shared[];   // BLOCK: a word per wave; otherwise [waves][lanes * N * VEC]
     const int t = threadIdx.x, C = a.channels;
     const int lanes = BLOCK ? (int)blockDim.x : 1 << a.log2, l = t & (lanes - 1);
     const int per = BLOCK ? 1 : TB >> a.log2;
-    float w[N][VEC], dw[N][VEC];
+    auto place = [&](int n) { return Place<T, FIT>(n * lanes + l, C); };
+    u32x4 w[N];
+    float dw[N][VEC];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-        const int c = (n * lanes + l) * VEC;
-        T o[VEC];
-        if (a.weight) load<T, VEC, WHOLE>((const T *)a.weight + c, C - c, o);
+        if (a.weight) w[n] = load<T, FIT>((const T *)a.weight, place(n), C);
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) w[n][v] = a.weight ? (float)o[v] : 1.f, dw[n][v] = 0.f;
+        for (int v = 0; v < VEC; ++v) dw[n][v] = 0.f;
     }
+    auto weights = [&](int n, float *f) {
+        if (a.weight) {
+            widen<T>(w[n], f);
+        } else {
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) f[v] = 1.f;
+        }
+    };
     for (int64_t row = (int64_t)blockIdx.x * per + (BLOCK ? 0 : t >> a.log2); row < a.rows; row += (int64_t)gridDim.x * per) {
         const int64_t at = row * C;
-        T x[N][VEC], dy[N][VEC], ds[N][VEC];
+        u32x4 x[N], dy[N], ds[N];
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int c = (n * lanes + l) * VEC;
-            load<T, VEC, WHOLE>((const T *)a.x + at + c, C - c, x[n]);
-            load<T, VEC, WHOLE>((const T *)a.dy + at + c, C - c, dy[n]);
+            x[n] = load<T, FIT>((const T *)a.x + at, place(n), C);
+            dy[n] = load<T, FIT>((const T *)a.dy + at, place(n), C);
         }
         if (a.dsum)
 #pragma unroll
-            for (int n = 0; n < N; ++n) {
-                const int c = (n * lanes + l) * VEC;
-                load<T, VEC, WHOLE>((const T *)a.dsum + at + c, C - c, ds[n]);
-            }
+            for (int n = 0; n < N; ++n) ds[n] = load<T, FIT>((const T *)a.dsum + at, place(n), C);
         const float rstd = a.rstd[row];
-        float h[N][VEC], dh[N][VEC], dot = 0.f;
+        float dot = 0.f;
 #pragma unroll
-        for (int n = 0; n < N; ++n)
+        for (int n = 0; n < N; ++n) {
+            float fx[VEC], fd[VEC], fw[VEC];
+            widen<T>(x[n], fx), widen<T>(dy[n], fd), weights(n, fw);
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
-                const float d = (float)dy[n][v];
-                h[n][v] = (float)x[n][v] * rstd;
-                dh[n][v] = d * w[n][v];
-                dw[n][v] = fmaf(d, h[n][v], dw[n][v]);
-                dot = fmaf(dh[n][v], h[n][v], dot);
+                const float h = fx[v] * rstd;
+                dw[n][v] = fmaf(fd[v], h, dw[n][v]);
+                dot = fmaf(place(n).own(v) ? fd[v] * fw[v] : 0.f, h, dot);
             }
+        }
         if (a.dx) {
             dot = over_row<Add, BLOCK>(dot, a.log2, shared) * a.inv_channels;
 #pragma unroll
             for (int n = 0; n < N; ++n) {
-                const int c = (n * lanes + l) * VEC;
+                if constexpr (N > 1) anew(x[n]), anew(dy[n]), anew(w[n]);
+                float fx[VEC], fd[VEC], fw[VEC], fs[VEC] = {};
+                widen<T>(x[n], fx), widen<T>(dy[n], fd), weights(n, fw);
+                if (a.dsum) widen<T>(ds[n], fs);
                 T o[VEC];
 #pragma unroll
-                for (int v = 0; v < VEC; ++v)
-                    o[v] = (T)fmaf(rstd, fmaf(-h[n][v], dot, dh[n][v]), a.dsum ? (float)ds[n][v] : 0.f);
-                store<T, VEC, WHOLE>((T *)a.dx + at + c, C - c, o);
+                for (int v = 0; v < VEC; ++v) o[v] = (T)fmaf(rstd, fmaf(-(fx[v] * rstd), dot, fd[v] * fw[v]), fs[v]);
+                store<T, FIT>((T *)a.dx + at, place(n), C, o);
             }
         }
     }
-    if (!a.part) return;
-    float *part = a.part + (int64_t)blockIdx.x * C;
+    if (!a.part && !a.dweight) return;
+    auto put = [&](int c, float v) {
+        if (a.dweight) ((T *)a.dweight)[c] = (T)v;
+        else a.part[(int64_t)blockIdx.x * C + c] = v;
+    };
     if constexpr (BLOCK) {
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int c = (n * lanes + l) * VEC;
-            store<float, VEC, false>(part + c, C - c, dw[n]);
-        }
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v)
+                if (place(n).on && place(n).c + v < C) put(place(n).c + v, dw[n][v]);
     } else {
         // the rows that share a wave, then the waves
         const int width = lanes * N * VEC, wave = t >> 6;
@@ -429,50 +477,52 @@ __global__ void __launch_bounds__(BLOCK ? GRAD_TB : TB) row_grad_kernel(RowGradK
 #pragma unroll
                 for (int m = 0; m < 6; ++m)
                     if (m >= a.log2) s += __shfl_xor(s, 1 << m);
-                if ((t & 63) < lanes) shared[wave * width + (n * lanes + l) * VEC + v] = s;
+                if ((t & 63) < lanes && place(n).on) shared[wave * width + place(n).c + v] = s;
             }
         __syncthreads();
         for (int c = t; c < C; c += TB) {
             float s = shared[c];
 #pragma unroll
             for (int k = 1; k < TB / 64; ++k) s += shared[k * width + c];
-            part[c] = s;
+            put(c, s);
         }
     }
 }
 
 // Rows beyond a workgroup's registers: dx row by row in two readings, the weight's gradient column by column
-template <typename T, bool WHOLE> __global__ void __launch_bounds__(MOST_TB) long_row_grad_kernel(RowGradKernelArgs a) {
+template <typename T, int FIT> __global__ void __launch_bounds__(LONG_TB) long_row_grad_kernel(RowGradKernelArgs a) {
     constexpr int VEC = vec<T>();
-    __shared__ float red[MOST_TB / 64];
+    __shared__ float red[LONG_TB / 64];
     const int t = threadIdx.x, C = a.channels;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const int64_t at = row * C;
         const float rstd = a.rstd[row];
-        float dot = 0.f;
-        auto read = [&](int c, float *h, float *dh) {
-            T x[VEC], dy[VEC], w[VEC];
-            load<T, VEC, WHOLE>((const T *)a.x + at + c, C - c, x);
-            load<T, VEC, WHOLE>((const T *)a.dy + at + c, C - c, dy);
-            if (a.weight) load<T, VEC, WHOLE>((const T *)a.weight + c, C - c, w);
+        auto read = [&](const Place<T, FIT> &k, float *h, float *dh) {
+            float w[VEC];
+            widen<T>(load<T, FIT>((const T *)a.x + at, k, C), h);
+            widen<T>(load<T, FIT>((const T *)a.dy + at, k, C), dh);
+            if (a.weight) widen<T>(load<T, FIT>((const T *)a.weight, k, C), w);
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) h[v] = (float)x[v] * rstd, dh[v] = (float)dy[v] * (a.weight ? (float)w[v] : 1.f);
+            for (int v = 0; v < VEC; ++v) h[v] *= rstd, dh[v] *= a.weight ? w[v] : 1.f;
         };
-        for (int c = t * VEC; c < C; c += MOST_TB * VEC) {
+        float dot = 0.f;
+        for (int i = t; i * VEC < C; i += LONG_TB) {
+            const Place<T, FIT> k(i, C);
             float h[VEC], dh[VEC];
-            read(c, h, dh);
+            read(k, h, dh);
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) dot = fmaf(dh[v], h[v], dot);
+            for (int v = 0; v < VEC; ++v) dot = fmaf(k.own(v) ? dh[v] : 0.f, h[v], dot);
         }
         dot = over_row<Add, true>(dot, 6, red) * a.inv_channels;
-        for (int c = t * VEC; c < C; c += MOST_TB * VEC) {
-            float h[VEC], dh[VEC];
-            T ds[VEC] = {}, o[VEC];
-            read(c, h, dh);
-            if (a.dsum) load<T, VEC, WHOLE>((const T *)a.dsum + at + c, C - c, ds);
+        for (int i = t; i * VEC < C; i += LONG_TB) {
+            const Place<T, FIT> k(i, C);
+            float h[VEC], dh[VEC], ds[VEC] = {};
+            T o[VEC];
+            read(k, h, dh);
+            if (a.dsum) widen<T>(load<T, FIT>((const T *)a.dsum + at, k, C), ds);
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) o[v] = (T)fmaf(rstd, fmaf(-h[v], dot, dh[v]), (float)ds[v]);
-            store<T, VEC, WHOLE>((T *)a.dx + at + c, C - c, o);
+            for (int v = 0; v < VEC; ++v) o[v] = (T)fmaf(rstd, fmaf(-h[v], dot, dh[v]), ds[v]);
+            store<T, FIT>((T *)a.dx + at, k, C, o);
         }
     }
 }
@@ -518,7 +568,8 @@ struct RowShape {
     int log2, n, threads;
     bool block;
 };
-RowShape row_shape(int channels, int vec, int most) {
+// grad: two accesses of more lanes, where there are as many, leave registers for twice the waves
+RowShape row_shape(int channels, int vec, bool grad) {
     const int packs = (int)ceil_div(channels, vec);
     RowShape k{0, 1, 0, false};
     if (packs <= 64 * HELD) {
@@ -527,31 +578,45 @@ RowShape row_shape(int channels, int vec, int most) {
         return k;
     }
     k.block = true;
-    k.n = HELD;
-    for (k.threads = 128; k.threads < most && k.threads * HELD < packs;) k.threads *= 2;
-    if (k.threads * HELD < packs) k.threads = 0;
+    k.n = grad && packs <= 2 * HELD_TB ? 2 : HELD;
+    for (k.threads = 128; k.threads < HELD_TB && k.threads * k.n < packs;) k.threads *= 2;
+    if (k.threads * k.n < packs) k.threads = 0;
     return k;
 }
 
+// Workgroups of the forward: eight times what is there at once, so that the quick ones go on (65536 x 2048 bfloat16 into 8 bits:
+// 1024 / 2048 / 4096 / 8192 workgroups take 84 / 84 / 80 / 77 us; 131072 x 71 12.5 / 11.8 / 11.6 / 13.2 normalised)
+constexpr int64_t MOST_GROUPS = 8192;
 unsigned row_grid(int64_t units, int64_t most) { return (unsigned)std::min(units, most); }
 
-template <typename T, bool WHOLE, int MODE> hipError_t launch_rows(const RowArgs &a, hipStream_t s) {
-    const RowShape k = row_shape(a.channels, vec<T>(), MOST_TB);
+// calls f with the Fit of rows of this type and length as a constant
+template <typename T, typename F> hipError_t with_fit(int channels, F &&f) {
+    if (channels % vec<T>() == 0) return f(std::integral_constant<int, WHOLE>());
+    if (channels > vec<T>()) return f(std::integral_constant<int, LOOSE>());
+    return f(std::integral_constant<int, TINY>());
+}
+
+template <typename T, int MODE> hipError_t launch_rows(const RowArgs &a, hipStream_t s) {
+    const RowShape k = row_shape(a.channels, vec<T>(), false);
     const RowKernelArgs p{a.rows, a.channels, k.log2, (float)(1.0 / a.channels), a.eps, a.x, a.residual, a.weight,
                           a.sum, a.y, a.rstd, a.scales, a.codes};
-    if (k.block) {
-        if (k.threads) row_kernel<T, HELD, WHOLE, MODE, true><<<row_grid(a.rows, 4096), k.threads, 0, s>>>(p);
-        else long_row_kernel<T, WHOLE, MODE><<<row_grid(a.rows, 1024), MOST_TB, 0, s>>>(p);
+    return with_fit<T>(a.channels, [&](auto fit) {
+        constexpr int FIT = decltype(fit)::value;
+        const unsigned grid = row_grid(ceil_div(a.rows, TB >> k.log2), MOST_GROUPS);
+        if constexpr (FIT == TINY) {
+            row_kernel<T, 1, FIT, MODE, false><<<grid, TB, 0, s>>>(p);
+        } else if (k.block) {
+            if (k.threads) row_kernel<T, HELD, FIT, MODE, true><<<row_grid(a.rows, MOST_GROUPS), k.threads, 0, s>>>(p);
+            else long_row_kernel<T, FIT, MODE><<<row_grid(a.rows, 1024), LONG_TB, 0, s>>>(p);
+        } else if (k.n == 1) {
+            row_kernel<T, 1, FIT, MODE, false><<<grid, TB, 0, s>>>(p);
+        } else if (k.n == 2) {
+            row_kernel<T, 2, FIT, MODE, false><<<grid, TB, 0, s>>>(p);
+        } else {
+            row_kernel<T, HELD, FIT, MODE, false><<<grid, TB, 0, s>>>(p);
+        }
         return hipGetLastError();
-    }
-    const unsigned grid = row_grid(ceil_div(a.rows, TB >> k.log2), 4096);
-    if (k.n == 1) row_kernel<T, 1, WHOLE, MODE, false><<<grid, TB, 0, s>>>(p);
-    else if (k.n == 2) row_kernel<T, 2, WHOLE, MODE, false><<<grid, TB, 0, s>>>(p);
-    else row_kernel<T, HELD, WHOLE, MODE, false><<<grid, TB, 0, s>>>(p);
-    return hipGetLastError();
-}
-template <typename T, int MODE> hipError_t launch_rows(const RowArgs &a, hipStream_t s) {
-    return a.channels % vec<T>() == 0 ? launch_rows<T, true, MODE>(a, s) : launch_rows<T, false, MODE>(a, s);
+    });
 }
 template <int MODE> hipError_t launch_rows(const RowArgs &a, hipStream_t s) {
     if (a.rows == 0) return hipSuccess;
@@ -566,53 +631,54 @@ template <typename T> hipError_t dequantize(int64_t rows, int channels, const in
     int log2 = 0;
     while (log2 < 8 && vec<T>() << log2 < channels) ++log2;
     const unsigned grid = row_grid(ceil_div(rows, TB >> log2), 16384);
-    if (channels % vec<T>() == 0) dequantize_kernel<T, true><<<grid, TB, 0, s>>>(rows, channels, log2, codes, scales, y);
-    else dequantize_kernel<T, false><<<grid, TB, 0, s>>>(rows, channels, log2, codes, scales, y);
-    return hipGetLastError();
+    return with_fit<T>(channels, [&](auto fit) {
+        dequantize_kernel<T, decltype(fit)::value><<<grid, TB, 0, s>>>(rows, channels, log2, codes, scales, y);
+        return hipGetLastError();
+    });
 }
 
-// Workgroups of the backward: each keeps a part of the weight's gradient
+// Workgroups of the backward: each keeps a part of the weight's gradient. One alone writes the gradient itself: where it has up to
+// four rounds of rows, which take less than the launch that would add up the parts.
 int64_t grad_parts(const RowGradArgs &a) {
-    const RowShape k = row_shape(a.channels, a.dtype == TVDCN_DTYPE_FLOAT32 ? 4 : 8, GRAD_TB);
+    const RowShape k = row_shape(a.channels, a.dtype == TVDCN_DTYPE_FLOAT32 ? 4 : 8, true);
     if (k.block && !k.threads) return std::min<int64_t>(a.rows, 256);
-    return k.block ? std::min<int64_t>(a.rows, 1024) : std::min<int64_t>(ceil_div(a.rows, TB >> k.log2), 1024);
+    const int64_t units = k.block ? a.rows : ceil_div(a.rows, TB >> k.log2);
+    // (long rows: the parts of 1024 would be a quarter of what 4096 x 8192 reads and writes)
+    return units > 0 && units <= 4 ? 1 : std::min<int64_t>(units, k.block ? 512 : 1024);
 }
 
-template <typename T, int N, bool WHOLE> hipError_t launch_held_grad(const RowGradKernelArgs &p, unsigned grid, hipStream_t s) {
-    row_grad_kernel<T, N, WHOLE, false><<<grid, TB, (TB / 64) * (N << p.log2) * vec<T>() * 4, s>>>(p);
-    return hipGetLastError();
-}
-
-template <typename T, bool WHOLE> hipError_t launch_grad(const RowGradArgs &a, hipStream_t s) {
-    const RowShape k = row_shape(a.channels, vec<T>(), GRAD_TB);
-    RowGradKernelArgs p{a.rows, a.channels, k.log2, (float)(1.0 / a.channels), a.dy, a.dsum, a.x, a.weight, a.rstd, a.dx,
-                        a.dweight ? a.part : nullptr};
+template <typename T> hipError_t launch_grad(const RowGradArgs &a, hipStream_t s) {
+    const RowShape k = row_shape(a.channels, vec<T>(), true);
     const int64_t parts = grad_parts(a);
-    hipError_t e = hipSuccess;
-    if (a.rows == 0) {
-    } else if (k.block && !k.threads) {
-        if (a.dx) long_row_grad_kernel<T, WHOLE><<<row_grid(a.rows, 1024), MOST_TB, 0, s>>>(p);
-        if (e = hipGetLastError(); e != hipSuccess) return e;
-        if (a.dweight) {
-            const int64_t chunk = ceil_div(a.rows, parts);
+    const bool in_turn = k.block && !k.threads, alone = parts == 1 && !in_turn;
+    RowGradKernelArgs p{a.rows, a.channels, k.log2, (float)(1.0 / a.channels), a.dy, a.dsum, a.x, a.weight, a.rstd, a.dx,
+                        a.dweight && !alone ? a.part : nullptr, alone ? a.dweight : nullptr};
+    const hipError_t e = a.rows == 0 ? hipSuccess : with_fit<T>(a.channels, [&](auto fit) {
+        constexpr int FIT = decltype(fit)::value;
+        const unsigned grid = (unsigned)parts, bytes = (TB / 64) * (k.n << k.log2) * vec<T>() * 4;
+        if constexpr (FIT == TINY) {
+            row_grad_kernel<T, 1, FIT, false><<<grid, TB, bytes, s>>>(p);
+        } else if (in_turn) {
+            if (a.dx) long_row_grad_kernel<T, FIT><<<row_grid(a.rows, 1024), LONG_TB, 0, s>>>(p);
+            if (hipError_t e = hipGetLastError()) return e;
             // (fewer chunks than parts where they do not divide: the rest stand for no rows and are zeros)
-            long_weight_grad_kernel<T><<<dim3((unsigned)ceil_div(a.channels, TB), (unsigned)parts), TB, 0, s>>>(p, chunk);
+            if (a.dweight)
+                long_weight_grad_kernel<T><<<dim3((unsigned)ceil_div(a.channels, TB), grid), TB, 0, s>>>(p, ceil_div(a.rows, parts));
+        } else if (k.block) {
+            const auto kernel = k.n == 2 ? row_grad_kernel<T, 2, FIT, true> : row_grad_kernel<T, HELD, FIT, true>;
+            kernel<<<grid, k.threads, HELD_TB / 64 * 4, s>>>(p);
+        } else if (k.n == 1) {
+            row_grad_kernel<T, 1, FIT, false><<<grid, TB, bytes, s>>>(p);
+        } else if (k.n == 2) {
+            row_grad_kernel<T, 2, FIT, false><<<grid, TB, bytes, s>>>(p);
+        } else {
+            row_grad_kernel<T, HELD, FIT, false><<<grid, TB, bytes, s>>>(p);
         }
-        e = hipGetLastError();
-    } else if (k.block) {
-        row_grad_kernel<T, HELD, WHOLE, true><<<(unsigned)parts, k.threads, GRAD_TB / 64 * 4, s>>>(p);
-        e = hipGetLastError();
-    } else {
-        e = k.n == 1   ? launch_held_grad<T, 1, WHOLE>(p, (unsigned)parts, s)
-            : k.n == 2 ? launch_held_grad<T, 2, WHOLE>(p, (unsigned)parts, s)
-                       : launch_held_grad<T, HELD, WHOLE>(p, (unsigned)parts, s);
-    }
-    if (e != hipSuccess || !a.dweight) return e;
+        return hipGetLastError();
+    });
+    if (e != hipSuccess || !a.dweight || alone) return e;
     row_finish_kernel<T><<<(unsigned)ceil_div(a.channels, 16), FIN, 0, s>>>(a.part, (T *)a.dweight, a.channels, (int)parts);
     return hipGetLastError();
-}
-template <typename T> hipError_t launch_grad(const RowGradArgs &a, hipStream_t s) {
-    return a.channels % vec<T>() == 0 ? launch_grad<T, true>(a, s) : launch_grad<T, false>(a, s);
 }
 
 }  // namespace

@@ -416,10 +416,19 @@ class DropoutFunction : public torch::autograd::Function<DropoutFunction> {
         check_no_tangents(DROPOUT, {g[0]});
         const Tensor none;
         if (!g[0].defined()) return {none, none, none, none};
-        const auto s = ctx->get_saved_variables();
-        static auto op = op_of<Dropout>("tvdcn::seeded_dropout");
-        return {ctx->needs_input_grad(0) ? op.call(g[0], ctx->saved_data["p"].toDouble(), s[0], {}) : none, none, none,
-                wanted(ctx, "residual") ? g[0] : none};
+        Tensor dx;
+        if (ctx->needs_input_grad(0)) {
+            const auto s = ctx->get_saved_variables();
+            const double p = ctx->saved_data["p"].toDouble();
+            if (any_grad({g[0]})) {   // (a graph of the backward is made)
+                static auto op = op_of<Dropout>("tvdcn::seeded_dropout");
+                dx = op.call(g[0], p, s[0], {});
+            } else {
+                at::AutoDispatchBelowADInplaceOrView guard;
+                dx = dropout_op().call(g[0], p, s[0], {});
+            }
+        }
+        return {dx, none, none, wanted(ctx, "residual") ? g[0] : none};
     }
 };
 
