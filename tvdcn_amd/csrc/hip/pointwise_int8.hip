@@ -5,11 +5,11 @@
 // ones. Channels that are no multiple of 16 are copied to rows that are, with zeros behind them. Small products have a kernel of
 // their own, without copies.
 //
-// 8192 x 8192 to 8192 runs at 2570 TOP/s (a plain library product of 8-bit integers: 2150). With few channels the results bound it:
-// 65536 x 2048 to 512 takes 70 us, 86 with a residual and 83 with gelu, of which 53 are products; 65536 x 512 to 2048 108, 175 and
-// 158. A tile's stores, and the residual's loads before them, come from all CUs at about the same time, and nothing overlaps them:
-// two workgroups of 256 x 128 to a CU, one storing while the other multiplies, ran at 1920 TOP/s and were slower throughout (89, 106
-// and 98 us for the former).
+// 8192 x 8192 to 8192 runs at 2590 TOP/s (a plain library product of 8-bit integers: 2150). With few channels the results bound it:
+// 65536 x 2048 to 512 takes 71 us, 77 with a residual and 83 with gelu, of which 53 are products; 65536 x 512 to 2048 103, 137 and
+// 146. A tile's stores come from all CUs at about the same time, and only the next tile's first stage overlaps them: two workgroups of
+// 256 x 128 to a CU, one storing while the other multiplies, ran at 1920 TOP/s and were slower throughout (the former 89, 106 and
+// 98 us).
 #include <cmath>
 
 #include "product_kernels.h"
@@ -186,6 +186,10 @@ template <typename T, int MF> hipError_t launch_direct(Product &p, const int8_t 
 }
 
 template <typename T> hipError_t launch_one(Kernel kernel, Product &p, const int8_t *x, const int8_t *w, int K, hipStream_t s) {
+    if constexpr (!is_f32<T>()) {
+        if (p.residual && kernel == WIDE) return launch_wide<T, false, false, 4, Codes, true>(p, s);
+        if (p.residual && kernel == HALF) return launch_wide<T, false, false, 2, Codes, true>(p, s);
+    }
     switch (kernel) {
         case WIDE: return launch_wide<T, false, false, 4, Codes>(p, s);
         case HALF: return launch_wide<T, false, false, 2, Codes>(p, s);

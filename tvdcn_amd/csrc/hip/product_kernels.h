@@ -96,6 +96,13 @@ __device__ __forceinline__ void load_to_lds(const u32x4 &rsrc, uint32_t offset, 
                  : "s"(lds), "v"(offset), "s"(rsrc)
                  : "memory", "m0");
 }
+// 64 lanes x 4 bytes, into 256 bytes of LDS
+__device__ __forceinline__ void load_words_to_lds(const u32x4 &rsrc, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+                 :
+                 : "s"(lds), "v"(offset), "s"(rsrc)
+                 : "memory", "m0");
+}
 #pragma clang diagnostic pop
 
 template <int N> constexpr int log2_of() { return N <= 1 ? 0 : 1 + log2_of<N / 2>(); }
@@ -485,20 +492,41 @@ __device__ __forceinline__ void store_results(const Product &p, const fvec4 (&ac
             }
 }
 
-// The same of 8-bit operands, scaled by row and column. Their products take half the time, so what is read on the way weighs
-// twice: everything is asked for at once, the residual AHEAD rows before its use.
+// What a tile's scaled results need, in LDS: scales of the columns and of the rows, and the bias (zeros where there is none), 1 KB
+// each. A wave loads at most two runs of 256 bytes of them.
+template <typename T> struct TileScales {
+    static constexpr int BYTES = 3072, BIAS = 2048;
+    static __device__ __forceinline__ void stage(const Product &p, int row0, int col0, uint32_t lds, int wave, int lane) {
+        auto scalar = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
+        auto load = [&](const void *from, int first, int left, uint32_t size, int part, uint32_t to) {
+            const uint64_t base = (uint64_t)from + size * (uint64_t)(uint32_t)first;
+            const uint32_t bytes = from ? (uint32_t)min(left, 256) * size : 0u;
+            load_words_to_lds(u32x4{scalar((uint32_t)base), scalar((uint32_t)(base >> 32)), scalar(bytes), 0x00020000u},
+                              (uint32_t)(part * 256 + lane * 4), scalar(to + part * 256));
+        };
+        if (wave < 4) load(p.scale_c, col0, p.cols - col0, 4, wave, lds);
+        else load(p.scale_r, row0, p.rows - row0, 4, wave - 4, lds + 1024);
+        if (wave < (int)sizeof(T)) load(p.bias, col0, p.cols - col0, sizeof(T), wave, lds + BIAS);
+    }
+};
+
+// Results of 8-bit operands, scaled by row and column, of rows 32 FIRST .. 32 (FIRST + ROWS) - 1 of the tile. Their products take half the
+// time, so what is read on the way weighs twice: scales and bias lie in LDS (`scales`), and so does a residual of 16 bits (STAGED:
+// `staged`, the lane's first value of row 32 FIRST at `place`; rows of 128 FC bytes); one of float32 is read AHEAD rows before its use.
 // row0, col0: the tile's (uniform) first row and column; lane_row, lane_col: from there to the lane's first.
-template <typename T, int FC>
-__device__ __forceinline__ void store_scaled(const Product &p, const i32x4 (&acc)[FC][8], int row0, int col0, int lane_row, int lane_col) {
-    constexpr int RUN = 8, RUNS = FC / 2, AHEAD = 2;
+template <typename T, int FC, int FIRST, int ROWS, bool STAGED>
+__device__ __forceinline__ void store_scaled(const Product &p, const i32x4 (&acc)[FC][8], int row0, int col0, int lane_row, int lane_col,
+                                             const char *scales, const char *staged = nullptr, uint32_t place = 0) {
+    constexpr int RUN = 8, RUNS = FC / 2, AHEAD = FC == 4 ? 1 : 2;   // (as registers allow)
+    constexpr bool READ = !STAGED && is_f32<T>();   // (a residual of 16 bits is staged)
     typedef Pack<T, RUN> Run;
     typedef Pack<float, RUN> Scales;
     const int rows = p.rows - row0 - lane_row, cols = p.cols - col0 - lane_col;   // from the lane's first to the edge
     const uint32_t off = (uint32_t)lane_row * (uint32_t)p.cols + (uint32_t)lane_col;
     const int64_t origin = (int64_t)row0 * p.cols + col0;
-    Run bias[RUNS] = {}, ahead[AHEAD][RUNS] = {};
+    Run bias[RUNS], ahead[READ ? AHEAD : 1][RUNS] = {};
     Scales scale[RUNS];
-    float scale_r[8];
+    float scale_r[ROWS];
     auto residual = [&](int j) {
         const T *from = (const T *)p.residual + origin + (int64_t)j * 32 * p.cols;
 #pragma unroll
@@ -506,33 +534,35 @@ __device__ __forceinline__ void store_scaled(const Product &p, const i32x4 (&acc
             if (j * 32 < rows && r * 32 < cols) ahead[j % AHEAD][r] = *reinterpret_cast<const Run *>(from + (off + r * 32));
     };
 #pragma unroll
-    for (int j = 0; j < 8; ++j) scale_r[j] = p.scale_r[row0 + (j * 32 < rows ? lane_row + j * 32 : 0)];
+    for (int j = 0; j < ROWS; ++j) scale_r[j] = *reinterpret_cast<const float *>(scales + 1024 + (lane_row + (FIRST + j) * 32) * 4);
 #pragma unroll
-    for (int r = 0; r < RUNS; ++r) scale[r] = *reinterpret_cast<const Scales *>(p.scale_c + col0 + (r * 32 < cols ? lane_col + r * 32 : 0));
-    if (p.bias)
+    for (int r = 0; r < RUNS; ++r) {
+        scale[r] = *reinterpret_cast<const Scales *>(scales + (lane_col + r * 32) * 4);
+        bias[r] = *reinterpret_cast<const Run *>(scales + TileScales<T>::BIAS + (lane_col + r * 32) * sizeof(T));
+    }
+    if constexpr (READ)
+        if (p.residual)
 #pragma unroll
-        for (int r = 0; r < RUNS; ++r)
-            if (r * 32 < cols) bias[r] = *reinterpret_cast<const Run *>((const T *)p.bias + col0 + (lane_col + r * 32));
-    if (p.residual)
+            for (int j = 0; j < AHEAD; ++j) residual(FIRST + j);
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j) residual(j);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = FIRST; j < FIRST + ROWS; ++j) {
         T *to = (T *)p.out + origin + (int64_t)j * 32 * p.cols;
-        Run res[RUNS];
+        Run res[RUNS] = {};
 #pragma unroll
-        for (int r = 0; r < RUNS; ++r) res[r] = ahead[j % AHEAD][r];
-        if (p.residual && j + AHEAD < 8) residual(j + AHEAD);
+        for (int r = 0; r < RUNS; ++r) {
+            // (chunks of 16 bytes lie turned by their row: the run 32 columns on is four chunks away either way)
+            if constexpr (STAGED) res[r] = *reinterpret_cast<const Run *>(staged + (place ^ (r * 64u)) + (j - FIRST) * 32 * 128 * FC);
+            if constexpr (READ) res[r] = ahead[j % AHEAD][r];
+        }
+        if constexpr (READ)
+            if (p.residual && j + AHEAD < FIRST + ROWS) residual(j + AHEAD);
 #pragma unroll
         for (int r = 0; r < RUNS; ++r) {
             float v[RUN];
 #pragma unroll
-            for (int e = 0; e < RUN; ++e) v[e] = (float)acc[r * 2 + e / 4][j][e % 4] * scale_r[j] * scale[r].v[e];
-            if (p.bias)
-#pragma unroll
-                for (int e = 0; e < RUN; ++e) v[e] += (float)bias[r].v[e];
+            for (int e = 0; e < RUN; ++e) v[e] = (float)acc[r * 2 + e / 4][j][e % 4] * scale_r[j - FIRST] * scale[r].v[e] + (float)bias[r].v[e];
             act_values<is_f32<T>(), RUN>(v, p.act);
-            if (p.residual)
+            if constexpr (STAGED || READ)
 #pragma unroll
                 for (int e = 0; e < RUN; ++e) v[e] += (float)res[r].v[e];
             Run o;
@@ -576,13 +606,19 @@ template <int BC, int STEP = 64> struct WideTile {
 
 // Where a workgroup's loads of one operand are: the stage's base, and how many bytes from a sub-tile's first element on are
 // its own (rows, or columns of the last t, behind the edge are then read as zeros)
-template <bool TM, int B, int STEP = 64, int ES = 2> struct WideSource {
+// ANY: sub-tiles of `unit` output indexes instead of 64, which may be set to lie anywhere.
+template <bool TM, int B, int STEP = 64, int ES = 2, bool ANY = false> struct WideSource {
     uint64_t base, step;     // of a stage; from sub-tile to sub-tile
     int inside;              // output indexes from the tile's first one on
     uint32_t rows;           // t-major: the bytes of the stage's t before the last one
     uint32_t pitch;          // bytes
     uint32_t off;            // the lane's offset, past the end where its reduction indexes are
     int stages, tail;        // from this one to the operand's end, and the length of the last of them
+    int unit_;
+    __device__ __forceinline__ int unit() const { return ANY ? unit_ : 64; }
+    __device__ __forceinline__ void set(uint64_t from, uint32_t row_bytes, int indexes, int unit, uint32_t lane_off) {
+        base = from, pitch = row_bytes, step = (uint64_t)(uint32_t)unit * row_bytes, inside = indexes, unit_ = unit, off = lane_off;
+    }
     __device__ __forceinline__ int left() const { return stages > 1 ? STEP : tail; }
     __device__ __forceinline__ void trim(uint32_t lane_off, int lane_at) {
         if (TM) rows = (uint32_t)(left() - 1) * pitch, off = lane_off;
@@ -593,6 +629,7 @@ template <bool TM, int B, int STEP = 64, int ES = 2> struct WideSource {
         inside = __builtin_amdgcn_readfirstlane((int)(o.width - first < B ? o.width - first : B));
         pitch = (uint32_t)ES * (uint32_t)o.ld;
         step = TM ? 64 * ES : 64 * (uint64_t)pitch;
+        if (ANY) unit_ = 64;
         const int64_t t = o.lim - k0, n = (t + STEP - 1) / STEP;
         stages = __builtin_amdgcn_readfirstlane((int)(n < (1 << 30) ? n : 1 << 30));
         tail = (((int)t - 1) & (STEP - 1)) + 1;
@@ -605,7 +642,7 @@ template <bool TM, int B, int STEP = 64, int ES = 2> struct WideSource {
     }
     __device__ __forceinline__ u32x4 descriptor(int q, uint64_t beyond = 0) const {
         const uint64_t b = base + q * step + beyond;
-        const int n = min(max(inside - 64 * q, 0), 64);
+        const int n = min(max(inside - unit() * q, 0), unit());
         const uint32_t bytes = TM ? (n ? rows + (uint32_t)ES * n : 0u) : (uint32_t)n * pitch;
         // (uniform, which the compiler does not always see)
         auto scalar = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
@@ -613,7 +650,38 @@ template <bool TM, int B, int STEP = 64, int ES = 2> struct WideSource {
     }
 };
 
-template <typename T, bool RT, bool CT, int FC, typename E = T>
+//
+// 8-bit operands: what the results read comes through LDS, so that no load waits behind those of the next stages, and a tile's
+// stores are not waited for: the counts of the next tile's first stage allow for them. 65536 x 512 to 2048 takes 103 us (110 with
+// scales read and stores waited for as the results are made, 134 with the scales row by row), with gelu 146 (159).
+//
+// STAGED: their results of 16 bits with a residual. The residual's tile goes through LDS as two more stages behind the tile's own, rows
+// 0..127 and 128..255: its loads are under way during the last products, all of them at once, where a lane's registers hold two
+// rows' (65536 x 512 to 2048: 137 us instead of 177, 65536 x 2048 to 512 77 instead of 89). The next tile's first loads are issued as
+// the halves are done with.
+template <int FC> struct StagedResidual {
+    static constexpr int BYTES = 128 * FC, LANES = 8 * FC, ROWS = 64 / FC;   // of a row; lanes to a row; rows of a sub-tile of 8 KB
+    // the lane's row of a sub-tile and its chunk of 16 bytes: chunk c of row n lies at c ^ n % 16, so that a read of 16 rows
+    // falls into different banks
+    int row, chunk;
+    uint32_t off;
+    __device__ __forceinline__ StagedResidual(const Product &p, int wave, int lane) {
+        row = wave * (ROWS / 8) + lane / LANES;
+        chunk = (lane & (LANES - 1)) ^ (row & 15);
+        off = (uint32_t)row * (uint32_t)p.cols * 2u + (uint32_t)chunk * 16u;
+    }
+    // the next stage's loads are of a half of the tile at row0, col0: from the rows' places and, FC = 4, the columns'
+    template <typename R, typename C>
+    __device__ __forceinline__ void aim(const Product &p, int row0, int col0, int half, bool any, R &rows, C &cols) const {
+        const int first = row0 + half * 128, inside = any ? min(max(p.rows - first, 0), 128) : 0;
+        const uint64_t base = (uint64_t)p.residual + 2 * ((uint64_t)(uint32_t)first * (uint32_t)p.cols + (uint32_t)col0);
+        const uint32_t pitch = (uint32_t)p.cols * 2u, at = chunk * 8 < p.cols - col0 ? off : 0x80000000u;
+        rows.set(base, pitch, inside, ROWS, at);
+        cols.set(base + 4 * ROWS * (uint64_t)pitch, pitch, FC == 4 ? inside - 4 * ROWS : 0, ROWS, at);
+    }
+};
+
+template <typename T, bool RT, bool CT, int FC, typename E = T, bool STAGED = false>
 __global__ void __launch_bounds__(512, 2) wide_product_kernel(Product p) {
     constexpr int BC = 64 * FC, COLS = 32768, STAGE = COLS + BC * 128;   // bytes; the columns' sub-tiles follow the rows'
     constexpr int ES = sizeof(E), STEP = 128 / ES;                       // of the reduction in a stage
@@ -634,8 +702,9 @@ __global__ void __launch_bounds__(512, 2) wide_product_kernel(Product p) {
     // the stage to load next
     int tile_n = 0, step = 0, buf = 0;
     WideTile<BC, STEP> ahead(p, tiles.first);
-    WideSource<RT, 256, STEP, ES> rows;
-    WideSource<CT, BC, STEP, ES> cols;
+    WideSource<RT, 256, STEP, ES, STAGED> rows;
+    WideSource<CT, BC, STEP, ES, STAGED> cols;
+    const StagedResidual<FC> residual(p, wave, lane);
     auto enter = [&]() {
         const int64_t k0 = ahead.kbeg + (int64_t)step * STEP;
         rows.enter(p.R, ahead.row0, k0, off_r, at_r);
@@ -649,6 +718,11 @@ __global__ void __launch_bounds__(512, 2) wide_product_kernel(Product p) {
             cols.advance(off_c, at_c);
             return;
         }
+        if constexpr (STAGED)
+            if (step < ahead.nk + 2) {
+                residual.aim(p, ahead.row0, ahead.col0, step - ahead.nk, tile_n < tiles.count, rows, cols);
+                return;
+            }
         step = 0;
         if (++tile_n < tiles.count) ahead = WideTile<BC, STEP>(p, tiles.first + tile_n * tiles.step);
         enter();
@@ -672,9 +746,13 @@ __global__ void __launch_bounds__(512, 2) wide_product_kernel(Product p) {
     aim_rows(2);
     asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(4 + FC) : "memory");
 
+    constexpr bool CODES = std::is_same<E, Codes>::value;
+    constexpr int SCALES = 2 * STAGE, STORES = 8 * (FC / 2) * (sizeof(T) / 2);   // stores of a lane's results, 16 bytes each
+    bool stored = false;   // CODES: the last tile's stores may be under way, STORES of them behind its last loads (STAGED: half of them)
     int at = 0;
     for (int n = 0; n < tiles.count; ++n) {
         const WideTile<BC, STEP> tile(p, tiles.first + n * tiles.step);
+        if constexpr (CODES) TileScales<T>::stage(p, tile.row0, tile.col0, lds - wave * 1024u + SCALES + (n & 1) * TileScales<T>::BYTES, wave, lane);
         typedef typename Sums<E>::type Sum;
         Sum acc[FC][8];
 #pragma unroll
@@ -699,7 +777,11 @@ __global__ void __launch_bounds__(512, 2) wide_product_kernel(Product p) {
                     for (int j = 0; j < 2; ++j) b[kk][j] = SR::template frag<E>(tr + ph * 8192, j * 32 + wr * 16, kk, lane);
                 }
                 if constexpr (FC == 4 || ph != 2) load();
-                if constexpr (ph == 1)
+                if (CODES && ph == 1 && it == 0 && stored)
+                    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((FC == 4 ? 10 : 8) + (STAGED ? STORES / 2 : STORES)) : "memory");
+                else if (CODES && ph == 3 && it == 0 && stored && !STAGED)
+                    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(4 + FC + STORES) : "memory");
+                else if constexpr (ph == 1)
                     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(FC == 4 ? 10 : 8) : "memory");
                 else if constexpr (ph == 3)
                     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(4 + FC) : "memory");
@@ -733,13 +815,50 @@ __global__ void __launch_bounds__(512, 2) wide_product_kernel(Product p) {
             phase(std::integral_constant<int, 3>());
         }
         if (!wr) asm volatile("s_barrier" ::: "memory");   // level again
-        if constexpr (std::is_same<E, Codes>::value)
-            store_scaled<T, FC>(p, acc, tile.row0, tile.col0, wr * 16 + (lane & 15), wc * 16 * FC + (lane >> 4) * 8);
-        else
+        if constexpr (CODES) {
+            // A whole tile's stores are counted, STORES a lane; at an edge some lanes have none, and all are waited for. So are they
+            // where a tile has one stage alone, since that one's waits are for its scales too.
+            const bool whole = tile.row0 + 256 <= p.rows && tile.col0 + BC <= p.cols && tile.nk > 1;
+            const int lane_row = wr * 16 + (lane & 15), lane_col = wc * 16 * FC + (lane >> 4) * 8;
+            const char *scales = smem + SCALES + (n & 1) * TileScales<T>::BYTES;
+            if constexpr (STAGED) {
+                // Every wave has read the last stage: the last loads of the residual's second half. Its first half has landed when
+                // those of the second are the only ones left.
+                const uint32_t place = lane_row * 128 * FC + (((lane_col >> 3) ^ (lane & 15)) << 4);
+                load();
+                asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(4 + FC) : "memory");
+                next();
+                store_scaled<T, FC, 0, 4, true>(p, acc, tile.row0, tile.col0, lane_row, lane_col, scales, smem + at * STAGE, place);
+                if (whole) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(STORES / 2) : "memory");
+                else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                aim_cols(0), load();
+                if (FC == 4) aim_cols(2), load();
+                aim_rows(0), load();
+                aim_rows(2), load();
+                next();
+                store_scaled<T, FC, 4, 4, true>(p, acc, tile.row0, tile.col0, lane_row, lane_col, scales, smem + (at ^ 1) * STAGE, place);
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                aim_cols(0), load();
+                if (FC == 4) aim_cols(2), load();
+                aim_rows(0), load();
+                aim_rows(2);
+                if (whole) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(4 + FC + STORES / 2) : "memory");
+                else asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(4 + FC) : "memory");
+                stored = whole;
+            } else {
+                store_scaled<T, FC, 0, 8, false>(p, acc, tile.row0, tile.col0, lane_row, lane_col, scales);
+                stored = whole && !(is_f32<T>() && p.residual);
+                if (stored) asm volatile("s_barrier" ::: "memory");
+                else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+            }
+        } else {
             store_results<T, CT, FC>(p, acc, tile.split, tile.row0 + wr * 16 + (lane & 15), tile.col0 + wc * 16 * FC, lane >> 4);
-        // the loads' counts above are of loads alone
-        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+            // the loads' counts above are of loads alone
+            asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+        }
     }
+    // (no load to LDS outlives the workgroup)
+    if constexpr (CODES) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
 // ---- host ----
@@ -765,9 +884,10 @@ template <typename K> hipError_t launch_persistent(K kernel, std::atomic<unsigne
     kernel<<<(unsigned)(tiles < 256 ? tiles : 256), 512, lds, s>>>(p);
     return hipGetLastError();
 }
-template <typename T, bool RT, bool CT, int FC, typename E = T> hipError_t launch_wide(Product &p, hipStream_t s) {
+template <typename T, bool RT, bool CT, int FC, typename E = T, bool STAGED = false> hipError_t launch_wide(Product &p, hipStream_t s) {
     static std::atomic<unsigned long long> done{0};
-    return launch_persistent(wide_product_kernel<T, RT, CT, FC, E>, done, p, 64 * FC, 2 * (32768 + 64 * FC * 128), s);
+    return launch_persistent(wide_product_kernel<T, RT, CT, FC, E, STAGED>, done, p, 64 * FC,
+                             2 * (32768 + 64 * FC * 128) + (std::is_same<E, Codes>::value ? 2 * TileScales<T>::BYTES : 0), s);
 }
 
 }  // namespace
