@@ -495,7 +495,7 @@ __device__ __forceinline__ void store_results(const Product &p, const fvec4 (&ac
 // What a tile's scaled results need, in LDS: scales of the columns and of the rows, and the bias (zeros where there is none), 1 KB
 // each. A wave loads at most two runs of 256 bytes of them.
 template <typename T> struct TileScales {
-    static constexpr int BYTES = 3072, BIAS = 2048;
+    static constexpr int BIAS = 2048, BYTES = BIAS + 1024;
     static __device__ __forceinline__ void stage(const Product &p, int row0, int col0, uint32_t lds, int wave, int lane) {
         auto scalar = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
         auto load = [&](const void *from, int first, int left, uint32_t size, int part, uint32_t to) {
