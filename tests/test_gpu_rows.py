@@ -552,3 +552,21 @@ def test_kernel_timer_families():
             assert lib.tvdcn_kernel_timer_read(family, ctypes.byref(ms), ctypes.byref(n)) == 0 and n.value == 1
     finally:
         lib.tvdcn_kernel_timer_enable(0)
+
+
+@pytest.mark.parametrize("seed", range(16))
+def test_int8_products_of_random_sizes(seed):
+    """Sizes that fill the chip with the largest tiles and end anywhere in them: one stage along the reduction to many, one tile a
+    workgroup to several, whole tiles and ragged ones, with and without what is added."""
+    import random
+    rng = random.Random(seed)
+    channels = rng.choice((16, 64, 128, 144, 256, 257, 384, 1040, 2048))
+    out = 8 * rng.randint(1, 96) if seed % 4 else rng.randint(1, 700)
+    rows = rng.randint(1, 1 << 25) // max(channels, 256) * 256 // out
+    rows = max(1, min(rows if seed % 3 else rows // 256 * 256, 120000))
+    dtype = DTYPES[seed % 3]
+    a = [*codes_of((rows, channels), seed), *codes_of((out, channels), seed + 1)]
+    b, r = make((out,), dtype, 3), torch.randn(rows, out, device="cuda", generator=torch.Generator("cuda").manual_seed(seed)).to(dtype)
+    for act, bias, res in (("none", None, r), ("silu", b, r), ("relu", b, None)):
+        y = tvdcn.pointwise_conv_int8(*a, bias, res, act, dtype)
+        check([y], [pointwise_int8(*a, bias, res, act, dtype)], (rows, channels, out, act))
