@@ -4,6 +4,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/autocast_mode.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/autograd.h>
@@ -82,6 +83,8 @@ inline Tensor new_map(at::IntArrayRef sizes, const at::TensorOptions &options) {
     strides[1] = run, run *= std::max<int64_t>(sizes[1], 1);
     for (size_t i = n - 1; i >= 2; --i) strides[i] = run, run *= std::max<int64_t>(sizes[i], 1);
     strides[0] = run;
+    // (on the GPU without the dispatcher: 0.3 us of a call's 6)
+    if (options.device().is_cuda()) return Tensor(at::detail::empty_strided_cuda(sizes, strides, options));
     return at::empty_strided(sizes, strides, options);
 }
 // the map with its channels contiguous per pixel, 16-byte aligned: itself, or a copy
@@ -121,7 +124,9 @@ inline void check_status(tvdcn_status st, const char *what) {
 }
 inline void *stream_of(const Tensor &t) { return (void *)c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 inline void *ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
-inline Tensor bytes(const Tensor &x, size_t n) { return at::empty({(int64_t)n}, x.options().dtype(at::kByte)); }
+// (on the GPU; see new_map)
+inline Tensor new_flat(at::IntArrayRef sizes, const at::TensorOptions &options) { return Tensor(at::detail::empty_cuda(sizes, options)); }
+inline Tensor bytes(const Tensor &x, size_t n) { return new_flat({(int64_t)n}, x.options().dtype(at::kByte)); }
 
 inline at::ScalarType wide_type(const Tensor &t) { return t.scalar_type() == at::kDouble ? at::kDouble : at::kFloat; }
 

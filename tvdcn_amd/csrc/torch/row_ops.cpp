@@ -58,7 +58,7 @@ Three rms_forward_hip(const Tensor &x, MaybeTensor residual, MaybeTensor weight,
     const Tensor r = rows_of(x), res = rows_of(residual), w = flat(weight);
     Tensor y = new_map(x.sizes(), x.options());
     Tensor sum = has(residual) ? new_map(x.sizes(), x.options()) : Tensor();
-    Tensor rstd = save ? at::empty(pixel_shape(x), x.options().dtype(at::kFloat)) : Tensor();
+    Tensor rstd = save ? new_flat(pixel_shape(x), x.options().dtype(at::kFloat)) : Tensor();
     check_status(tvdcn_rms_norm_forward(&d, ptr(r), ptr(res), ptr(w), ptr(sum), ptr(y), (float *)ptr(rstd), stream_of(x)), RMS);
     return {y, sum, rstd};
 }
@@ -70,7 +70,7 @@ Two rms_backward_hip(const Tensor &grad, MaybeTensor grad_sum, const Tensor &nor
     const Tensor g = rows_of(grad), gs = rows_of(grad_sum), x = rows_of(normalised), w = flat(weight), st = floats(rstd);
     Tensor dx, dw;
     if (want[0]) dx = new_map(grad.sizes(), grad.options());
-    if (want[1]) dw = at::empty({grad.size(1)}, grad.options());
+    if (want[1]) dw = new_flat({grad.size(1)}, grad.options());
     const size_t n = want[1] ? tvdcn_rms_norm_backward_workspace_size(&d) : 0;
     const Tensor work = n ? bytes(grad, n) : Tensor();
     check_status(tvdcn_rms_norm_backward(&d, ptr(g), ptr(gs), ptr(x), (const float *)ptr(st), ptr(w), ptr(dx), ptr(dw), ptr(work), n,
@@ -85,7 +85,7 @@ Three rms8_hip(const Tensor &x, MaybeTensor residual, MaybeTensor weight, double
     const auto d = rms_desc(x, eps, RMS8);
     const Tensor r = rows_of(x), res = rows_of(residual), w = flat(weight);
     Tensor codes = new_map(x.sizes(), x.options().dtype(at::kChar));
-    Tensor scales = at::empty(pixel_shape(x), x.options().dtype(at::kFloat));
+    Tensor scales = new_flat(pixel_shape(x), x.options().dtype(at::kFloat));
     Tensor sum = has(residual) ? new_map(x.sizes(), x.options()) : Tensor();
     check_status(tvdcn_rms_norm_int8(&d, ptr(r), ptr(res), ptr(w), ptr(sum), (int8_t *)ptr(codes), (float *)ptr(scales), stream_of(x)),
                  RMS8);
@@ -201,7 +201,7 @@ Two quantize_hip(const Tensor &x) {
     c10::DeviceGuard guard(x.device());
     const Tensor r = rows_of(x);
     Tensor codes = new_map(x.sizes(), x.options().dtype(at::kChar));
-    Tensor scales = at::empty(pixel_shape(x), x.options().dtype(at::kFloat));
+    Tensor scales = new_flat(pixel_shape(x), x.options().dtype(at::kFloat));
     check_status(tvdcn_quantize_int8(map_dtype(x.scalar_type(), QUANTIZE), rows_in(x), x.size(1), ptr(r), (int8_t *)ptr(codes),
                                      (float *)ptr(scales), stream_of(x)),
                  QUANTIZE);
