@@ -570,3 +570,16 @@ def test_int8_products_of_random_sizes(seed):
     for act, bias, res in (("none", None, r), ("silu", b, r), ("relu", b, None)):
         y = tvdcn.pointwise_conv_int8(*a, bias, res, act, dtype)
         check([y], [pointwise_int8(*a, bias, res, act, dtype)], (rows, channels, out, act))
+
+
+def test_int8_products_of_rows_in_several_launches():
+    """So many tiles that the rows go out in runs: the rows at the border between them, and the last."""
+    rows, channels, out = (1 << 21) // (1 << 14) * 64 + 70, 24, 1 << 20
+    q, s = codes_of((rows, channels), 1)
+    wq, ws = codes_of((out, channels), 2)
+    r = torch.randn(rows, out, generator=torch.Generator("cuda").manual_seed(3), device="cuda", dtype=torch.bfloat16)
+    y = tvdcn.pointwise_conv_int8(q, s, wq, ws, None, r)
+    for part in (slice(0, 70), slice(rows - 200, rows)):
+        for cols in (slice(0, 500), slice(out - 500, out)):
+            want = pointwise_int8(q[part], s[part], wq[cols], ws[cols], None, r[part, cols], "none", torch.bfloat16)
+            check([y[part, cols]], [want], (part, cols))

@@ -483,3 +483,42 @@ def test_c_abi_refuses_pointers_and_workspaces(lib):
     g = lib.tvdcn_seeded_dropout
     assert g(0, 8, 0.5, None, p, p, p, None) == INVALID and g(0, 8, 0.5, P(4100), p, p, p, None) == INVALID
     assert g(0, 8, 0.5, p, None, p, p, None) == INVALID and g(0, 8, 0.5, p, p, odd, p, None) == INVALID
+
+
+def test_a_sum_that_needs_no_gradient_asks_for_none():
+    x, r, w = torch.randn(2, 6, 3), torch.randn(2, 6, 3), torch.randn(6, requires_grad=True)
+    y, s = tvdcn.add_rms_norm(x, r, w)
+    assert y.requires_grad and not s.requires_grad
+    s.add_(1)                       # (what the backward reads has changed)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    y, s = tvdcn.add_rms_norm(x, leaf(r), w)
+    assert s.requires_grad
+
+
+def test_a_convolution_weight_in_8_bits():
+    conv, x = torch.nn.Conv2d(6, 4, 1), torch.randn(2, 6, 3, 5)
+    with torch.no_grad():
+        codes, scales = tvdcn.quantize_int8(conv.weight)
+        assert codes.shape == (4, 6, 1, 1) and scales.shape == (4, 1, 1)
+        a = tvdcn.quantize_int8(x)
+        y = tvdcn.pointwise_conv_int8(*a, codes, scales, conv.bias, dtype=torch.float32)
+        assert torch.equal(y, tvdcn.pointwise_conv_int8(*a, codes[:, :, 0, 0], scales[:, 0, 0], conv.bias, dtype=torch.float32))
+        for q, s in ((codes.expand(4, 6, 2, 1), scales), (codes, scales[:3])):
+            with pytest.raises(RuntimeError, match="pointwise_conv_int8: expected"):
+                tvdcn.pointwise_conv_int8(*a, q, s)
+
+
+@pytest.mark.parametrize("requires", [True, False])
+def test_operators_are_registered_as_torch_expects(requires):
+    """Schemas, autograd registration, shapes without data and traced calls, by torch's own check."""
+    x, w, seed = torch.randn(2, 6, 4, 3, requires_grad=requires), torch.randn(6, requires_grad=requires), seed_of()
+    calls = [(OPS.rms_norm, (x, w, 1e-6)), (OPS.add_rms_norm, (x, x.detach(), w, 1e-6)), (OPS.seeded_dropout, (x, 0.3, seed, None))]
+    if not requires:
+        codes, scales = tvdcn.quantize_int8(x)
+        q, s = tvdcn.quantize_int8(torch.randn(4, 6))
+        calls += [(OPS.rms_norm_int8, (x, w, 1e-6)), (OPS.add_rms_norm_int8, (x, x, w, 1e-6)), (OPS.quantize_int8, (x,)),
+                  (OPS.dequantize_int8, (codes, scales, torch.float16)),
+                  (OPS.pointwise_conv_int8, (codes, scales, q, s, None, None, 3, torch.bfloat16))]
+    for op, args in calls:
+        assert set(torch.library.opcheck(op.default, args).values()) == {"SUCCESS"}

@@ -377,8 +377,9 @@ class RmsFunction : public torch::autograd::Function<RmsFunction> {
         ctx->save_for_backward({has(residual) ? std::get<1>(r) : x, std::get<2>(r), get(weight)});
         ctx->saved_data["residual"] = (int64_t)(has(residual) ? 1 : -1);
         ctx->saved_data["weight"] = (int64_t)(has(weight) ? 1 + has(residual) : -1);
-        if (has(residual)) return {std::get<0>(r), std::get<1>(r)};
-        return {std::get<0>(r)};
+        if (!has(residual)) return {std::get<0>(r)};
+        if (!needs(x) && !needs(residual)) ctx->mark_non_differentiable({std::get<1>(r)});   // (the sum does not know the weight)
+        return {std::get<0>(r), std::get<1>(r)};
     }
     static variable_list backward(AutogradContext *ctx, const variable_list &g) {
         const Tensor gy = g[0], gs = g.size() > 1 ? g[1] : Tensor();

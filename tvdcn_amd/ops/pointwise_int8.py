@@ -47,7 +47,7 @@ def pointwise_conv_int8(codes: Tensor, scales: Tensor, weight_codes: Tensor, wei
             or :func:`rms_norm_int8`. int8 and float32; channels-last codes are read as they are, others are copied
             first. At most 131071 channels.
         weight_codes (Tensor[out_channels, in_channels]), weight_scales (Tensor[out_channels]): the weight, from
-            :func:`quantize_int8`.
+            :func:`quantize_int8`. Both may have more axes of size one, as a convolution's weight has.
         bias (Tensor[out_channels]), residual (Tensor[batch, out_channels, \*size]): of type ``dtype`` (autocast
             rounds them to it).
         activation (str): "none", "relu", "silu" or "gelu" (with the error function).
@@ -62,6 +62,11 @@ def pointwise_conv_int8(codes: Tensor, scales: Tensor, weight_codes: Tensor, wei
     if not torch.jit.is_scripting():
         _log_api_usage_once(pointwise_conv_int8)
     _assert_has_ops()
+    if weight_codes.dim() > 2:
+        if weight_codes.numel() != weight_codes.size(0) * weight_codes.size(1):
+            raise RuntimeError("pointwise_conv_int8: expected weight codes of shape (out_channels, in_channels) and axes of "
+                               "size one, got {}".format(list(weight_codes.shape)))
+        weight_codes, weight_scales = weight_codes.flatten(1), weight_scales.flatten()
     return torch.ops.tvdcn.pointwise_conv_int8(codes, scales, weight_codes, weight_scales, bias, residual,
                                                _activation_code(activation), dtype)
 
