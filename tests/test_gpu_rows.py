@@ -583,3 +583,34 @@ def test_int8_products_of_rows_in_several_launches():
         for cols in (slice(0, 500), slice(out - 500, out)):
             want = pointwise_int8(q[part], s[part], wq[cols], ws[cols], None, r[part, cols], "none", torch.bfloat16)
             check([y[part, cols]], [want], (part, cols))
+
+
+@pytest.mark.parametrize("channels", [24, 71, 2500, 4097, 8192, 40000, 1 << 20])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_norms_of_the_largest_finite_values(channels, dtype):
+    """Rows at the type's largest finite value, of one sign, of both, beside small values, and alone among zeros, with the least and
+    the largest eps."""
+    most = torch.finfo(dtype).max
+    x = make((6, channels), dtype, 1)
+    x[0], x[1], x[2] = most, x[2].sign() * most, 2e38
+    x[3, ::2] = -most
+    x[4] = 0
+    x[4, channels // 2] = most
+    x[5] = 0
+    x[5, 0] = 1.8e19                # (its square is a float32, the mean of that with the largest eps is none)
+    w, dy = make((channels,), dtype, 2, shift=1.0), make((6, channels), dtype, 3)
+    assert torch.isfinite(x).all()
+    for eps in (1e-6, 2e-38, 3.4e38):
+        t = [leaf(x), leaf(w)]
+        y = tvdcn.rms_norm(*t, eps)
+        want = rms(x, None, w, eps, None, dy)
+        # beside the largest values the small ones' product with the reciprocal root is subnormal: it is rounded to a multiple of
+        # 2^-149, by up to 2^-150, and then multiplied by the weight
+        want[0] = want[0][0], want[0][1] + 2.0 ** -150 * w.double().abs()
+        check([y, *torch.autograd.grad(y, t, dy)], want, eps)
+        assert y[:5].any(1).all()
+        check_rms_int8(*tvdcn.rms_norm_int8(x, w, eps), x, w, eps)
+    y, s = tvdcn.add_rms_norm(x, torch.zeros_like(x), w)
+    assert torch.equal(s, x) and torch.equal(y, tvdcn.rms_norm(x, w))
+    codes, scales, s = tvdcn.add_rms_norm_int8(x, torch.zeros_like(x))
+    assert torch.equal(s, x) and (codes[:2].abs() == 127).all()

@@ -10,7 +10,7 @@
 // rows to a wave), rows beyond a wave's registers over a workgroup, rows beyond that are read twice.
 // (Rows that end within an access: Fit, below.)
 //
-// Sums are float32, in a fixed order. Squares beyond float32 are summed again at 2^-140 of their size.
+// Sums are float32, in a fixed order. A mean beyond float32 is taken again of squares at 2^-160 of their size.
 #include <algorithm>
 #include <type_traits>
 
@@ -124,10 +124,17 @@ template <typename Op, bool BLOCK> __device__ __forceinline__ float over_row(flo
     return v;
 }
 
-constexpr float DOWN = 8.470329472543003e-22f, DOWN2 = DOWN * DOWN;   // 2^-70
-static_assert(DOWN * 1180591620717411303424.f == 1.f && DOWN2 > 0, "");
-
-__device__ __forceinline__ bool is_infinite(float v) { return v == __builtin_inff(); }
+// The reciprocal root of a row whose squares `squares(f)` sums, of its values times f. Where the mean is no float32, the values are taken at
+// 2^-80 of their size: the largest square is then 2^96, 2^20 channels of them 2^116, and what made the mean infinite (a sum of 2^128,
+// or eps) is 2^-52 at least, beside which what vanishes below float32 does not count. (2^-160 itself is no float32: eps takes 2^-80
+// twice.) The mean is the same for all lanes of the row, and so is the way taken.
+constexpr float DOWN = 8.271806125530277e-25f;   // 2^-80
+static_assert(DOWN * 1099511627776.f * 1099511627776.f == 1.f, "");
+template <typename F> __device__ __forceinline__ float reciprocal_root(F &&squares, float inv_channels, float eps) {
+    const float mean = fmaf(squares(1.f), inv_channels, eps);
+    if (mean != __builtin_inff()) return 1.f / sqrtf(mean);
+    return DOWN / sqrtf(fmaf(squares(DOWN), inv_channels, eps * DOWN * DOWN));
+}
 
 // Codes of VEC values: v / scale rounded to the nearest, ties to even, as if the quotient were exact. v inv is within 2^-16 of it
 // (|v / scale| <= 127), so the rounding is settled unless it comes that close to a border; there v - code scale, which is exact,
@@ -236,10 +243,7 @@ __global__ void __launch_bounds__(BLOCK ? HELD_TB : TB) row_kernel(RowKernelArgs
                     }
                 return over_row<Add, BLOCK>(ss, a.log2, red);
             };
-            const float ss = squares(1.f);
-            float rstd = 1.f / sqrtf(fmaf(ss, a.inv_channels, a.eps));
-            if (is_infinite(ss))   // (the same for all lanes of the row)
-                rstd = DOWN / sqrtf(fmaf(squares(DOWN), a.inv_channels, a.eps * DOWN2));
+            const float rstd = reciprocal_root(squares, a.inv_channels, a.eps);
             if (a.rstd && l == 0) a.rstd[row] = rstd;
 #pragma unroll
             for (int n = 0; n < N; ++n)
@@ -302,9 +306,7 @@ template <typename T, int FIT, int MODE> __global__ void __launch_bounds__(LONG_
                 }
                 return over_row<Add, true>(ss, 6, red);
             };
-            const float ss = squares(1.f);
-            rstd = 1.f / sqrtf(fmaf(ss, a.inv_channels, a.eps));
-            if (is_infinite(ss)) rstd = DOWN / sqrtf(fmaf(squares(DOWN), a.inv_channels, a.eps * DOWN2));
+            rstd = reciprocal_root(squares, a.inv_channels, a.eps);
             if (a.rstd && t == 0) a.rstd[row] = rstd;
         }
         auto result = [&](const Place<T, FIT> &k, float *f) {
