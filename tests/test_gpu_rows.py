@@ -614,3 +614,26 @@ def test_norms_of_the_largest_finite_values(channels, dtype):
     assert torch.equal(s, x) and torch.equal(y, tvdcn.rms_norm(x, w))
     codes, scales, s = tvdcn.add_rms_norm_int8(x, torch.zeros_like(x))
     assert torch.equal(s, x) and (codes[:2].abs() == 127).all()
+
+
+# of every kernel that takes the products: straight from memory, tiles of 64, of 128, the persistent ones
+@pytest.mark.parametrize("rows,channels,out", [(5, 64, 40), (70, 71, 30), (4096, 512, 512), (4100, 333, 264), (65536, 1024, 300), (20000, 64, 128),
+                                               (100000, 64, 128), (65536, 64, 512)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_int8_products_of_scales_at_the_range_ends(rows, channels, out, dtype):
+    """Scales of 2^112 to 2^120 with some of 2^-126: their product with the sums alone is no float32, the result is an ordinary value.
+    On rows among others, and on columns."""
+    (q, _), (wq, _) = codes_of((rows, channels), 1), codes_of((out, channels), 2)
+    g = torch.Generator().manual_seed(3)
+
+    def scales(n):
+        far, near = (torch.exp2(torch.randint(lo, lo + 9, (n,), generator=g)) * (1 + torch.rand(n, generator=g)) for lo in (112, 0))
+        return torch.where(torch.rand(n, generator=g) < 0.1, far, near).cuda()
+
+    least = [torch.full((n,), 2.0 ** -126, device="cuda") for n in (rows, out)]
+    r = make((rows, out), dtype, 4)
+    for s, ws in ((scales(rows), least[1]), (least[0], scales(out))):
+        for act, res in (("none", None), ("relu", r)):
+            y = tvdcn.pointwise_conv_int8(q, s, wq, ws, None, res, act, dtype)
+            assert y.isfinite().all()
+            check([y], [pointwise_int8(q, s, wq, ws, None, res, act, dtype)], act)

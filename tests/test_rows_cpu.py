@@ -522,3 +522,18 @@ def test_operators_are_registered_as_torch_expects(requires):
                   (OPS.pointwise_conv_int8, (codes, scales, q, s, None, None, 3, torch.bfloat16))]
     for op, args in calls:
         assert set(torch.library.opcheck(op.default, args).values()) == {"SUCCESS"}
+
+
+def test_host_int8_product_of_scales_at_the_range_ends():
+    """A large scale of a pixel with small ones of the weight, and the other way round, where the result is an ordinary value."""
+    x, w = cpu((5, 64), torch.float32, 1), cpu((10, 64), torch.float32, 2)
+    up = torch.tensor([1e36, 1e37, 1.0, 1e30, 1e37])[:, None]
+    for a, b in ((x * up, w * 1e-37), (x * 1e-37, w * up.repeat(2, 1))):
+        q = [*tvdcn.quantize_int8(a), *tvdcn.quantize_int8(b)]
+        for dtype in DTYPES[1:]:
+            y = tvdcn.pointwise_conv_int8(*q, dtype=dtype)
+            assert y.isfinite().all()
+            check([y], [pointwise_int8(*q, None, None, "none", dtype)], dtype)
+    # where the result is no float32, it is infinite
+    q = tvdcn.quantize_int8(x * 1e37)
+    assert (tvdcn.pointwise_conv_int8(*q, *q, dtype=torch.float32).diagonal() == math.inf).all()

@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(TB) direct_product_kernel(Product p, const int
     const float sr = p.scale_r[row];
     float v[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = (float)sum[e] * sr * p.scale_c[min(col + e, p.cols - 1)];
+    for (int e = 0; e < 4; ++e) v[e] = scaled((float)sum[e], sr, p.scale_c[min(col + e, p.cols - 1)]);
     emit<T, 4>(p, 0, row, col, v);
 }
 

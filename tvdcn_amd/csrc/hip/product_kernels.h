@@ -178,6 +178,18 @@ template <bool TM, bool PERM, int B, int F, int NW> struct Stager {
     }
 };
 
+// A sum of products of codes (below 2^31), times the scales of its row and column: the row's first, which a float32 holds up to 2^96, and
+// a larger one last, so that an infinity stands only for a result that is one. (Scales of 2^-126 and more lose nothing either way.) Such
+// rows are rare: a wave without one (`far`) does not choose for every value, which would take two instructions each.
+constexpr float FAR_SCALE = 7.922816251426434e+28f;   // 2^96
+__device__ __forceinline__ bool is_far(float scale_r) { return fabsf(scale_r) > FAR_SCALE; }
+__device__ __forceinline__ float scaled(float sum, float scale_r, float scale_c) {
+    return is_far(scale_r) ? sum * scale_c * scale_r : sum * scale_r * scale_c;
+}
+__device__ __forceinline__ float scaled(float sum, float scale_r, float scale_c, float bias) {
+    return is_far(scale_r) ? fmaf(sum * scale_c, scale_r, bias) : fmaf(sum * scale_r, scale_c, bias);
+}
+
 // RUN neighbouring outputs of one row
 template <typename T, int RUN>
 __device__ __forceinline__ void emit(const Product &p, int split, int row, int col, const float *acc) {
@@ -339,7 +351,7 @@ __global__ void __launch_bounds__(WR * WC * 64, BLOCKS * WR * WC / 4) product_ke
                 if constexpr (CODES) {
                     const float sr = p.scale_r[row];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = v[e] * sr * scale[i + e / 4][e % 4];
+                    for (int e = 0; e < 8; ++e) v[e] = scaled(v[e], sr, scale[i + e / 4][e % 4]);
                 }
                 emit<T, 8>(p, split, row, col0 + wc * 16 * FC + q * 4 * FC + i * 4, v);
             }
@@ -535,6 +547,10 @@ __device__ __forceinline__ void store_scaled(const Product &p, const i32x4 (&acc
     };
 #pragma unroll
     for (int j = 0; j < ROWS; ++j) scale_r[j] = *reinterpret_cast<const float *>(scales + 1024 + (lane_row + (FIRST + j) * 32) * 4);
+    bool far = false;
+#pragma unroll
+    for (int j = 0; j < ROWS; ++j) far = far || is_far(scale_r[j]);
+    far = __any(far);
 #pragma unroll
     for (int r = 0; r < RUNS; ++r) {
         scale[r] = *reinterpret_cast<const Scales *>(scales + (lane_col + r * 32) * 4);
@@ -559,8 +575,13 @@ __device__ __forceinline__ void store_scaled(const Product &p, const i32x4 (&acc
 #pragma unroll
         for (int r = 0; r < RUNS; ++r) {
             float v[RUN];
+            if (far) {
 #pragma unroll
-            for (int e = 0; e < RUN; ++e) v[e] = (float)acc[r * 2 + e / 4][j][e % 4] * scale_r[j - FIRST] * scale[r].v[e] + (float)bias[r].v[e];
+                for (int e = 0; e < RUN; ++e) v[e] = scaled((float)acc[r * 2 + e / 4][j][e % 4], scale_r[j - FIRST], scale[r].v[e], (float)bias[r].v[e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < RUN; ++e) v[e] = fmaf((float)acc[r * 2 + e / 4][j][e % 4] * scale_r[j - FIRST], scale[r].v[e], (float)bias[r].v[e]);
+            }
             act_values<is_f32<T>(), RUN>(v, p.act);
             if constexpr (STAGED || READ)
 #pragma unroll

@@ -14,6 +14,7 @@ const char *RMS = "rms_norm", *RMS8 = "rms_norm_int8", *QUANTIZE = "quantize_int
            *POINT8 = "pointwise_conv_int8", *DROPOUT = "seeded_dropout";
 constexpr int64_t kMostSum = 131071;   // channels whose products of codes 32 bits hold the sum of
 const double kLeastScale = std::ldexp(1.0, -126), kMostScale = 2.6793883890187504e+36;   // (127 of the latter are finite)
+const double kFarScale = std::ldexp(1.0, 96);
 
 // (batch, *size): one value per pixel
 std::vector<int64_t> pixel_shape(const Tensor &x) {
@@ -289,7 +290,9 @@ Tensor point8_cpu(const Tensor &codes, const Tensor &scales, const Tensor &wcode
     if (codes.numel() == 0) return point8_meta(codes, scales, wcodes, wscales, bias, residual, act, dtype);
     // (the whole sums are exact in float64)
     const Tensor sums = rows_matrix(codes, at::kDouble).mm(wcodes.to(at::kDouble).t()).to(at::kFloat);
-    Tensor z = sums * scales.reshape({-1, 1}) * wscales;
+    // (a row's scale beyond 2^96 comes last: up to that its product with the sum, below 2^31, is a float32)
+    const Tensor sr = scales.reshape({-1, 1}), far = sr.abs() > kFarScale;
+    Tensor z = far.any().item<bool>() ? at::where(far, sums * wscales * sr, sums * sr * wscales) : sums * sr * wscales;
     if (has(bias)) z = z + bias->to(at::kFloat);
     z = act_value(z, act);
     if (has(residual)) z = z + rows_matrix(*residual, at::kFloat);

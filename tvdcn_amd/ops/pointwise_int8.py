@@ -53,8 +53,8 @@ def pointwise_conv_int8(codes: Tensor, scales: Tensor, weight_codes: Tensor, wei
         activation (str): "none", "relu", "silu" or "gelu" (with the error function).
         dtype: of the result: float32, float16 or bfloat16.
 
-    The products are summed exactly; scales, bias, activation and residual are applied in float32 and the result is
-    rounded once. Not differentiable: a call that would need a gradient raises.
+    The products are summed exactly; scales, bias, activation and residual are applied in float32 (the scales in an order
+    that overflows only where their result does) and the result is rounded once. Not differentiable: a call that would need a gradient raises.
 
     Returns:
         Tensor[batch, out_channels, \*size]: channels-last.
