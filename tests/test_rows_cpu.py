@@ -537,3 +537,17 @@ def test_host_int8_product_of_scales_at_the_range_ends():
     # where the result is no float32, it is infinite
     q = tvdcn.quantize_int8(x * 1e37)
     assert (tvdcn.pointwise_conv_int8(*q, *q, dtype=torch.float32).diagonal() == math.inf).all()
+
+
+def test_int8_module_takes_its_type_from_a_loaded_bias():
+    m = tvdcn.PointwiseConvInt8.from_float(tvdcn.PointwiseConv(6, 4)).half()
+    x = torch.randn(3, 6)
+    other = tvdcn.PointwiseConvInt8(6, 4, device="meta")
+    other.load_state_dict(m.state_dict(), assign=True)
+    assert other(x).dtype == torch.float16 and torch.equal(other(x), m(x)) and "float16" in repr(other)
+    assert torch.equal(torch.jit.script(other)(x), m(x))
+    other = other.to(torch.float32)
+    assert other(x).dtype == torch.float32 and other.weight_scales.dtype == torch.float32
+    other = tvdcn.PointwiseConvInt8(6, 4, bias=False, device="meta", dtype=torch.float16)
+    other.load_state_dict(tvdcn.PointwiseConvInt8.from_float(tvdcn.PointwiseConv(6, 4, bias=False)).state_dict(), assign=True)
+    assert other(x).dtype == torch.float16

@@ -73,7 +73,7 @@ def pointwise_conv_int8(codes: Tensor, scales: Tensor, weight_codes: Tensor, wei
 
 class PointwiseConvInt8(nn.Module):
     """See :func:`pointwise_conv_int8`. Holds the weight's codes and scales as buffers; made from a layer with float weights
-    by :meth:`from_float`. A result has the bias's type (``dtype`` where there is none)."""
+    by :meth:`from_float`. A result has the bias's type (the module's ``dtype`` where there is none)."""
 
     def __init__(self, in_channels: int, out_channels: int, bias: bool = True, activation: str = "none", device=None,
                  dtype: torch.dtype = torch.bfloat16) -> None:
@@ -117,8 +117,9 @@ class PointwiseConvInt8(nn.Module):
         """``input``: codes, with their scales, or a map of floating values, which is quantized first."""
         if scales is None:
             input, scales = quantize_int8(input)
-        return pointwise_conv_int8(input, scales, self.weight_codes, self.weight_scales, self.bias, residual,
-                                   self.activation, self.dtype)
+        bias = self.bias
+        dtype = self.dtype if bias is None else bias.dtype   # (a loaded bias may be of another type than the one it replaces)
+        return pointwise_conv_int8(input, scales, self.weight_codes, self.weight_scales, bias, residual, self.activation, dtype)
 
     def extra_repr(self) -> str:
         s = "{}, {}".format(self.in_channels, self.out_channels)
@@ -126,4 +127,4 @@ class PointwiseConvInt8(nn.Module):
             s += ", bias=False"
         if self.activation != "none":
             s += ", activation={}".format(self.activation)
-        return s + ", dtype={}".format(self.dtype)
+        return s + ", dtype={}".format(self.dtype if self.bias is None else self.bias.dtype)
