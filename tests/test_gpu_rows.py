@@ -637,3 +637,42 @@ def test_int8_products_of_scales_at_the_range_ends(rows, channels, out, dtype):
             y = tvdcn.pointwise_conv_int8(q, s, wq, ws, None, res, act, dtype)
             assert y.isfinite().all()
             check([y], [pointwise_int8(q, s, wq, ws, None, res, act, dtype)], act)
+
+
+# Tiles of 128 x 128 (the first three), persistent ones of 256 x 128 and of 256 x 256, these with one stage along the reduction and
+# several tiles to a workgroup: whole tiles and ragged ones, rows of codes multiplied as they lie and copied first
+@pytest.mark.parametrize("rows,channels,out", [(65536, 1024, 300), (65537, 512, 1001), (50001, 900, 350), (131072, 128, 128), (100000, 64, 128),
+                                               (65536, 100, 384), (65536, 64, 512), (66000, 128, 1000), (70001, 64, 520), (70001, 120, 512)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_int8_products_of_many_tiles(rows, channels, out, dtype):
+    a = [*codes_of((rows, channels), 1), *codes_of((out, channels), 2)]
+    b = make((out,), dtype, 3)
+    r = torch.randn(rows, out, device="cuda", generator=torch.Generator("cuda").manual_seed(4)).to(dtype)
+    for act, bias, res in (("none", None, None), ("none", None, r), ("relu", b, r), ("gelu", b, None)):
+        y = tvdcn.pointwise_conv_int8(*a, bias, res, act, dtype)
+        check([y], [pointwise_int8(*a, bias, res, act, dtype)], act)
+        # (loads and stores that overlap from tile to tile: again, and beside another product)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            other = tvdcn.pointwise_conv_int8(*a, bias, res, act, dtype)
+        assert torch.equal(tvdcn.pointwise_conv_int8(*a, bias, res, act, dtype), y)
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(other, y)
+
+
+@pytest.mark.parametrize("seed", range(18))
+def test_int8_products_of_random_sizes_and_types(seed):
+    """As above, each of type, whole tiles of rows, columns by eights, and what is added drawn by itself."""
+    import random
+    rng = random.Random(1000 + seed)
+    channels, dtype = rng.choice((16, 48, 64, 100, 128, 192, 256, 520, 1024)), DTYPES[rng.randrange(3)]
+    out = 8 * rng.randint(1, 128) if rng.random() < 0.7 else rng.randint(1, 1000)
+    rows = max(1, min(int(2 ** rng.uniform(10, 25)) // out, 140000))
+    rows = -(-rows // 256) * 256 if rng.random() < 0.5 else rows
+    a = [*codes_of((rows, channels), seed), *codes_of((out, channels), seed + 1)]
+    b, r = make((out,), dtype, 3), torch.randn(rows, out, device="cuda", generator=torch.Generator("cuda").manual_seed(seed)).to(dtype)
+    for act in ACTIVATIONS:
+        bias, res = (b if rng.random() < 0.5 else None), (r if rng.random() < 0.5 else None)
+        y = tvdcn.pointwise_conv_int8(*a, bias, res, act, dtype)
+        check([y], [pointwise_int8(*a, bias, res, act, dtype)], (rows, channels, out, act, dtype, bias is None, res is None))
