@@ -681,7 +681,7 @@ template <bool TM, int B, int STEP = 64, int ES = 2, bool ANY = false> struct Wi
 // rows' (65536 x 512 to 2048: 137 us instead of 177, 65536 x 2048 to 512 77 instead of 89). The next tile's first loads are issued as
 // the halves are done with.
 template <int FC> struct StagedResidual {
-    static constexpr int BYTES = 128 * FC, LANES = 8 * FC, ROWS = 64 / FC;   // of a row; lanes to a row; rows of a sub-tile of 8 KB
+    static constexpr int LANES = 8 * FC, ROWS = 64 / FC;   // to a row of 128 FC bytes; rows of a sub-tile of 8 KB
     // the lane's row of a sub-tile and its chunk of 16 bytes: chunk c of row n lies at c ^ n % 16, so that a read of 16 rows
     // falls into different banks
     int row, chunk;
