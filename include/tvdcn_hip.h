@@ -306,12 +306,12 @@ tvdcn_status tvdcn_rms_norm_backward(const tvdcn_rms_norm_desc *desc, const void
                                      void *grad_weight, void *workspace, size_t workspace_bytes, void *stream);
 
 /*
- * 8 bits with a scale per row: scale = max(max |x| * (1 / 127), 2^-126) in float32 (at most the
- * largest of which 127 are finite), and codes x / scale rounded to the nearest integer, ties to
- * even (the quotient as if exact). A code stands for code * scale. A row that holds an infinity or a
- * NaN has codes 0 and the scale NaN: it stands for NaN. A weight (out x in) has a scale per output
- * channel so. tvdcn_rms_norm_int8 does this to the normalised row, held in float32. codes: rows x
- * channels; scales: rows, float32.
+ * 8 bits with a scale per row: scale = max(max |x| * (1 / 127), 2^-126), a product of float32 (at most
+ * the last bit off the rounded quotient), at most the largest scale of which 127 are finite, and codes
+ * x / scale rounded to the nearest integer, ties to even (the quotient as if exact). A code stands for
+ * code * scale. A row that holds an infinity or a NaN has codes 0 and the scale NaN: it stands for NaN.
+ * A weight (out x in) has a scale per output channel so. tvdcn_rms_norm_int8 does this to the
+ * normalised row, held in float32. codes: rows x channels; scales: rows, float32.
  */
 tvdcn_status tvdcn_quantize_int8(int32_t dtype, int64_t rows, int64_t channels, const void *input, int8_t *codes,
                                  float *scales, void *stream);
@@ -323,8 +323,8 @@ tvdcn_status tvdcn_rms_norm_int8(const tvdcn_rms_norm_desc *desc, const void *in
 /*
  * The pointwise convolution of 8-bit rows with 8-bit weights:
  * output = act(scale * weight_scale * sum(code * weight_code) + bias) + residual, the sums in whole
- * numbers. The descriptor's dtype is that of output, bias and residual (may be NULL); at most 131071 input
- * channels.
+ * numbers, the scales in an order that overflows only where their result does. The descriptor's dtype
+ * is that of output, bias and residual (may be NULL); at most 131071 input channels.
  */
 size_t tvdcn_pointwise_conv_int8_workspace_size(const tvdcn_pointwise_desc *desc);
 tvdcn_status tvdcn_pointwise_conv_int8(const tvdcn_pointwise_desc *desc, const int8_t *codes, const float *scales,

@@ -5,11 +5,14 @@
 // ones. Channels that are no multiple of 16 are copied to rows that are, with zeros behind them. Small products have a kernel of
 // their own, without copies.
 //
-// 8192 x 8192 to 8192 runs at 2590 TOP/s (a plain library product of 8-bit integers: 2150). With few channels the results bound it:
-// 65536 x 2048 to 512 takes 71 us, 77 with a residual and 83 with gelu, of which 53 are products; 65536 x 512 to 2048 103, 137 and
-// 146. A tile's stores come from all CUs at about the same time, and only the next tile's first stage overlaps them: two workgroups of
-// 256 x 128 to a CU, one storing while the other multiplies, ran at 1920 TOP/s and were slower throughout (the former 89, 106 and
-// 98 us).
+// 8192 x 8192 to 8192 runs at 2590 to 2680 TOP/s (a plain library product of 8-bit integers: 2150). With few channels the results bound
+// it. 65536 x 2048 to 512, 64 us of products at the library's rate: 66-68 us, 71-76 with a residual, 75-78 with gelu; float32 results
+// 77 and 105-108 with a residual (80 of reading and writing). 65536 x 512 to 2048, the same products: 100-104, 137-140 and 141-149;
+// float32 151-156, 258 with a residual (220 of reading and writing), 255-261 with gelu. A tile's stores come from all CUs at about the same
+// time, and only the next tile's first stage overlaps them (none where a float32 residual is read, whose loads are not counted): two
+// workgroups of 256 x 128 to a CU, one storing while the other multiplies, ran at 1920 TOP/s and were slower throughout. Rows that are no
+// whole 16 bytes are copied first: 65536 x 2040 to 512 takes 118-123 us, 65536 x 520 to 2048 135 and 186 with gelu. A reduction is not split
+// over workgroups: 1, 16, 64, 256 and 1024 x 4096 to 4096 take 5, 7, 12, 16 and 43 us, of which 3, 3, 4, 4 and 16 are memory and products.
 #include <cmath>
 
 #include "product_kernels.h"

@@ -20,9 +20,10 @@ def quantize_int8(input: Tensor) -> Tuple[Tensor, Tensor]:
     r"""A (batch, channels, \*size) map in 8 bits: int8 codes of its shape, channels-last, and a float32 scale for every
     pixel, (batch, \*size). A weight (out_channels, in_channels) has a scale for every output channel so.
 
-    ``scale = max(max |x| * (1 / 127), 2**-126)`` in float32 (at most the largest of which 127 are finite), and a code is ``x / scale`` rounded to the nearest integer,
-    ties to even, as if the quotient were exact. A code stands for ``code * scale``. A pixel that holds an infinity or a NaN
-    has the scale NaN. float32, float16 and bfloat16. Not differentiable: a call that would need a gradient raises.
+    ``scale = max(max |x| * (1 / 127), 2**-126)``, the product in float32 with 1 / 127 rounded to it (at most the last bit
+    off the rounded quotient), at most the largest scale of which 127 are finite. A code is ``x / scale`` rounded to the
+    nearest integer, ties to even, as if the quotient were exact. A code stands for ``code * scale``. A pixel that holds an
+    infinity or a NaN has the scale NaN. float32, float16 and bfloat16. Not differentiable: a call that would need a gradient raises.
     """
     if not torch.jit.is_scripting():
         _log_api_usage_once(quantize_int8)
