@@ -23,7 +23,8 @@ def quantize_int8(input: Tensor) -> Tuple[Tensor, Tensor]:
     ``scale = max(max |x| * (1 / 127), 2**-126)``, the product in float32 with 1 / 127 rounded to it (at most the last bit
     off the rounded quotient), at most the largest scale of which 127 are finite. A code is ``x / scale`` rounded to the
     nearest integer, ties to even, as if the quotient were exact. A code stands for ``code * scale``. A pixel that holds an
-    infinity or a NaN has the scale NaN. float32, float16 and bfloat16. Not differentiable: a call that would need a gradient raises.
+    infinity or a NaN has the scale NaN. float32, float16 and bfloat16. Not differentiable: a call that would need a gradient
+    raises.
     """
     if not torch.jit.is_scripting():
         _log_api_usage_once(quantize_int8)
@@ -55,7 +56,8 @@ def pointwise_conv_int8(codes: Tensor, scales: Tensor, weight_codes: Tensor, wei
         dtype: of the result: float32, float16 or bfloat16.
 
     The products are summed exactly; scales, bias, activation and residual are applied in float32 (the scales in an order
-    that overflows only where their result does) and the result is rounded once. Not differentiable: a call that would need a gradient raises.
+    that overflows only where their result does) and the result is rounded once. Not differentiable: a call that would need
+    a gradient raises.
 
     Returns:
         Tensor[batch, out_channels, \*size]: channels-last.
